@@ -1,6 +1,6 @@
 """Cases that measure the attention-layer operators: query/key norm with position
-rotation (forward and backward), attention with a sliding window and sink tokens,
-and attention over a prefix that a whole batch shares.
+rotation, attention with a sliding window and sink tokens (both forward and
+backward), and attention over a prefix that a whole batch shares.
 
 With `own` false, `run` computes an operator in its plain form: elementary torch
 operations in 32 bits (angles and long sums in 64), rounded once at the end.  With
@@ -30,15 +30,13 @@ def listed():
         # A full training/prefill step's tokens, read from the fused projection's output.
         dict(name="norm_rope_4x4096", op="norm_rope", B=4, S=4096, Hq=32, Hkv=8, D=128, R=128,
              interleaved=False, wbits=32, far=4096),
-        # Odd lengths and head counts, head size 64, half of it rotated, adjacent pairs.
-        dict(name="norm_rope_odd", op="norm_rope", B=3, S=517, Hq=10, Hkv=5, D=64, R=32,
-             interleaved=True, wbits=16, far=200000),
-        # The gradients of the training step.
+        # The gradients of that step.
         dict(name="norm_rope_bwd_4x4096", op="norm_rope_bwd", B=4, S=4096, Hq=32, Hkv=8, D=128,
              R=128, interleaved=False, wbits=32, far=4096),
-        # The gradients of a short odd batch: the weights' gradients weigh most here.
-        dict(name="norm_rope_bwd_odd", op="norm_rope_bwd", B=2, S=333, Hq=16, Hkv=16, D=64, R=64,
-             interleaved=True, wbits=16, far=333),
+        # A short odd batch, head size 64, half of it rotated, adjacent pairs: the weights'
+        # gradients weigh most here.
+        dict(name="norm_rope_bwd_odd", op="norm_rope_bwd", B=2, S=333, Hq=10, Hkv=5, D=64, R=32,
+             interleaved=True, wbits=16, far=200000),
         # Prefill of a sliding-window layer.
         dict(name="window_prefill_8192", op="window", B=1, Hq=32, Hkv=8, Sq=8192, Skv=8192, D=128,
              W=1024, sinks=4, lens="full"),
@@ -51,11 +49,14 @@ def listed():
         # A serving batch's tokens over caches longer than the window.
         dict(name="window_decode_64", op="window", B=64, Hq=64, Hkv=8, Sq=1, Skv=8192, D=128,
              W=4096, sinks=4, lens="mixed"),
-        # Two requests behind a short system text: latency.
-        dict(name="prefix_2", op="prefix", B=2, Hq=32, Hkv=8, Sq=1, P=512, S=128, D=128,
-             lens="mixed"),
-        # A head for each query, size 64, an odd batch and prefix.
-        dict(name="prefix_33_odd", op="prefix", B=33, Hq=16, Hkv=16, Sq=1, P=5003, S=300, D=64,
+        # The gradients of a training step's sliding-window layer.
+        dict(name="window_bwd_4096", op="window_bwd", B=2, Hq=32, Hkv=8, Sq=4096, Skv=4096, D=128,
+             W=1024, sinks=4, lens="full"),
+        # A padded batch's chunk: other lengths in each row of it, a head for each query.
+        dict(name="window_bwd_odd", op="window_bwd", B=3, Hq=6, Hkv=6, Sq=777, Skv=1001, D=64,
+             W=300, sinks=5, lens="mixed"),
+        # Three requests behind a short system text: latency.
+        dict(name="prefix_3", op="prefix", B=3, Hq=16, Hkv=4, Sq=1, P=517, S=128, D=64,
              lens="mixed"),
         # A serving batch behind a long document.
         dict(name="prefix_64", op="prefix", B=64, Hq=64, Hkv=8, Sq=1, P=16384, S=1024, D=128,
@@ -69,7 +70,8 @@ def _spread(rng, lo, hi):
 
 
 def draw(rng):
-    op = rng.choice(["norm_rope", "norm_rope_bwd", "window", "window", "prefix"])
+    op = rng.choice(["norm_rope", "norm_rope_bwd", "window", "window", "window_bwd", "prefix",
+                     "prefix"])
     D = rng.choice([64, 128])
     Hkv = rng.choice([1, 2, 3, 4, 8, 16])
     group = rng.choice([1, 1, 2, 3, 4, 5, 8, 16])
@@ -81,16 +83,18 @@ def draw(rng):
         return dict(op=op, B=B, S=S, Hq=Hq, Hkv=Hkv, D=D, R=rng.choice([16, 32, D // 2, D, D]),
                     interleaved=rng.random() < 0.5, wbits=rng.choice([16, 32]),
                     far=_spread(rng, 100, 1000000))
-    if op == "window":
+    if op in ("window", "window_bwd"):
+        back = op == "window_bwd"
         while True:
-            B = _spread(rng, 1, 64)
-            Skv = _spread(rng, 1, 16384)
+            B = _spread(rng, 1, 16 if back else 64)
+            # (With one key the scores' gradients are exact zeros, which says nothing.)
+            Skv = _spread(rng, 32, 8192) if back else _spread(rng, 1, 16384)
             if rng.random() < 0.5:
-                Sq = rng.choice([1, 1, 1, 2, 4, 8])
+                Sq = Skv if back else rng.choice([1, 1, 1, 2, 4, 8])
             else:
                 Sq = _spread(rng, 1, 8192)
             # The dense scores of the plain form, and the caches, within the listed cases'.
-            if (Sq <= Skv and B * Hq * Sq * Skv <= 32 * 8192 * 8192
+            if (Sq <= Skv and B * Hq * Sq * Skv <= (64 * 4096 * 4096 if back else 32 * 8192 * 8192)
                     and B * Hkv * Skv * D <= 64 * 8 * 8192 * 128):
                 break
         W = _spread(rng, 16, 8192)
@@ -151,11 +155,15 @@ def prepare(case, seed):
         return st
     Sq = case["Sq"]
     st["q"] = _normal(g, B, Hq, Sq, D)
-    if case["op"] == "window":
+    if case["op"] in ("window", "window_bwd"):
         st["k"] = _normal(g, B, Hkv, case["Skv"], D)
         st["v"] = _normal(g, B, Hkv, case["Skv"], D)
         # Some rows of a padded batch may be shorter than the queries: their first rows see nothing.
         st["len"] = _lens(case, g, case["Skv"], max(1, case["Skv"] // 2))
+        if case["op"] == "window_bwd":  # what the forward pass left, and the output's gradient
+            st["o"], st["lse"] = _window(st["q"], st["k"], st["v"], st["len"], case["W"],
+                                         case["sinks"])
+            st["do"] = _normal(g, B, Hq, Sq, D, scale=0.5)
     else:
         st["kp"] = _normal(g, Hkv, case["P"], D)
         st["vp"] = _normal(g, Hkv, case["P"], D)
@@ -182,6 +190,9 @@ def run(st):
         if c["op"] == "window":
             return ops.attention_window_fwd(st["q"], st["k"], st["v"], c["W"], c["sinks"],
                                             kv_len=st["len"])
+        if c["op"] == "window_bwd":
+            return ops.attention_window_bwd(st["do"], st["q"], st["k"], st["v"], st["o"],
+                                            st["lse"], c["W"], c["sinks"], kv_len=st["len"])
         return ops.attention_shared_prefix(st["q"], st["kp"], st["vp"], st["k"], st["v"],
                                            kv_len=st["len"])
     if c["op"] == "norm_rope":
@@ -194,7 +205,10 @@ def run(st):
         dk, dwk = _norm_rope_bwd(st["gk"], st["k"], st["wk"], cos, sin, c["interleaved"])
         return dq, dk, dwq, dwk
     if c["op"] == "window":
-        return _window(st["q"], st["k"], st["v"], st["len"], c["W"], c["sinks"])
+        return _window(st["q"], st["k"], st["v"], st["len"], c["W"], c["sinks"])[0]
+    if c["op"] == "window_bwd":
+        return _window_bwd(st["do"], st["q"], st["k"], st["v"], st["o"], st["lse"], st["len"],
+                           c["W"], c["sinks"])
     return _prefix(st["q"], st["kp"], st["vp"], st["k"], st["v"], st["len"])
 
 
@@ -234,24 +248,40 @@ def _norm_rope_bwd(gy, x, w, cos, sin, interleaved):
 
 
 def _softmax(s):
-    """Softmax over the last axis; a row of nothing but -inf gives zeros."""
+    """Softmax over the last axis, and the log of its sum; a row of nothing but -inf gives zeros."""
     m = s.amax(dim=-1, keepdim=True)
     p = torch.exp(s - torch.where(m == NEG, torch.zeros_like(m), m))
-    return p / p.sum(dim=-1, keepdim=True).clamp_min(1e-30)
+    t = p.sum(dim=-1, keepdim=True)
+    return p / t.clamp_min(1e-30), m + torch.log(t)
 
 
-def _window(q, k, v, lens, W, sinks):
+def _scores(q, k, lens, W, sinks):
+    """The scaled scores [B, Hkv, group * Sq, Skv], -inf where a query does not see a key."""
     B, Hq, Sq, D = q.shape
     Hkv, Skv = k.shape[1], k.shape[2]
     s = q.to(F32).reshape(B, Hkv, Hq // Hkv * Sq, D) @ k.to(F32).transpose(-1, -2)
     s = (s / math.sqrt(D)).reshape(B, Hkv, Hq // Hkv, Sq, Skv)
-    lens = lens.long()
-    i = lens[:, None] - Sq + torch.arange(Sq, device=q.device)  # the queries' positions
+    i = lens.long()[:, None] - Sq + torch.arange(Sq, device=q.device)  # the queries' positions
     j = torch.arange(Skv, device=q.device)
     seen = (j <= i[..., None]) & ((i[..., None] - j < W) | (j < sinks))
-    p = _softmax(s.masked_fill(~seen[:, None, None], NEG))
-    o = p.reshape(B, Hkv, Hq // Hkv * Sq, Skv) @ v.to(F32)
-    return o.reshape(B, Hq, Sq, D).to(BF16)
+    return s.masked_fill(~seen[:, None, None], NEG).reshape(B, Hkv, Hq // Hkv * Sq, Skv)
+
+
+def _window(q, k, v, lens, W, sinks):
+    p, lse = _softmax(_scores(q, k, lens, W, sinks))
+    return (p @ v.to(F32)).reshape(q.shape).to(BF16), lse.reshape(q.shape[:3])
+
+
+def _window_bwd(do, q, k, v, o, lse, lens, W, sinks):
+    B, Hkv, D = q.shape[0], k.shape[1], q.shape[3]
+    s = _scores(q, k, lens, W, sinks)
+    p = torch.exp(s - lse.reshape(B, Hkv, -1, 1).clamp_min(-1e30))
+    do, o, qf = (t.to(F32).reshape(B, Hkv, -1, D) for t in (do, o, q))
+    ds = p * (do @ v.to(F32).transpose(-1, -2) - (do * o).sum(dim=-1, keepdim=True))
+    ds = ds / math.sqrt(D)
+    dq = (ds @ k.to(F32)).reshape(q.shape)
+    dk, dv = ds.transpose(-1, -2) @ qf, p.transpose(-1, -2) @ do
+    return dq.to(BF16), dk.to(BF16), dv.to(BF16)
 
 
 def _prefix(q, kp, vp, k, v, lens):
@@ -264,7 +294,7 @@ def _prefix(q, kp, vp, k, v, lens):
     i = lens.long()[:, None] - Sq + torch.arange(Sq, device=q.device)
     seen = torch.arange(S, device=q.device) <= i[..., None]
     own_s = own_s.reshape(B, Hkv, Hq // Hkv, Sq, S).masked_fill(~seen[:, None, None], NEG)
-    p = _softmax(torch.cat((shared, own_s.reshape(B, Hkv, rows, S)), dim=-1) / math.sqrt(D))
+    p, _ = _softmax(torch.cat((shared, own_s.reshape(B, Hkv, rows, S)), dim=-1) / math.sqrt(D))
     pp = p[..., :P].transpose(0, 1).reshape(Hkv, B * rows, P) @ vp.to(F32)
     o = pp.reshape(Hkv, B, rows, D).transpose(0, 1) + p[..., P:] @ v.to(F32)
     return o.reshape(B, Hq, Sq, D).to(BF16)
@@ -292,9 +322,12 @@ def work(case):
             return {"bytes": 4 * n + small, "flops": 8 * n}
         return {"bytes": 6 * n + small + 8 * D, "flops": 16 * n}
     Sq = case["Sq"]
-    if case["op"] == "window":
+    if case["op"] in ("window", "window_bwd"):
         n = case["Skv"] if case["lens"] == "full" else (max(1, case["Skv"] // 2) + case["Skv"]) // 2
         pairs, keys = _seen(n, Sq, case["W"], case["sinks"])
+        if case["op"] == "window_bwd":  # q, o, do, dq; k, v, dk, dv; the row sums
+            return {"bytes": 8 * B * Hq * Sq * D + 4 * B * Hkv * (keys + case["Skv"]) * D
+                    + 4 * B * Hq * Sq + 4 * B, "flops": 10 * B * Hq * pairs * D}
         return {"bytes": 4 * B * Hq * Sq * D + 4 * B * Hkv * keys * D + 4 * B,
                 "flops": 4 * B * Hq * pairs * D}
     n = case["S"] if case["lens"] == "full" else (min(Sq, case["S"]) + case["S"]) // 2
@@ -337,23 +370,31 @@ def exact(case, seed):
     q, k, v = st["q"], st["k"], st["v"]
     B, Hq, Sq, D = q.shape
     group, lens = Hq // k.shape[1], st["len"].tolist()
-    out = torch.zeros((B, Hq, Sq, D), dtype=F64, device="cuda")
+    back = case["op"] == "window_bwd"
+    out = torch.zeros((B, Hq, Sq, D), dtype=F64, device="cuda")  # o, or dq
+    dk, dv = (torch.zeros(k.shape, dtype=F64, device="cuda") if back else None for _ in range(2))
     for b in range(B):
         n = lens[b]
         t = torch.arange(n - Sq, n, device="cuda").unsqueeze(1)
         j = torch.arange(n, device="cuda").unsqueeze(0)
         hide = j > t
-        if case["op"] == "window":
+        if case["op"] != "prefix":
             hide = hide | ((t - j >= case["W"]) & (j >= case["sinks"]))
         for h in range(k.shape[1]):
-            qh = q[b, h * group:(h + 1) * group].double() * D ** -0.5
-            kh, vh, mask = k[b, h, :n].double(), v[b, h, :n].double(), hide
+            heads = slice(h * group, (h + 1) * group)
+            qh, kh, vh = q[b, heads].double(), k[b, h, :n].double(), v[b, h, :n].double()
+            mask = hide
             if case["op"] == "prefix":
                 kh = torch.cat((st["kp"][h].double(), kh))
                 vh = torch.cat((st["vp"][h].double(), vh))
                 mask = torch.cat((hide.new_zeros(Sq, case["P"]), hide), dim=1)
-            s = torch.einsum("gsd,nd->gsn", qh, kh).masked_fill(mask, NEG)
-            lse = torch.logsumexp(s, dim=-1, keepdim=True)
-            p = torch.where(lse == NEG, torch.zeros_like(s), torch.exp(s - lse))
-            out[b, h * group:(h + 1) * group] = p @ vh
-    return out
+            leaves = [x.requires_grad_(back) for x in (qh, kh, vh)]
+            s = torch.einsum("gsd,nd->gsn", qh * D ** -0.5, kh).masked_fill(mask, NEG)
+            dead = mask.all(dim=-1, keepdim=True)
+            o = torch.softmax(s.masked_fill(dead, 0.0), dim=-1).masked_fill(dead, 0.0) @ vh
+            if back:
+                out[b, heads], dk[b, h, :n], dv[b, h, :n] = torch.autograd.grad(
+                    o, leaves, st["do"][b, heads].double())
+            else:
+                out[b, heads] = o
+    return (out, dk, dv) if back else out
