@@ -32,6 +32,19 @@ _f = ctypes.c_float
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint32
 
+_i64 = ctypes.c_int64
+_sz = ctypes.c_size_t
+
+
+class Tensor(ctypes.Structure):
+    """b200_tensor: a [B, H, S, D] tensor by its element strides."""
+
+    _fields_ = [("data", _vp), ("stride_b", _i64), ("stride_h", _i64), ("stride_s", _i64)]
+
+
+_t = ctypes.POINTER(Tensor)
+_szp = ctypes.POINTER(_sz)
+
 _PROTOTYPES = {
     "attention_fwd": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp],
     "attention_fwd_trace": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _i,
@@ -47,6 +60,20 @@ _PROTOTYPES = {
     "gemm_bf16_cublas": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
     "gemm_f32_reference": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
     "gemm_cublas_mode": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
+    "qk_norm_rope": [_t, _t, _vp, _vp, _i, _vp, _i, _i, _vp, _i64, _f, _t, _t, _i, _i, _i, _i, _i,
+                     _vp],
+    "qk_norm_rope_bwd_workspace": [_i, _i, _i, _szp],
+    "qk_norm_rope_bwd": [_t, _t, _t, _t, _vp, _vp, _i, _vp, _i, _i, _vp, _i64, _f, _t, _t, _vp,
+                         _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp],
+    "attention_window_fwd_workspace": [_i, _i, _i, _i, _i, _i, _i, _i, _szp],
+    "attention_window_fwd": [_t, _t, _t, _t, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
+                             _sz, _vp],
+    "attention_window_bwd_workspace": [_i, _i, _i, _szp],
+    "attention_window_bwd": [_t, _t, _t, _t, _t, _vp, _t, _t, _t, _vp, _i, _i, _i, _i, _i, _i, _i,
+                             _i, _f, _vp, _sz, _vp],
+    "attention_shared_prefix_workspace": [_i, _i, _i, _i, _i, _i, _i, _szp],
+    "attention_shared_prefix": [_t, _t, _t, _t, _t, _t, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
+                                _sz, _vp],
     "b200_fill_cublas_pattern": [_vp, _u64, _i, _f, _vp],
 }
 

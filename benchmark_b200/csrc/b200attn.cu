@@ -19,6 +19,9 @@
 #include "attention_pair_kernel.cuh"
 #include "reference_kernels.cuh"
 #include "gemm_kernel.cuh"
+#include "norm_rope_kernel.cuh"
+#include "split_attention_kernel.cuh"
+#include "window_bwd_kernel.cuh"
 
 #include <cublas_v2.h>
 #include <cuda_bf16.h>
@@ -991,3 +994,5 @@ extern "C" b200_status gemm_f32_reference(const void* A, const void* Bm, void* C
   if (e != cudaSuccess) return cuda_fail(e, "gemm_f32_reference launch");
   return B200_OK;
 }
+
+#include "layer_ops.cuh"

@@ -1,5 +1,6 @@
 /*
- * b200attn -- C ABI of the sm_100a fused attention forward and bf16 GEMM.
+ * b200attn -- C ABI of the sm_100a fused attention forward, the attention
+ * layer's operators around it, and bf16 GEMM.
  *
  * The reference (rhrnald/benchmark) has no library boundary: its harness
  * launches kernels directly.  Each entry point below replaces one such launch
@@ -126,6 +127,113 @@ b200_status attention_fwd_trace(const void* q, const void* k, const void* v, voi
 b200_status attention_fwd_scalar(const void* q, const void* k, const void* v, void* o, int B,
                                  int Hq, int Hkv, int Sq, int Skv, int D, int causal,
                                  float softmax_scale, b200_stream_t stream);
+
+/*
+ * A [B, H, S, D] bf16 tensor by its strides in elements; D is contiguous.
+ * The data is 16-byte aligned and the strides are multiples of 8, so a view
+ * of a fused projection's [B, S, heads, D] output, or of a cache with room
+ * for more tokens, is a tensor.  The stride of an axis of length 1 is not
+ * used.  An input's stride may be 0 (broadcast); the rows of an output may not
+ * overlap, and an output overlaps an input only where an entry point allows it.
+ */
+typedef struct {
+  const void* data;
+  int64_t stride_b, stride_h, stride_s;
+} b200_tensor;
+
+/*
+ * Norm of each query and key head, and rotation by position, in one pass:
+ *   y = R(pos) (x r w),  r = (mean(x^2) + eps)^-1/2  over the D columns.
+ * R turns pair i < rotary_dim/2 by positions * inv_freq[i] radians: columns
+ * (i, i + rotary_dim/2), or (2i, 2i + 1) if interleaved; columns from
+ * rotary_dim on are only normalised.  The angle is formed in 64 bits.
+ *   q, q_out: [B, Hq, S, D]   k, k_out: [B, Hkv, S, D]   D in {64, 128}
+ *   q_weight, k_weight: [D], bf16 or (weight_f32) fp32
+ *   inv_freq: [rotary_dim/2]; rotary_dim a multiple of 16, 0..D
+ *   positions[b * position_stride_b + s]; stride 0 shares them over the batch
+ * An output may be its own input (same data and strides).
+ */
+b200_status qk_norm_rope(const b200_tensor* q, const b200_tensor* k, const void* q_weight,
+                         const void* k_weight, int weight_f32, const float* inv_freq,
+                         int rotary_dim, int interleaved, const int32_t* positions,
+                         int64_t position_stride_b, float eps, const b200_tensor* q_out,
+                         const b200_tensor* k_out, int B, int S, int Hq, int Hkv, int D,
+                         b200_stream_t stream);
+
+/*
+ * Its gradients: dq and dk from dq_out and dk_out (the gradients of q_out and
+ * k_out) and the inputs of the forward call; dq_weight and dk_weight, [D]
+ * fp32, are sums over all rows, in an order that does not change between
+ * calls.  dq may be dq_out, and dk may be dk_out (same data and strides).
+ * Every call writes the workspace; calls that may overlap on the GPU need
+ * one each.
+ */
+b200_status qk_norm_rope_bwd_workspace(int B, int S, int D, size_t* bytes);
+b200_status qk_norm_rope_bwd(const b200_tensor* dq_out, const b200_tensor* dk_out,
+                             const b200_tensor* q, const b200_tensor* k, const void* q_weight,
+                             const void* k_weight, int weight_f32, const float* inv_freq,
+                             int rotary_dim, int interleaved, const int32_t* positions,
+                             int64_t position_stride_b, float eps, const b200_tensor* dq,
+                             const b200_tensor* dk, float* dq_weight, float* dk_weight, int B,
+                             int S, int Hq, int Hkv, int D, void* workspace,
+                             size_t workspace_bytes, b200_stream_t stream);
+
+/*
+ * Attention with a sliding window and sinks.  Request b has kv_len[b] keys
+ * (clamped to 0..Skv; null: Skv each); its queries are the last Sq positions,
+ * query i at p = kv_len[b] - Sq + i.  It sees key j iff
+ *   j <= p  and  (p - j < window  or  j < sinks).
+ * A query before the first key (p < 0) sees nothing and gives zeros.  K and V
+ * rows that no query of the call sees are not used, whatever they hold.
+ *   q, o: [B, Hq, Sq, D]   k, v: [B, Hkv, Skv, D]   D in {64, 128}
+ *   window >= 1 (INT_MAX: causal attention), sinks >= 0
+ *   softmax_scale < 0 selects 1/sqrt(D)
+ *   lse: null, or [B, Hq, Sq] fp32 contiguous: the log of each row's sum of
+ *   exponentials, -inf for a row that sees nothing (attention_window_bwd
+ *   reads it)
+ * Sq = 1 is a decoding step; short queries split the keys among CTAs and need
+ * a workspace, whose size attention_window_fwd_workspace gives for the
+ * current device (0: none).  Calls that may overlap on the GPU need one each.
+ */
+b200_status attention_window_fwd_workspace(int B, int Hq, int Hkv, int Sq, int Skv, int D,
+                                           int window, int sinks, size_t* bytes);
+b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, const b200_tensor* v,
+                                 const b200_tensor* o, float* lse, const int32_t* kv_len, int B,
+                                 int Hq, int Hkv, int Sq, int Skv, int D, int window, int sinks,
+                                 float softmax_scale, void* workspace, size_t workspace_bytes,
+                                 b200_stream_t stream);
+
+/*
+ * Gradients of attention_window_fwd: dq, dk and dv from dout (the gradient of
+ * o), the forward call's q, k, v and arguments, and its o and lse.  dk and dv
+ * sum over the query heads that share a key and are written whole (zeros for
+ * keys that no query sees).  No atomics: equal calls give equal bits.
+ */
+b200_status attention_window_bwd_workspace(int B, int Hq, int Sq, size_t* bytes);
+b200_status attention_window_bwd(const b200_tensor* dout, const b200_tensor* q,
+                                 const b200_tensor* k, const b200_tensor* v, const b200_tensor* o,
+                                 const float* lse, const b200_tensor* dq, const b200_tensor* dk,
+                                 const b200_tensor* dv, const int32_t* kv_len, int B, int Hq,
+                                 int Hkv, int Sq, int Skv, int D, int window, int sinks,
+                                 float softmax_scale, void* workspace, size_t workspace_bytes,
+                                 b200_stream_t stream);
+
+/*
+ * Attention of a batch whose requests share a prefix: query i of request b
+ * sees all P prefix keys, and of its own keys those at j <= kv_len[b] - Sq + i
+ * (kv_len as above, of at most S).  The prefix is read for the whole batch at
+ * once, not for each request.
+ *   q, o: [B, Hq, Sq, D]   k_prefix, v_prefix: [1, Hkv, P, D] (P = 0: ignored)
+ *   k, v: [B, Hkv, S, D]   D in {64, 128}
+ */
+b200_status attention_shared_prefix_workspace(int B, int Hq, int Hkv, int Sq, int P, int S, int D,
+                                              size_t* bytes);
+b200_status attention_shared_prefix(const b200_tensor* q, const b200_tensor* k_prefix,
+                                    const b200_tensor* v_prefix, const b200_tensor* k,
+                                    const b200_tensor* v, const b200_tensor* o,
+                                    const int32_t* kv_len, int B, int Hq, int Hkv, int Sq, int P,
+                                    int S, int D, float softmax_scale, void* workspace,
+                                    size_t workspace_bytes, b200_stream_t stream);
 
 /*
  * bf16 GEMM: C[M,N] (bf16, row-major) = A[M,K] (row-major) x B, fp32

@@ -1,0 +1,463 @@
+"""GPU tests of the attention layer's operators against their plain 64-bit forms
+(layer_util, which derives the tolerances)."""
+import math
+
+import pytest
+import torch
+
+import layer_util as U
+from benchmark_b200 import ops
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+NAN = float("nan")
+
+
+def randn(g, *shape, scale=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(BF16)
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ---------------------------------------------------------------------------
+# qk_norm_rope
+# ---------------------------------------------------------------------------
+def rope_inputs(B, S, Hq, Hkv, D, R, w32, far=100000, seed=0):
+    g = gen(seed)
+    qkv = randn(g, B, S, Hq + 2 * Hkv, D, scale=2.0)
+    q, k = qkv[:, :, :Hq].transpose(1, 2), qkv[:, :, Hq:Hq + Hkv].transpose(1, 2)
+    wt = torch.float32 if w32 else BF16
+    wq, wk = (torch.randn(D, generator=g, device="cuda").to(wt) for _ in range(2))
+    freq = (10000.0 ** (-torch.arange(R // 2, device="cuda") * 2.0 / max(R, 1))).float()
+    pos = torch.randint(0, far, (B, S), generator=g, device="cuda", dtype=torch.int32)
+    return q, k, wq, wk, freq, pos
+
+
+ROPE = [  # B, S, Hq, Hkv, D, R, interleaved, w32
+    (1, 1, 1, 1, 128, 128, False, False),
+    (1, 1, 32, 8, 128, 128, False, True),
+    (2, 5, 3, 1, 64, 64, True, False),
+    (3, 517, 10, 5, 64, 32, True, True),
+    (2, 333, 7, 7, 128, 48, False, False),
+    (1, 9000, 1, 1, 64, 16, False, True),
+    (4, 2100, 5, 2, 128, 16, True, False),
+    (1, 40, 64, 8, 128, 0, False, False),
+    (2, 4500, 32, 8, 128, 128, False, True),
+]
+
+
+@pytest.mark.parametrize("B,S,Hq,Hkv,D,R,il,w32", ROPE)
+def test_norm_rope(B, S, Hq, Hkv, D, R, il, w32):
+    q, k, wq, wk, freq, pos = rope_inputs(B, S, Hq, Hkv, D, R, w32)
+    qo, ko = ops.qk_norm_rope(q, k, wq, wk, freq, pos, eps=1e-5, interleaved=il)
+    angles = U.rope_angles(pos, freq, B)
+    assert qo.is_contiguous() and ko.is_contiguous()
+    U.check_close(qo, *U.norm_rope(q, wq, angles, 1e-5, il), "q")
+    U.check_close(ko, *U.norm_rope(k, wk, angles, 1e-5, il), "k")
+
+
+@pytest.mark.parametrize("B,S,Hq,Hkv,D,R,il,w32", ROPE)
+def test_norm_rope_bwd(B, S, Hq, Hkv, D, R, il, w32):
+    q, k, wq, wk, freq, pos = rope_inputs(B, S, Hq, Hkv, D, R, w32, seed=1)
+    g = gen(2)
+    gq, gk = randn(g, B, Hq, S, D), randn(g, B, S, Hkv, D).transpose(1, 2)
+    got = ops.qk_norm_rope_bwd(gq, gk, q, k, wq, wk, freq, pos, eps=1e-5, interleaved=il)
+    again = ops.qk_norm_rope_bwd(gq, gk, q, k, wq, wk, freq, pos, eps=1e-5, interleaved=il)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    angles = U.rope_angles(pos, freq, B)
+    for x, w, gy, dx, dw, n in ((q, wq, gq, got[0], got[2], "q"), (k, wk, gk, got[1], got[3], "k")):
+        ref = U.norm_rope_bwd(gy, x, w, angles, 1e-5, il)
+        U.check_close(dx, *ref[:2], "d" + n)
+        U.check_close(dw, *ref[2:], f"d{n}_weight")
+
+
+def test_norm_rope_far_and_negative_positions_and_shared_ones():
+    q, k, wq, wk, freq, _ = rope_inputs(3, 6, 4, 2, 128, 128, True)
+    for p in ([0, 1, -1, 2 ** 31 - 1, -2 ** 31, 1 << 20], [7, 7, 7, 0, 0, 123456789]):
+        qo, ko = ops.qk_norm_rope(q, k, wq, wk, freq, i32(p))
+        angles = U.rope_angles(i32(p), freq, 3)
+        U.check_close(qo, *U.norm_rope(q, wq, angles, 1e-6, False), "q")
+        U.check_close(ko, *U.norm_rope(k, wk, angles, 1e-6, False), "k")
+
+
+def test_norm_rope_in_place_and_into_a_cache():
+    q, k, wq, wk, freq, pos = rope_inputs(2, 130, 8, 2, 128, 64, False)
+    want = ops.qk_norm_rope(q, k, wq, wk, freq, pos)
+    cache = torch.full((2, 2, 400, 128), 7.0, dtype=BF16, device="cuda")
+    q2 = q.clone(memory_format=torch.preserve_format)
+    qo, ko = ops.qk_norm_rope(q2, k, wq, wk, freq, pos, q_out=q2, k_out=cache[:, :, 100:230])
+    assert qo is q2 and torch.equal(q2, want[0]) and torch.equal(cache[:, :, 100:230], want[1])
+    assert (cache[:, :, :100] == 7).all() and (cache[:, :, 230:] == 7).all()
+    g = randn(gen(3), 2, 8, 130, 128)
+    gk = randn(gen(4), 2, 2, 130, 128)
+    want = ops.qk_norm_rope_bwd(g, gk, q, k, wq, wk, freq, pos)
+    got = ops.qk_norm_rope_bwd(g, gk, q, k, wq, wk, freq, pos, dq=g, dk=gk)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is g
+
+
+def test_norm_rope_zero_and_tiny_rows():
+    """A row of zeros gives zeros (eps), rows near the type's smallest values stay exact."""
+    q, k, wq, wk, freq, pos = rope_inputs(1, 4, 2, 2, 64, 64, True)
+    q = q.clone()
+    q[:, :, 0] = 0
+    q[:, :, 1] *= 1e-30
+    qo, _ = ops.qk_norm_rope(q, k, wq, wk, freq, pos)
+    angles = U.rope_angles(pos, freq, 1)
+    assert (qo[:, :, 0] == 0).all()
+    U.check_close(qo, *U.norm_rope(q, wq, angles, 1e-6, False), "q")
+
+
+def test_norm_rope_gradient_is_the_difference_of_its_plain_form():
+    q, k, wq, wk, freq, pos = rope_inputs(2, 9, 3, 2, 64, 32, True, seed=5)
+    g = gen(6)
+    gq, gk = randn(g, 2, 3, 9, 64), randn(g, 2, 2, 9, 64)
+    dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(gq, gk, q, k, wq, wk, freq, pos)
+    angles, h = U.rope_angles(pos, freq, 2), 1e-6
+    for x, w, gy, dx, dw in ((q, wq, gq, dq, dwq), (k, wk, gk, dk, dwk)):
+        x, w, gy = x.double(), w.double(), gy.double()
+        ux, uw = (torch.randn(t.shape, generator=g, device="cuda", dtype=U.F64) for t in (x, w))
+        y = [U.norm_rope(x + s * h * ux, w + s * h * uw, angles, 1e-6, False)[0] for s in (1, -1)]
+        diff = ((y[0] - y[1]) * gy).sum() / (2 * h)
+        terms = (dx.double() * ux).abs().sum() + (dw.double() * uw).abs().sum()
+        got = (dx.double() * ux).sum() + (dw.double() * uw).sum()
+        assert (got - diff).abs() <= U.BF16_STEP * terms
+
+
+# ---------------------------------------------------------------------------
+# attention_window
+# ---------------------------------------------------------------------------
+WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks, lens
+    (1, 1, 1, 1, 1, 128, 1, 0, None),
+    (1, 4, 2, 1, 300, 64, 16, 0, None),
+    (2, 8, 1, 1, 1000, 128, 256, 4, [1000, 3]),
+    (3, 6, 2, 1, 2049, 128, 1 << 40, 0, [2049, 0, 1]),
+    (2, 32, 8, 1, 5000, 128, 1024, 130, [5000, 1100]),
+    (4, 10, 2, 3, 700, 64, 100, 5, [700, 2, 101, 0]),
+    (1, 16, 1, 8, 513, 128, 64, 64, None),
+    (2, 5, 5, 17, 40, 128, 7, 2, [40, 17]),
+    (1, 2, 1, 127, 127, 128, 50, 3, None),
+    (1, 2, 2, 128, 128, 64, 128, 0, None),
+    (2, 4, 2, 129, 300, 128, 1, 1, [300, 131]),
+    (2, 6, 3, 333, 517, 128, 128, 4, [517, 200]),
+    (1, 3, 1, 700, 1500, 64, 300, 150, None),
+    (3, 4, 4, 260, 1000, 128, 1 << 40, 0, [1000, 260, 17]),
+    (1, 8, 2, 1111, 1111, 128, 256, 128, None),
+    (2, 4, 1, 515, 515, 64, 100, 500, [515, 300]),
+    (1, 2, 1, 1024, 4096, 128, 2000, 1000, None),
+]
+
+
+def window_inputs(B, Hq, Hkv, Sq, Skv, D, W, sinks, lens, seed=0, poison=True):
+    """q, k, v with NaN and infinity wherever nothing may look, lens, visibility."""
+    g = gen(seed)
+    q, k, v = randn(g, B, Hq, Sq, D), randn(g, B, Hkv, Skv, D), randn(g, B, Hkv, Skv, D)
+    n = i32(lens) if lens is not None else None
+    seen = U.visible(torch.full((B,), Skv, device="cuda") if n is None else n, Sq, Skv, W, sinks,
+                     "cuda")
+    if poison:
+        unused = ~seen.any(2).unsqueeze(-1)
+        k = torch.where(unused, torch.tensor(NAN, dtype=BF16, device="cuda"), k)
+        v = torch.where(unused, torch.tensor(math.inf, dtype=BF16, device="cuda"), v)
+        v = torch.where(unused & (torch.arange(Skv, device="cuda") % 2 == 0)[:, None],
+                        torch.tensor(NAN, dtype=BF16, device="cuda"), v)
+        q = torch.where(seen.any(-1, keepdim=True), q,
+                        torch.tensor(NAN, dtype=BF16, device="cuda"))
+    return q, k, v, n, seen
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=str)
+def test_window_fwd(case):
+    B, Hq, Hkv, Sq, Skv, D, W, sinks, lens = case
+    q, k, v, n, seen = window_inputs(*case)
+    lse = torch.full((B, Hq, Sq), 5.0, device="cuda")
+    o = ops.attention_window_fwd(q, k, v, W, sinks, kv_len=n, lse=lse)
+    ops.check()
+    want, bound, want_lse, lse_bound = U.attention(q, k, v, seen)
+    U.check_close(o, want, bound, "o")
+    dead = ~seen.any(-1).expand(B, Hq, Sq)
+    assert (o[dead] == 0).all() and (lse[dead] == -math.inf).all()
+    assert (lse[~dead] - want_lse[~dead]).abs().max() <= lse_bound[~dead].max()
+    again = ops.attention_window_fwd(q, k, v, W, sinks, kv_len=n)
+    assert torch.equal(o, again)
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=str)
+def test_window_bwd(case):
+    q, k, v, n, seen = window_inputs(*case, seed=1)
+    B, Hq, Hkv, Sq, Skv, D, W, sinks, _ = case
+    do = randn(gen(2), B, Hq, Sq, D)
+    do = torch.where(seen.any(-1, keepdim=True), do, torch.tensor(NAN, dtype=BF16, device="cuda"))
+    lse = torch.empty((B, Hq, Sq), device="cuda")
+    o = ops.attention_window_fwd(q, k, v, W, sinks, kv_len=n, lse=lse)
+    got = ops.attention_window_bwd(do, q, k, v, o, lse, W, sinks, kv_len=n)
+    ops.check()
+    want = U.attention_bwd(do, q, k, v, o, lse, seen)
+    for name, a, (w, bound) in zip(("dq", "dk", "dv"), got, want):
+        U.check_close(a, w, bound, name)
+    again = ops.attention_window_bwd(do, q, k, v, o, lse, W, sinks, kv_len=n)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("Sq", [1, 40, 300])
+def test_window_strides(Sq):
+    """[B, S, H, D] storage, a cache with room, heads that share one K by stride 0, an
+    output inside a larger buffer whose other rows stay as they were."""
+    g = gen(3)
+    B, Hq, Hkv, Skv, D, W, sinks = 2, 4, 2, 700, 128, 200, 3
+    q = randn(g, B, Sq, Hq, D).transpose(1, 2)
+    k = randn(g, B, 1, 900, D)[:, :, 50:50 + Skv].expand(B, Hkv, Skv, D)
+    v = randn(g, 1, Skv, Hkv, D).transpose(1, 2).expand(B, Hkv, Skv, D)
+    out = torch.full((B, Sq + 9, Hq, D), 3.0, dtype=BF16, device="cuda")
+    view = out[:, :Sq].transpose(1, 2)
+    seen = U.visible(i32([Skv] * B), Sq, Skv, W, sinks, "cuda")
+    ops.attention_window_fwd(q, k, v, W, sinks, out=view)
+    ops.check()
+    U.check_close(view, *U.attention(q, k, v, seen)[:2], "o")
+    assert (out[:, Sq:] == 3).all()
+    lse = torch.empty((B, Hq, Sq), device="cuda")
+    o = ops.attention_window_fwd(q, k, v, W, sinks, lse=lse)
+    do = randn(g, B, Sq, Hq, D).transpose(1, 2)
+    kv = torch.full((2, B, Skv, 2 * Hkv, D), 3.0, dtype=BF16, device="cuda")
+    dk, dv = (t[:, :, :Hkv].transpose(1, 2) for t in kv)
+    got = ops.attention_window_bwd(do, q, k, v, o, lse, W, sinks, dk=dk, dv=dv)
+    ops.check()
+    for name, a, (w, bound) in zip(("dq", "dk", "dv"), got,
+                                   U.attention_bwd(do, q, k, v, o, lse, seen)):
+        U.check_close(a, w, bound, name)
+    assert (kv[:, :, :, Hkv:] == 3).all()
+
+
+@pytest.mark.parametrize("Sq,scale", [(1, 0.0), (200, 0.0), (1, 0.3), (200, 1.5)])
+def test_window_scales(Sq, scale):
+    q, k, v, n, seen = window_inputs(2, 4, 2, Sq, 400, 128, 150, 2, [400, 350], seed=4)
+    lse = torch.empty((2, 4, Sq), device="cuda")
+    o = ops.attention_window_fwd(q, k, v, 150, 2, kv_len=n, softmax_scale=scale, lse=lse)
+    ops.check()
+    U.check_close(o, *U.attention(q, k, v, seen, scale)[:2], "o")
+    do = randn(gen(5), *q.shape)
+    got = ops.attention_window_bwd(do, q, k, v, o, lse, 150, 2, kv_len=n, softmax_scale=scale)
+    ops.check()
+    for a, (w, bound) in zip(got, U.attention_bwd(do, q, k, v, o, lse, seen, scale)):
+        U.check_close(a, w, bound, "gradient")
+
+
+@pytest.mark.parametrize("Sq", [1, 300])
+def test_window_large_scores(Sq):
+    """Rising scores, so that the running maximum moves at every block."""
+    g = gen(6)
+    q = randn(g, 1, 2, Sq, 64, scale=4.0).abs()
+    ramp = torch.linspace(0.01, 8.0, 900, device="cuda")[:, None]
+    k = (ramp * (1 + 0.01 * torch.randn(1, 1, 900, 64, generator=g, device="cuda"))).to(BF16)
+    v = randn(g, 1, 1, 900, 64)
+    seen = U.visible(i32([900]), Sq, 900, 500, 20, "cuda")
+    o = ops.attention_window_fwd(q, k, v, 500, 20)
+    ops.check()
+    U.check_close(o, *U.attention(q, k, v, seen)[:2], "o")
+
+
+def test_window_lengths_outside_the_cache_are_clamped():
+    q, k, v, _, _ = window_inputs(2, 4, 2, 5, 100, 64, 30, 2, None, poison=False)
+    got = ops.attention_window_fwd(q, k, v, 30, 2, kv_len=i32([1 << 30, -5]))
+    want = ops.attention_window_fwd(q, k, v, 30, 2, kv_len=i32([100, 0]))
+    ops.check()
+    assert torch.equal(got, want) and (got[1] == 0).all()
+
+
+def test_window_offsets_past_32_bits():
+    """One head's cache of more than 2^31 elements; the window lies behind them."""
+    n, D = (1 << 24) + 300, 128
+    kv = torch.zeros((1, 1, n, D), dtype=BF16, device="cuda")
+    kv[:, :, -1000:] = randn(gen(7), 1, 1, 1000, D)
+    kv[:, :, :8] = randn(gen(8), 1, 1, 8, D)
+    for Sq in (1, 200):
+        q = randn(gen(9), 1, 2, Sq, D)
+        o = ops.attention_window_fwd(q, kv, kv, 500, 8)
+        ops.check()
+        # The same keys in a short cache: the window's reach and the sinks before it.
+        short = torch.cat((kv[:, :, :8], kv[:, :, -1000:]), dim=2)
+        seen = U.visible(i32([1008]), Sq, 1008, 500, 8, "cuda")
+        U.check_close(o, *U.attention(q, short, short, seen)[:2], f"Sq {Sq}")
+
+
+# ---------------------------------------------------------------------------
+# attention_shared_prefix
+# ---------------------------------------------------------------------------
+PREFIX = [  # B, Hq, Hkv, Sq, P, S, D, lens
+    (1, 1, 1, 1, 1, 1, 128, None),
+    (1, 4, 4, 1, 0, 50, 64, None),
+    (2, 32, 8, 1, 512, 128, 128, [128, 1]),
+    (3, 16, 4, 1, 517, 128, 64, [0, 70, 128]),
+    (33, 16, 16, 1, 1003, 300, 64, None),
+    (17, 10, 2, 3, 700, 40, 128, None),
+    (5, 16, 1, 4, 129, 2000, 128, [2000, 0, 3, 1500, 64]),
+    (70, 8, 2, 1, 3001, 5, 128, None),
+    (2, 48, 16, 2, 127, 9, 64, [9, 2]),
+]
+
+
+@pytest.mark.parametrize("case", PREFIX, ids=str)
+def test_shared_prefix(case):
+    B, Hq, Hkv, Sq, P, S, D, lens = case
+    g = gen(10)
+    q, kp, vp = randn(g, B, Hq, Sq, D), randn(g, Hkv, P, D), randn(g, Hkv, P, D)
+    n = i32(lens) if lens else torch.randint(0, S + 1, (B,), generator=g, device="cuda",
+                                             dtype=torch.int32)
+    k, v = randn(g, B, Hkv, S, D), randn(g, B, Hkv, S, D)
+    past = (torch.arange(S, device="cuda")[None, :] >= n[:, None])[:, None, :, None]
+    k = torch.where(past, torch.tensor(NAN, dtype=BF16, device="cuda"), k)
+    v = torch.where(past, torch.tensor(math.inf, dtype=BF16, device="cuda"), v)
+    o = ops.attention_shared_prefix(q, kp, vp, k, v, kv_len=n)
+    ops.check()
+    U.check_close(o, *U.shared_prefix(q, kp, vp, k, v, n), "o")
+    assert torch.equal(o, ops.attention_shared_prefix(q, kp, vp, k, v, kv_len=n))
+
+
+def test_shared_prefix_strides_and_default_lengths():
+    g = gen(11)
+    B, Hq, Hkv, Sq, P, S, D = 6, 8, 2, 2, 300, 30, 128
+    q = randn(g, B, Sq, Hq, D).transpose(1, 2)
+    kp, vp = (randn(g, P + 5, Hkv, D).transpose(0, 1)[:, 5:] for _ in range(2))
+    k, v = (randn(g, B, S, Hkv, D).transpose(1, 2) for _ in range(2))
+    out = torch.full((B, Sq, 2 * Hq, D), 3.0, dtype=BF16, device="cuda")
+    view = out[:, :, Hq:].transpose(1, 2)
+    ops.attention_shared_prefix(q, kp, vp, k, v, out=view, softmax_scale=0.2)
+    ops.check()
+    U.check_close(view, *U.shared_prefix(q, kp, vp, k, v, i32([S] * B), 0.2), "o")
+    assert (out[:, :, :Hq] == 3).all()
+
+
+# ---------------------------------------------------------------------------
+# Together, and where they run
+# ---------------------------------------------------------------------------
+def test_layer_prefill_decode_and_training_step():
+    """A layer as it is used: prefill with a window, its gradients, tokens decoded into
+    the cache, and a second batch behind the first as its shared prefix."""
+    B, S, Hq, Hkv, D, W, sinks, cap = 2, 300, 8, 2, 128, 100, 4, 320
+    q, k, wq, wk, freq, _ = rope_inputs(B, S, Hq, Hkv, D, 128, True, seed=12)
+    g = gen(13)
+    v = randn(g, B, Hkv, S, D)
+    pos = torch.arange(S, dtype=torch.int32, device="cuda")
+    kc, vc = (torch.full((B, Hkv, cap, D), NAN, dtype=BF16, device="cuda") for _ in range(2))
+    qn, _ = ops.qk_norm_rope(q, k, wq, wk, freq, pos, k_out=kc[:, :, :S])
+    vc[:, :, :S] = v
+    lse = torch.empty((B, Hq, S), device="cuda")
+    n = i32([S] * B)
+    o = ops.attention_window_fwd(qn, kc, vc, W, sinks, kv_len=n, lse=lse)
+    ops.check()
+    seen = U.visible(n, S, S, W, sinks, "cuda")
+    kn = kc[:, :, :S]
+    U.check_close(o, *U.attention(qn, kn, v, seen)[:2], "prefill")
+
+    do = randn(g, B, Hq, S, D)
+    dqn, dkn, dv = ops.attention_window_bwd(do, qn, kc, vc, o, lse, W, sinks, kv_len=n)
+    assert (dkn[:, :, S:] == 0).all() and (dv[:, :, S:] == 0).all()
+    grads = ops.qk_norm_rope_bwd(dqn, dkn[:, :, :S], q, k, wq, wk, freq, pos)
+    angles = U.rope_angles(pos, freq, B)
+    want = U.norm_rope_bwd(dqn, q, wq, angles, 1e-6, False)
+    U.check_close(grads[0], *want[:2], "dq")
+    U.check_close(grads[2], *want[2:], "dq_weight")
+
+    for step in range(3):  # decode
+        qkv = randn(g, B, 1, Hq + 2 * Hkv, D)
+        q1, k1, v1 = (t.transpose(1, 2) for t in qkv.split((Hq, Hkv, Hkv), dim=2))
+        at = S + step
+        qn, _ = ops.qk_norm_rope(q1, k1, wq, wk, freq, i32([at]), k_out=kc[:, :, at:at + 1])
+        vc[:, :, at:at + 1] = v1
+        o = ops.attention_window_fwd(qn, kc, vc, W, sinks, kv_len=i32([at + 1] * B))
+        ops.check()
+        seen = U.visible(i32([at + 1] * B), 1, at + 1, W, sinks, "cuda")
+        U.check_close(o, *U.attention(qn, kc[:, :, :at + 1], vc[:, :, :at + 1], seen)[:2], "decode")
+
+    m = 7  # requests behind request 0's tokens
+    kp, vp = kc[0, :, :S], vc[0, :, :S]
+    q2, k2, v2 = randn(g, m, Hq, 1, D), randn(g, m, Hkv, 20, D), randn(g, m, Hkv, 20, D)
+    lens = torch.arange(1, m + 1, dtype=torch.int32, device="cuda")
+    o = ops.attention_shared_prefix(q2, kp, vp, k2, v2, kv_len=lens)
+    ops.check()
+    U.check_close(o, *U.shared_prefix(q2, kp, vp, k2, v2, lens), "prefix")
+
+
+def calls(seed):
+    """One call of each operator on inputs of its own: (function, its inputs)."""
+    q, k, wq, wk, freq, pos = rope_inputs(2, 37, 4, 2, 128, 64, True, seed=seed)
+    g = gen(seed)
+    v = randn(g, 2, 2, 37, 128)
+    long_k, long_v = randn(g, 1, 2, 3000, 128), randn(g, 1, 2, 3000, 128)
+    one = randn(g, 1, 4, 1, 128)
+
+    def run():
+        qn, kn = ops.qk_norm_rope(q, k, wq, wk, freq, pos)
+        lse = torch.empty((2, 4, 37), device="cuda")
+        o = ops.attention_window_fwd(qn, kn, v, 16, 2, lse=lse)
+        dq, dk, dv = ops.attention_window_bwd(o, qn, kn, v, o, lse, 16, 2)
+        g = ops.qk_norm_rope_bwd(dq, dk, q, k, wq, wk, freq, pos)
+        dec = ops.attention_window_fwd(one, long_k, long_v, 2500, 4)
+        pre = ops.attention_shared_prefix(qn[:, :, :1], long_k[0], long_v[0], kn, v)
+        return (o, dv, *g, dec, pre)
+    return run
+
+
+def test_captured_calls_replayed_side_by_side():
+    """Two captured graphs, captured on one stream and replayed on two at once, give what
+    eager calls give: no workspace is shared."""
+    runs = [calls(20), calls(21)]
+    want = [[t.clone() for t in r()] for r in runs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for r in runs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(r())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(5):
+        for t in (x for o in outs for x in o):
+            t.fill_(NAN)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, w))
+    ops.check()
+
+
+def test_stream_argument():
+    q, k, v, n, seen = window_inputs(2, 8, 2, 1, 3000, 128, 2000, 4, [3000, 10])
+    want = ops.attention_window_fwd(q, k, v, 2000, 4, kv_len=n)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    got = ops.attention_window_fwd(q, k, v, 2000, 4, kv_len=n, stream=s)
+    ops.check(s)
+    assert torch.equal(got, want)
+
+
+def test_python_refusals():
+    q = torch.zeros(1, 4, 8, 64, dtype=BF16, device="cuda")
+    k = torch.zeros(1, 2, 8, 64, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="bf16"):
+        ops.attention_window_fwd(q, k.float(), k, 4)
+    with pytest.raises(ValueError, match="shape"):
+        ops.attention_window_fwd(q, k, k[:, :, :7], 4)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.attention_window_fwd(q, k.transpose(2, 3).contiguous().transpose(2, 3), k, 4)
+    with pytest.raises(ValueError, match="kv_len"):
+        ops.attention_window_fwd(q, k, k, 4, kv_len=torch.ones(1, device="cuda"))
+    with pytest.raises(ValueError, match="lse"):
+        ops.attention_window_fwd(q, k, k, 4, lse=torch.ones(1, 4, 7, device="cuda"))
+    with pytest.raises(RuntimeError, match="window"):
+        ops.attention_window_fwd(q, k, k, 0)
+    w, f = torch.ones(64, device="cuda"), torch.ones(32, device="cuda")
+    with pytest.raises(ValueError, match="positions"):
+        ops.qk_norm_rope(q, k, w, w, f, torch.zeros(8, device="cuda"))
+    with pytest.raises(ValueError, match="k_weight"):
+        ops.qk_norm_rope(q, k, w, w.bfloat16(), f, i32([0] * 8))
+    with pytest.raises(ValueError, match="v_prefix"):
+        ops.attention_shared_prefix(q, k[0], k[0, :, :5], k, k)
