@@ -1,6 +1,8 @@
 """Build the in-tree sm_100a shared library (libb200attn.so) and the C++ harness
-binaries with nvcc.  Everything is compiled for `-gencode arch=compute_100a,code=sm_100a`
-only; the artefacts land next to this file so they travel with the source tree.
+binaries with nvcc, and the torch binding of the attention layer's operators
+(_binding.so) with the host compiler.  Device code is compiled for `-gencode
+arch=compute_100a,code=sm_100a` only; the artefacts land next to this file so they
+travel with the source tree.
 
 Usage: python -m benchmark_b200.build [--verbose] [--ptxas-info]
 """
@@ -18,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libb200attn.so"
+BINDING = PKG / "_binding.so"
 HARNESS_SRC = PKG / "harness"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -68,6 +71,30 @@ def build_lib(verbose: bool = False, ptxas_info: bool = False, force: bool = Fal
     return LIB
 
 
+def build_binding(verbose: bool = False, force: bool = False) -> Path:
+    """The torch extension over the C ABI (csrc/binding.cpp)."""
+    src = CSRC / "binding.cpp"
+    if not force and not _stale(BINDING, [src, INCLUDE / "b200attn.h"]):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = Path(nvcc()).resolve().parents[1]
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"],
+                str(cuda / "include")]
+    torch_lib = Path(torch.__file__).parent / "lib"
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           *[a for i in includes for a in ("-isystem", i)], "-o", str(tmp), str(src), f"-L{PKG}",
+           "-lb200attn", "-Wl,-rpath,$ORIGIN", f"-L{torch_lib}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    _run(cmd, verbose)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build_harness(verbose: bool = False, force: bool = False) -> list[Path]:
     built = []
     if not HARNESS_SRC.exists():
@@ -106,6 +133,7 @@ def main() -> None:
     ap.add_argument("--force", action="store_true")
     a = ap.parse_args()
     print(build_lib(a.verbose, a.ptxas_info, a.force))
+    print(build_binding(a.verbose, a.force))
     for exe in build_harness(a.verbose, a.force):
         print(exe)
 
