@@ -62,6 +62,17 @@
 // merges all units (O = sum_u O_u 2^(m_u - m) / sum_u l_u 2^(m_u - m)),
 // stores O and resets the counter.  No second launch is needed.
 //
+// Two more forms of the same pipeline (kForm), on strided tensors (4-D maps):
+//   kWindow: sliding window and sinks, a key count per batch row.  An item
+//     visits the tiles of [0, sinks), then the window's; masked tiles test
+//     both ends.  V rows that no row of the item sees are zeroed in shared
+//     memory before the PV product reads them, since they may hold anything
+//     (0 * NaN is NaN); K's need not be: their scores are replaced.
+//   kPrefix: the queries of a whole batch against one shared K/V.  A tile's
+//     128 rows are a box of (batches, tokens, heads of one kv head) of Q; every
+//     unit takes a share of the keys and leaves unnormalised O and (m, l) in a
+//     workspace.
+//
 // Every wait is bounded (ptx.cuh).  A timeout sets the device status word;
 // the epilogue warps, which meet at a named barrier, agree on aborting
 // through a shared flag written before the barrier, so no barrier is ever
@@ -124,7 +135,19 @@ struct Params {
   unsigned long long* trace;
   int trace_cap;
   int trace_cta;
+  // kWindow and kPrefix.  A tensor broadcast along an axis has extent 1 there
+  // in its map: its coordinate is multiplied by 0 (q, k, v; batch and head).
+  int q_mb, q_mh, k_mb, k_mh, v_mb, v_mh;
+  int window, sinks;      // kWindow
+  const int32_t* kv_len;  // kWindow: [B] or null (Skv)
+  float* lse;             // kWindow: [B, Hq, Sq] or null
+  int tile_batches;       // kPrefix: batches of a tile
+  int tile_rows;          // kPrefix: its rows, tile_batches * Sq * group <= 128
+  int rows;               // kPrefix: B * Sq * group
 };
+
+// Forms of the kernel.
+constexpr int kDense = 0, kWindow = 1, kPrefix = 2;
 
 // Clock-trace events (kTrace); names in benchmark_b200/trace.py.
 enum : uint32_t {
@@ -229,6 +252,66 @@ struct Item {
   int min_lim;
   int tile;  // Q tile index (unit / nsplit): the merge counter of split units
 };
+
+// kWindow and kPrefix.
+struct FormItem : Item {
+  int b, hq, hkv;
+  int split;       // kPrefix
+  // kWindow: rows of the item see keys of [0, se) and [lo, hi) only; tile j is
+  // j for the n_sink tiles before the window's and j + skip after them; row r
+  // is at position off + row0 + r; keys below top_lo (and past the sinks) are
+  // hidden from the last row.
+  int se, lo, hi, n_sink, skip, off, top_lo, kv_len;
+};
+
+__device__ __forceinline__ FormItem decode_window_item(const Params& p, int k) {
+  const int bhs = p.B * p.Hq;
+  const int per_group = p.cgroup * p.n_qtiles;
+  const int g = k / per_group;
+  const int kl = k - g * per_group;
+  const int gs = min(p.cgroup, bhs - g * p.cgroup);
+  const int qt = p.n_qtiles - 1 - kl / gs;
+  const int bh = g * p.cgroup + (kl - (kl / gs) * gs);
+  FormItem it;
+  it.b = bh / p.Hq;
+  it.hq = bh - it.b * p.Hq;
+  it.hkv = it.hq / p.group;
+  it.row0 = qt * kBM;
+  it.kv_len = p.kv_len ? max(0, min(__ldg(p.kv_len + it.b), p.Skv)) : p.Skv;
+  it.off = it.kv_len - p.Sq;
+  const int last = it.off + min(it.row0 + kBM, p.Sq) - 1;  // the last row's position
+  it.hi = max(0, last + 1);
+  it.lo = max(0, it.off + it.row0 - p.window + 1);
+  if (p.sinks >= it.lo || it.hi == 0) it.lo = 0;
+  it.se = it.lo > 0 ? p.sinks : 0;
+  const int w0 = it.lo / kBN;
+  it.n_sink = min((it.se + kBN - 1) / kBN, w0);
+  it.skip = w0 - it.n_sink;
+  it.n = it.n_sink + (it.hi + kBN - 1) / kBN - w0;
+  it.j0 = 0;
+  it.top_lo = last - p.window + 1;
+  it.min_lim = min(it.kv_len, it.off + it.row0 + 1);
+  return it;
+}
+
+// Units of one (kv head, share of the keys) are adjacent: they read the same
+// K/V at the same time.
+__device__ __forceinline__ FormItem decode_prefix_item(const Params& p, int k) {
+  const int mt = k % p.n_qtiles, rest = k / p.n_qtiles;
+  FormItem it;
+  it.split = rest % p.nsplit;
+  it.hkv = rest / p.nsplit;
+  it.hq = it.hkv * p.group;
+  it.b = mt * p.tile_batches;
+  it.row0 = mt * p.tile_rows;
+  const int n_all = (p.Skv + kBN - 1) / kBN;
+  it.j0 = static_cast<int>(static_cast<int64_t>(n_all) * it.split / p.nsplit);
+  it.n = static_cast<int>(static_cast<int64_t>(n_all) * (it.split + 1) / p.nsplit) - it.j0;
+  it.n_sink = it.n;  // tile j is j0 + j
+  it.skip = 0;
+  it.min_lim = p.Skv;
+  return it;
+}
 
 // Work item k.  Non-causal: items of one head are adjacent, so the CTAs
 // running at one time share a few heads' K/V in L2.  Causal: planes are taken
@@ -358,7 +441,7 @@ __device__ __forceinline__ void p_rows(const float* s, float sc, float nm_a, flo
   }
 }
 
-template <int D, int kEmu, bool kTrace = false, bool kPair = false>
+template <int D, int kEmu, bool kTrace = false, bool kPair = false, int kForm = kDense>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap q_map,
                          const __grid_constant__ CUtensorMap k_map,
@@ -406,12 +489,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int rounds = (p.n_items + units_per_round - 1) / units_per_round;
   auto item_at = [&](int r) { return kPair ? pair_item_index(r) : item_index(p, r); };
   auto decode_at = [&](int k) {
-    return kPair ? decode_pair_item(p, k) : decode_item(p, k);
+    if constexpr (kForm == kWindow)
+      return decode_window_item(p, k);
+    else if constexpr (kForm == kPrefix)
+      return decode_prefix_item(p, k);
+    else
+      return kPair ? decode_pair_item(p, k) : decode_item(p, k);
+  };
+  // Index of an item's K/V tile j.
+  auto kv_tile = [](const auto& it, int j) {
+    if constexpr (kForm == kDense)
+      return it.j0 + j;
+    else
+      return it.j0 + (j < it.n_sink ? j : j + it.skip);
   };
   // The leader's copy of a barrier of this CTA's layout (shared::cluster).
   auto lead_bar = [&](uint64_t* b_) { return mapa_shared(smem_u32(b_), 0u); };
 
   // ---- setup ----
+  if constexpr (kForm == kPrefix) {
+    // Rows past a tile's box stay zero (their scores are computed, and dropped).
+    for (int i = static_cast<int>(threadIdx.x); i < 2 * C::kTileBytes / 16; i += kThreads)
+      reinterpret_cast<uint4*>(q_buf)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
@@ -486,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int r = 0; r < rounds && ok; ++r) {
           const int k = item_at(r);
           if (k >= p.n_items) continue;
-          const Item it = decode_at(k);
+          const auto it = decode_at(k);
           const int qb = li & 1;
           const uint32_t qpar = static_cast<uint32_t>(li >> 1) & 1u;
           ++li;
@@ -500,6 +601,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int h = 0; h < C::kBoxes; ++h)
                 tma_load_3d_pair(q_buf + qb * C::kTileBytes + h * C::kBoxBytes, &q_map,
                                  lead_bar(&q_full[qb]), h * 64, it.row0, it.zq, pol_q);
+            } else if constexpr (kForm == kWindow) {
+              mbar_arrive_expect_tx(&q_full[qb], C::kTileBytes);
+              for (int h = 0; h < C::kBoxes; ++h)
+                tma_load_4d(q_buf + qb * C::kTileBytes + h * C::kBoxBytes, &q_map, &q_full[qb],
+                            h * 64, it.row0, it.hq * p.q_mh, it.b * p.q_mb, pol_q);
+            } else if constexpr (kForm == kPrefix) {
+              // A box of (64 columns, heads of the kv head, tokens, batches).
+              mbar_arrive_expect_tx(&q_full[qb],
+                                    static_cast<uint32_t>(C::kBoxes * 128 * p.tile_rows));
+              for (int h = 0; h < C::kBoxes; ++h)
+                tma_load_4d(q_buf + qb * C::kTileBytes + h * C::kBoxBytes, &q_map, &q_full[qb],
+                            h * 64, it.hq, 0, it.b, pol_q);
             } else {
               mbar_arrive_expect_tx(&q_full[qb], C::kTileBytes);
               for (int h = 0; h < C::kBoxes; ++h)
@@ -524,6 +637,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    lead_bar(&k_full[ks]), h * 64,
                                    (it.j0 + j) * kBN + static_cast<int>(rank) * C::kKRows,
                                    it.zkv, pol_kv);
+              } else if constexpr (kForm != kDense) {
+                mbar_arrive_expect_tx(&k_full[ks], C::kTileBytes);
+                for (int h = 0; h < C::kBoxes; ++h)
+                  tma_load_4d(k_buf + ks * C::kTileBytes + h * C::kBoxBytes, &k_map, &k_full[ks],
+                              h * 64, kv_tile(it, j) * kBN, it.hkv * p.k_mh, it.b * p.k_mb,
+                              pol_kv);
               } else {
                 mbar_arrive_expect_tx(&k_full[ks], C::kTileBytes);
                 for (int h = 0; h < C::kBoxes; ++h)
@@ -544,6 +663,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    lead_bar(&v_full[vs]),
                                    (static_cast<int>(rank) * C::kVBoxes + h) * 64,
                                    (it.j0 + j) * kBN, it.zkv, pol_kv);
+              } else if constexpr (kForm != kDense) {
+                mbar_arrive_expect_tx(&v_full[vs], C::kTileBytes);
+                for (int h = 0; h < C::kBoxes; ++h)
+                  tma_load_4d(v_buf + vs * C::kTileBytes + h * C::kBoxBytes, &v_map, &v_full[vs],
+                              h * 64, kv_tile(it, j) * kBN, it.hkv * p.v_mh, it.b * p.v_mb,
+                              pol_kv);
               } else {
                 mbar_arrive_expect_tx(&v_full[vs], C::kTileBytes);
                 for (int h = 0; h < C::kBoxes; ++h)
@@ -643,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int r = 0; r < rounds && ok; ++r) {
             const int k = item_at(r);
             if (k >= p.n_items) continue;
-            const Item it = decode_at(k);
+            const auto it = decode_at(k);
             const int qb = li & 1;
             const uint32_t qpar = static_cast<uint32_t>(li >> 1) & 1u;
             ++li;
@@ -675,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int r = 0; r < rounds && ok; ++r) {
             const int k = item_at(r);
             if (k >= p.n_items) continue;
-            const Item it = decode_at(k);
+            const auto it = decode_at(k);
             const uint32_t oe_par = (static_cast<uint32_t>(li) & 1u) ^ 1u;  // epilogue of li-1
             if (it.n == 0) {
               // No K/V tiles: O stays unwritten (the epilogue stores zeros in Q's
@@ -770,11 +895,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int r = 0; r < rounds && ok; ++r) {
       const int k = item_at(r);
       if (k >= p.n_items) continue;
-      const Item it = decode_at(k);
+      const auto it = decode_at(k);
       const int qb = li & 1;
       const uint32_t tO = tmem_base + lane_addr + C::kColO;
-      const int lim_a = p.causal ? min(p.Skv, it.row0 + ra + p.causal_off + 1) : p.Skv;
-      const int lim_b = p.causal ? min(p.Skv, it.row0 + rb + p.causal_off + 1) : p.Skv;
+      int lim_a, lim_b;        // keys below these are visible to rows a and b,
+      int low_a = 0, low_b = 0;  // kWindow: from these on (or before the sinks' end)
+      if constexpr (kForm == kWindow) {
+        lim_a = min(it.kv_len, it.off + it.row0 + ra + 1);
+        lim_b = min(it.kv_len, it.off + it.row0 + rb + 1);
+        low_a = it.off + it.row0 + ra - p.window + 1;
+        low_b = it.off + it.row0 + rb - p.window + 1;
+      } else {
+        lim_a = p.causal ? min(p.Skv, it.row0 + ra + p.causal_off + 1) : p.Skv;
+        lim_b = p.causal ? min(p.Skv, it.row0 + rb + p.causal_off + 1) : p.Skv;
+      }
       // Running max of scaled scores (log2 units) and this thread's share of
       // the row sums, for rows a and b.
       float m_a = -INFINITY, m_b = -INFINITY;
@@ -798,8 +932,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         have_s = false;
         tr(kEvSmLdDone, warp >> 2, tt);
         float* s = reinterpret_cast<float*>(sr);
-        const int kbase = (it.j0 + j) * kBN;
-        const bool masked = kbase + kBN > it.min_lim;  // uniform across the tile
+        const int kbase = kv_tile(it, j) * kBN;
+        bool masked = kbase + kBN > it.min_lim;  // uniform across the tile
+        if constexpr (kForm == kWindow)
+          masked |= kbase < it.top_lo && kbase + kBN > p.sinks;
         float f_a = 1.0f, f_b = 1.0f;
         bool rescale = false;    // this thread's rows
         uint64_t rs_a = 0ull, rs_b = 0ull;
@@ -899,14 +1035,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (masked) {
             // Scale first, then mask, so masked keys are exactly -inf for any scale.
             const int va = lim_a - kbase - 2 * t0, vb = lim_b - kbase - 2 * t0;
+            const int wa = low_a - kbase - 2 * t0, wb = low_b - kbase - 2 * t0;
+            const int sk = p.sinks - kbase - 2 * t0;
             mx_a = -INFINITY;
             mx_b = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 16; ++g) {
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const float xa = 8 * g + e < va ? s[4 * g + e] * c : -INFINITY;
-                const float xb = 8 * g + e < vb ? s[4 * g + 2 + e] * c : -INFINITY;
+                const int u = 8 * g + e;
+                bool see_a = u < va, see_b = u < vb;
+                if constexpr (kForm == kWindow) {
+                  see_a &= u >= wa || u < sk;
+                  see_b &= u >= wb || u < sk;
+                }
+                const float xa = see_a ? s[4 * g + e] * c : -INFINITY;
+                const float xb = see_b ? s[4 * g + 2 + e] * c : -INFINITY;
                 s[4 * g + e] = xa;
                 s[4 * g + 2 + e] = xb;
                 mx_a = fmaxf(mx_a, xa);
@@ -968,6 +1112,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           ready = mbar_try_wait(smem_u32(&s_ready[nb]), static_cast<uint32_t>((tt + 1) / kSBufs) & 1u);
           ready_all = __all_sync(0xffffffffu, ready);
           if (rescale_w && j > 0) rescale_o();
+        }
+        if constexpr (kForm == kWindow) {
+          // Zero the V rows of keys that no row of the item sees: eight warps,
+          // two threads to a row, before this warp's P is published.
+          if (ok && (kbase + kBN > it.hi || (kbase < it.lo && kbase + kBN > it.se))) {
+            const int vs = tt % C::kVStages;
+            ok = warp_wait(&v_full[vs], static_cast<uint32_t>(tt / C::kVStages) & 1u, kSiteVFull);
+            const int row = static_cast<int>(threadIdx.x >> 1), key = kbase + row;
+            if (ok && (key >= it.hi || (key < it.lo && key >= it.se))) {
+              const uint32_t at = smem_u32(v_buf + vs * C::kVTileBytes) +
+                                  static_cast<uint32_t>(row * 128 + (threadIdx.x & 1) * 64);
+#pragma unroll
+              for (int i = 0; i < C::kVBoxes * 4; ++i)
+                st_shared_v4(at + (i >> 2) * C::kBoxBytes + (i & 3) * 16, 0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+          }
         }
         tr(kEvSmPComputed, warp >> 2, tt);
         // S(tt+1) (the next item's first tile after an item's last), if it is
@@ -1044,7 +1205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int r = 0; r < rounds; ++r) {
       const int k = item_at(r);
       if (k >= p.n_items) continue;
-      const Item it = decode_at(k);
+      const auto it = decode_at(k);
       const int qb = li & 1;
       const uint32_t qpar = static_cast<uint32_t>(li >> 1) & 1u;
       ++li;
@@ -1084,7 +1245,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                      w[3]);
       };
       bool store = true;  // this unit stores the O tile
-      if (kPair || p.nsplit == 1) {
+      if constexpr (kForm == kWindow) {
+        if (p.lse && it.row0 + row < p.Sq)
+          p.lse[(static_cast<int64_t>(it.b) * p.Hq + it.hq) * p.Sq + it.row0 + row] =
+              have_o && ml.y > 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : -INFINITY;
+      }
+      if constexpr (kForm == kPrefix) {
+        // This unit's unnormalised O rows and (m, l), [kv head][split][row].
+        const int r_all = it.row0 + row;
+        const bool live = got && row < p.tile_rows && r_all < p.rows;
+        const int64_t at =
+            (static_cast<int64_t>(it.hkv) * p.nsplit + it.split) * p.rows + r_all;
+#pragma unroll 1
+        for (int c0 = 0; c0 < (got ? D : 0); c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32(tO + c0, o);
+          tmem_wait_ld(o);
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<uint4*>(p.ws_o + at * D + c0)[e] =
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (live) p.ws_ml[at] = ml;
+        store = false;
+        tc_fence_before();
+        mbar_arrive(o_empty);
+      } else if (kPair || kForm == kWindow || p.nsplit == 1) {
         const float inv = (have_o && ml.y > 0.0f) ? 1.0f / ml.y : 0.0f;
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
@@ -1222,8 +1410,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (quad == 0 && lane == 0) {
         // (A pair's second tile past the last Q row has nothing to store.)
         if (store && it.row0 < p.Sq) {
-          for (int b = 0; b < C::kBoxes; ++b)
-            tma_store_3d_hint(&o_map, obuf + b * C::kBoxBytes, b * 64, it.row0, it.zq, pol_o);
+          for (int b = 0; b < C::kBoxes; ++b) {
+            if constexpr (kForm == kWindow)
+              tma_store_4d_hint(&o_map, obuf + b * C::kBoxBytes, b * 64, it.row0, it.hq, it.b,
+                                pol_o);
+            else
+              tma_store_3d_hint(&o_map, obuf + b * C::kBoxBytes, b * 64, it.row0, it.zq, pol_o);
+          }
           bulk_commit_group();
           bulk_wait_group_read<0>();
         }

@@ -30,6 +30,8 @@ b200_status check_tensor(const char* who, const char* name, const b200_tensor* t
     if (x.stride >= (int64_t{1} << 39))
       return fail(B200_EUNSUPPORTED, "%s: a stride of %s is 2^39 elements or more", who, name);
   }
+  if (S > 1 && t->stride_s == 0)
+    return fail(B200_EINVAL, "%s: the tokens of %s may not share a row (stride 0)", who, name);
   if (!output) return B200_OK;
   std::sort(d, d + 3, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
   int64_t reach = D;
@@ -55,13 +57,32 @@ b200_status check_launch(const char* what) {
   return e == cudaSuccess ? B200_OK : cuda_fail(e, what);
 }
 
+// Launch on `stream` a kernel that starts while its predecessor there still
+// runs (it waits with pdl_wait before it reads what that one wrote).
+template <typename... P, typename... A>
+b200_status launch_dependent(void (*kernel)(P...), unsigned grid, unsigned threads,
+                             cudaStream_t stream, const char* what, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, what);
+}
+
 size_t round16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
 // ---- query/key norm with rotation ----
 struct RopeArgs {
   b200::rope::Params p;
-  int D;
-  bool interleaved;
+  bool per_row;     // few heads: a token to each row of a warp
+  int groups_q, groups_k;  // row groups of a token
+  int64_t token_groups;
 };
 
 b200_status rope_args(const char* who, const b200_tensor* q, const b200_tensor* k,
@@ -73,11 +94,16 @@ b200_status rope_args(const char* who, const b200_tensor* q, const b200_tensor* 
     return fail(B200_EINVAL, "%s: invalid shape B=%d S=%d Hq=%d Hkv=%d", who, B, S, Hq, Hkv);
   if (D != 64 && D != 128)
     return fail(B200_EUNSUPPORTED, "%s: head_dim must be 64 or 128; got D=%d", who, D);
-  if (Hq > 4096 || Hkv > 4096) return fail(B200_EUNSUPPORTED, "%s: more than 4096 heads", who);
+  if (static_cast<int64_t>(B) * S > (int64_t{1} << 30))
+    return fail(B200_EUNSUPPORTED, "%s: more than 2^30 tokens", who);
+  if (Hq > (1 << 20) || Hkv > (1 << 20))
+    return fail(B200_EUNSUPPORTED, "%s: more than 2^20 heads", who);
   if (rotary_dim < 0 || rotary_dim > D || rotary_dim % 16 != 0)
     return fail(B200_EUNSUPPORTED, "%s: rotary_dim must be a multiple of 16 in [0, D]; got %d",
                 who, rotary_dim);
   if (!q_weight || !k_weight) return fail(B200_EINVAL, "%s: null weight", who);
+  if (!aligned16(q_weight) || !aligned16(k_weight))
+    return fail(B200_EINVAL, "%s: weights must be 16-byte aligned", who);
   if (rotary_dim > 0 && (!inv_freq || !positions))
     return fail(B200_EINVAL, "%s: null inv_freq or positions", who);
   if (!(eps >= 0.0f) || !std::isfinite(eps))
@@ -96,30 +122,47 @@ b200_status rope_args(const char* who, const b200_tensor* q, const b200_tensor* 
   p.inv_freq = inv_freq;
   p.pos = positions;
   p.pos_sb = position_stride_b;
-  p.tokens = static_cast<int64_t>(B) * S;
+  p.tokens = static_cast<uint32_t>(B) * static_cast<uint32_t>(S);
   p.S = S;
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.rot = rotary_dim;
-  auto reciprocal = [](int H) {
-    return H == 1 ? 0u : static_cast<uint32_t>((uint64_t{1} << 32) / static_cast<uint64_t>(H) + 1);
-  };
-  p.mul_q = reciprocal(Hq);
-  p.mul_k = reciprocal(Hkv);
   p.eps = eps;
-  // Blocks of tokens: long enough to share the angles among heads, short
-  // enough that the grid fills the GPU.
-  const int64_t per = p.tokens / (static_cast<int64_t>(sm_count()) * 8);
-  p.block = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(per, b200::rope::kMaxTokens)));
-  *out = RopeArgs{p, D, interleaved != 0};
+  // Rows of a warp hold heads of one token unless half of them or more would
+  // stay empty.
+  const int rows = 512 / D;
+  RopeArgs a{p, false, (Hq + rows - 1) / rows, (Hkv + rows - 1) / rows, p.tokens};
+  a.per_row = 2ll * (Hq + Hkv) <= static_cast<long long>(a.groups_q + a.groups_k) * rows;
+  if (a.per_row) {
+    a.groups_q = Hq;
+    a.groups_k = Hkv;
+    a.token_groups = (p.tokens + rows - 1) / rows;
+  }
+  *out = a;
   return B200_OK;
 }
 
-int rope_bwd_grid(int64_t tokens, int block) {
-  const int64_t blocks = (tokens + block - 1) / block;
-  return static_cast<int>(
-      std::min<int64_t>(blocks, static_cast<int64_t>(sm_count()) * b200::rope::kGradCtasPerSm));
+// f(head size, interleaved, per_row) with these as integral constants.
+template <typename F>
+b200_status rope_dispatch(int D, bool interleaved, bool per_row, F&& f) {
+  using T = std::true_type;
+  using N = std::false_type;
+  auto by_row = [&](auto d, auto il) { return per_row ? f(d, il, T{}) : f(d, il, N{}); };
+  auto by_pairs = [&](auto d) { return interleaved ? by_row(d, T{}) : by_row(d, N{}); };
+  return D == 128 ? by_pairs(std::integral_constant<int, 128>{})
+                  : by_pairs(std::integral_constant<int, 64>{});
+}
+
+// CTAs of the backward kernel for the queries and for the keys, by their rows.
+struct RopeGrid {
+  int q, k;
+};
+
+RopeGrid rope_bwd_grid(const RopeArgs& a) {
+  const int64_t ctas = (a.token_groups + b200::rope::kWarps - 1) / b200::rope::kWarps;
+  const int64_t most = static_cast<int64_t>(sm_count()) * b200::rope::kGradCtasPerSm;
+  const int64_t k = std::max<int64_t>(1, most * a.groups_k / (a.groups_q + a.groups_k));
+  return RopeGrid{static_cast<int>(std::min(ctas, most - k)), static_cast<int>(std::min(ctas, k))};
 }
 
 // ---- window and prefix attention ----
@@ -161,25 +204,51 @@ int split_plan(int64_t units, int64_t keys) {
       std::max<int64_t>(1, std::min<int64_t>({want, most, b200::split::kMaxSplits})));
 }
 
+int row_tiles_of(int64_t rows) {
+  return static_cast<int>((rows + b200::split::kRows - 1) / b200::split::kRows);
+}
+
+// Work of the 16-row kernel, in us at the rate it was measured at with the GPU
+// full (keys x units per us; a unit is a 16-row tile of one kv head).
+double split_us(int64_t units, int64_t keys, int D) {
+  return static_cast<double>(units) * static_cast<double>(keys) / (D == 128 ? 23400.0 : 36400.0);
+}
+
+// Whether a window call goes by 128-row tiles: by the time of each kernel's
+// work, since both start alike (about 7 us).  A 128-row tile spends about 1 us
+// on 128 keys, whatever its rows; the 16-row kernel splits the keys, so that
+// few rows fill the GPU.  Measured (us, 16-row / 128-row): B 1, heads 32/8,
+// window 1024, Sq 64: 15.5 / 18.9, Sq 128: 19.6 / 18.8; B 8, 8192 keys, Sq 16:
+// 107 / 124, Sq 32: 210 / 125; D 64, B 8, window 1024, Sq 32: 24.5 / 32.3,
+// Sq 64: 44.0 / 32.3.
+bool window_by_tiles(const WindowShape& s) {
+  const int64_t rows = static_cast<int64_t>(s.Hq / s.Hkv) * s.Sq;
+  const int64_t reach = static_cast<int64_t>(s.window) + s.sinks;
+  const int64_t units = static_cast<int64_t>(s.B) * s.Hkv * row_tiles_of(rows);
+  const int64_t items = static_cast<int64_t>(s.B) * s.Hq * ((s.Sq + 127) / 128);
+  const int64_t sms = sm_count(), rounds = (items + sms - 1) / sms;
+  const double tiles_us =
+      static_cast<double>(rounds * (std::min<int64_t>(s.Skv, reach + 127) / 128 + 1));
+  return split_us(units, std::min<int64_t>(s.Skv, reach), s.D) > tiles_us;
+}
+
 size_t part_bytes(int64_t rows, int D) {
   return round16(static_cast<size_t>(rows) * D * sizeof(float)) +
          round16(static_cast<size_t>(rows) * sizeof(float2));
 }
 
-int row_tiles_of(int64_t rows) {
-  return static_cast<int>((rows + b200::split::kRows - 1) / b200::split::kRows);
-}
-
 struct WindowPlan {
+  bool tiles;   // 128-row tiles (tcgen05); else 16-row tiles that split the keys
   int nsplit;
   size_t bytes;
 };
 
 WindowPlan window_plan(const WindowShape& s, bool partial = false) {
+  if (!partial && window_by_tiles(s)) return WindowPlan{true, 1, 0};
   const int64_t rows = static_cast<int64_t>(s.Hq / s.Hkv) * s.Sq;
   const int64_t units = static_cast<int64_t>(s.B) * s.Hkv * row_tiles_of(rows);
   const int64_t keys = std::min<int64_t>(s.Skv, static_cast<int64_t>(s.window) + s.sinks);
-  WindowPlan p{split_plan(units, keys), 0};
+  WindowPlan p{false, split_plan(units, keys), 0};
   if (p.nsplit > 1 || partial)
     p.bytes = part_bytes(static_cast<int64_t>(s.B) * s.Hkv * p.nsplit * rows, s.D);
   return p;
@@ -249,18 +318,181 @@ b200_status check_qkvo(const char* who, const WindowShape& s, const b200_tensor*
   return check_tensor(who, "o", o, s.B, s.Hq, s.Sq, s.D, true);
 }
 
+// ---- the tiled (tcgen05) forms ----
+// Map of a [B, H, S, D] tensor with boxes of `rows` tokens.  An axis that is
+// broadcast (stride 0) gets extent 1, and its coordinate the factor 0.
+b200_status encode_view(CUtensorMap* map, const b200_tensor* t, int B, int H, int S, int D,
+                        uint32_t rows, int* mul_b, int* mul_h) {
+  const bool wide_b = B > 1 && t->stride_b != 0, wide_h = H > 1 && t->stride_h != 0;
+  *mul_b = wide_b;
+  *mul_h = wide_h;
+  const cuuint64_t any = static_cast<cuuint64_t>(D) * 2;  // stride of an axis of extent 1
+  const cuuint64_t d[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S),
+                           static_cast<cuuint64_t>(wide_h ? H : 1),
+                           static_cast<cuuint64_t>(wide_b ? B : 1)};
+  const cuuint64_t s[3] = {S > 1 ? static_cast<cuuint64_t>(t->stride_s) * 2 : any,
+                           wide_h ? static_cast<cuuint64_t>(t->stride_h) * 2 : any,
+                           wide_b ? static_cast<cuuint64_t>(t->stride_b) * 2 : any};
+  const cuuint32_t box[4] = {64, rows, 1, 1};
+  return encode_bf16_4d(map, t->data, d, s, box);
+}
+
+template <int D, int kForm>
+b200_status launch_tiles(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
+                         const CUtensorMap& om, b200::attn::Params p, long long items,
+                         cudaStream_t stream) {
+  using C = b200::attn::Cfg<D>;
+  static unsigned attr_done = 0;
+  auto kernel = b200::attn::attention_fwd_kernel<D, D == 128 ? kDefaultEmuD128 : kDefaultEmuD64,
+                                                 false, false, kForm>;
+  const b200_status st = ensure_smem_attr(kernel, C::kSmemBytes, &attr_done);
+  if (st != B200_OK) return st;
+  static const int launch_regs = [kernel] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : -1;
+  }();
+  if (launch_regs != b200::attn::kLaunchRegs)
+    return fail(B200_EUNSUPPORTED,
+                "attention: kernel has %d registers per thread at launch; its register split "
+                "needs exactly %d",
+                launch_regs, b200::attn::kLaunchRegs);
+  if (items > 0x3fffffffll) return fail(B200_EUNSUPPORTED, "attention: too many work items");
+  p.n_items = static_cast<int>(items);
+  const int grid = static_cast<int>(std::min<long long>(items, sm_count()));
+  kernel<<<grid, b200::attn::kThreads, C::kSmemBytes, stream>>>(qm, km, vm, om, p);
+  return check_launch("attention tiles launch");
+}
+
+b200::attn::Params tile_params(const WindowShape& s) {
+  b200::attn::Params p{};
+  p.B = s.B;
+  p.Hq = s.Hq;
+  p.Hkv = s.Hkv;
+  p.Sq = s.Sq;
+  p.Skv = s.Skv;
+  p.group = s.Hq / s.Hkv;
+  p.nsplit = 1;
+  p.scale_log2 = s.scale * 1.4426950408889634f;
+  return p;
+}
+
+template <int D>
+b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, const b200_tensor* k,
+                                const b200_tensor* v, const b200_tensor* o, float* lse,
+                                const int32_t* kv_len, cudaStream_t stream) {
+  b200::attn::Params p = tile_params(s);
+  CUtensorMap qm, km, vm, om;
+  int one;
+  b200_status st;
+  constexpr uint32_t kRows = b200::attn::kBM, kKeys = b200::attn::kBN;
+  if ((st = encode_view(&qm, q, s.B, s.Hq, s.Sq, D, kRows, &p.q_mb, &p.q_mh)) != B200_OK ||
+      (st = encode_view(&km, k, s.B, s.Hkv, s.Skv, D, kKeys, &p.k_mb, &p.k_mh)) != B200_OK ||
+      (st = encode_view(&vm, v, s.B, s.Hkv, s.Skv, D, kKeys, &p.v_mb, &p.v_mh)) != B200_OK ||
+      (st = encode_view(&om, o, s.B, s.Hq, s.Sq, D, kRows, &one, &one)) != B200_OK)
+    return st;
+  p.n_qtiles = (s.Sq + b200::attn::kBM - 1) / b200::attn::kBM;
+  p.causal = 1;  // the order of the items, as causal attention's
+  p.window = s.window;
+  p.sinks = s.sinks;
+  p.kv_len = kv_len;
+  p.lse = lse;
+  const long long planes = static_cast<long long>(s.B) * s.Hq;
+  // Planes of an ordering group: their K/V in use fit in half of the L2 (as
+  // for causal attention).
+  const double keys = std::min<double>(s.Skv, static_cast<double>(s.window) + b200::attn::kBM);
+  const long long g = static_cast<long long>(64.0 * (1 << 20) / (4.0 * keys * D)) * p.group;
+  p.cgroup = static_cast<int>(std::max<long long>(1, std::min<long long>(g, planes)));
+  return launch_tiles<D, b200::attn::kWindow>(qm, km, vm, om, p, planes * p.n_qtiles, stream);
+}
+
+// Tiles of the prefix form: whole batches, up to 128 rows.
+struct PrefixTiles {
+  int batches, rows, count;  // of a tile; tiles
+};
+
+PrefixTiles prefix_tiles(const WindowShape& own) {
+  const int rows = own.Hq / own.Hkv * own.Sq;  // of a batch
+  const int nb = std::min(own.B, b200::attn::kBM / rows);
+  return PrefixTiles{nb, nb * rows, (own.B + nb - 1) / nb};
+}
+
+template <int D>
+b200_status launch_prefix_tiles(const WindowShape& own, int P, const b200_tensor* q,
+                                const b200_tensor* k, const b200_tensor* v, int nsplit,
+                                float* part_o, float2* part_ml, cudaStream_t stream) {
+  WindowShape shared = own;
+  shared.Skv = P;
+  b200::attn::Params p = tile_params(shared);
+  const PrefixTiles t = prefix_tiles(own);
+  p.n_qtiles = t.count;
+  p.tile_batches = t.batches;
+  p.tile_rows = t.rows;
+  p.rows = own.B * p.group * own.Sq;
+  p.nsplit = nsplit;
+  p.ws_o = part_o;
+  p.ws_ml = part_ml;
+  CUtensorMap qm, km, vm;
+  b200_status st;
+  const cuuint64_t any = static_cast<cuuint64_t>(D) * 2;
+  auto stride = [&](int n, int64_t x) { return n > 1 ? static_cast<cuuint64_t>(x) * 2 : any; };
+  const cuuint64_t d[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(own.Hq),
+                           static_cast<cuuint64_t>(own.Sq), static_cast<cuuint64_t>(own.B)};
+  const cuuint64_t str[3] = {stride(own.Hq, q->stride_h), stride(own.Sq, q->stride_s),
+                             stride(own.B, q->stride_b)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(p.group),
+                             static_cast<cuuint32_t>(own.Sq), static_cast<cuuint32_t>(t.batches)};
+  if ((st = encode_bf16_4d(&qm, q->data, d, str, box)) != B200_OK) return st;
+  constexpr uint32_t kKeys = b200::attn::kBN;
+  if ((st = encode_view(&km, k, 1, own.Hkv, P, D, kKeys, &p.k_mb, &p.k_mh)) != B200_OK ||
+      (st = encode_view(&vm, v, 1, own.Hkv, P, D, kKeys, &p.v_mb, &p.v_mh)) != B200_OK)
+    return st;
+  return launch_tiles<D, b200::attn::kPrefix>(
+      qm, km, vm, qm, p, static_cast<long long>(own.Hkv) * t.count * nsplit, stream);
+}
+
 // The prefix as one batch whose rows are those of every request's queries.
 struct PrefixPlan {
+  bool tiles;         // the prefix by 128-row tiles (tcgen05); else 16-row tiles
   int prefix_splits;  // 0: no prefix
   int own_splits;
   size_t prefix_bytes, own_bytes;
 };
 
-PrefixPlan prefix_plan(const WindowShape& own, int P) {
+// Whether the prefix goes by 128-row tiles: where the 16-row kernel's work
+// would take more than 4 us (the tiles' later start and larger partial sums).
+// Measured (us of a call, 16-row / 128-row): heads 32/8, 2048 keys, 16 requests:
+// 16.3 / 17.6, 32: 20.5 / 19.8; 8192 keys, 4: 18.4 / 19.2, 8: 20.7 / 19.6, 64:
+// 69.8 / 30.1; D 64, 8192 keys, 8: 17.5 / 18.2, 16: 19.8 / 19.0.  A tile holds
+// whole requests, and the queries' map cannot broadcast.
+bool prefix_by_tiles(const WindowShape& own, int P, const b200_tensor* q) {
+  const int64_t rows = static_cast<int64_t>(own.Hq / own.Hkv) * own.Sq;
+  if (rows > b200::attn::kBM) return false;
+  if (q && ((own.B > 1 && q->stride_b == 0) || (own.Hq > 1 && q->stride_h == 0))) return false;
+  return own.B * rows > b200::split::kRows &&
+         split_us(own.Hkv * static_cast<int64_t>(row_tiles_of(own.B * rows)), P, own.D) > 4.0;
+}
+
+// q's strides decide too; null: they do not.
+PrefixPlan prefix_plan(const WindowShape& own, int P, const b200_tensor* q) {
   PrefixPlan p{};
   if (P > 0) {
     const int64_t rows = static_cast<int64_t>(own.B) * (own.Hq / own.Hkv) * own.Sq;
-    p.prefix_splits = split_plan(static_cast<int64_t>(own.Hkv) * row_tiles_of(rows), P);
+    p.tiles = prefix_by_tiles(own, P, q);
+    if (p.tiles) {
+      // Least rounds x (tiles of K/V per unit + a unit's fixed cost of about 3).
+      const int64_t units = static_cast<int64_t>(own.Hkv) * prefix_tiles(own).count;
+      const int64_t kv = (P + b200::attn::kBN - 1) / b200::attn::kBN, sms = sm_count();
+      int64_t best = INT64_MAX;
+      for (int ns = 1; ns <= std::min<int64_t>(kv, b200::split::kMaxSplits); ++ns) {
+        const int64_t cost = (units * ns + sms - 1) / sms * ((kv + ns - 1) / ns + 3);
+        if (cost < best) {
+          best = cost;
+          p.prefix_splits = ns;
+        }
+      }
+    } else {
+      p.prefix_splits = split_plan(static_cast<int64_t>(own.Hkv) * row_tiles_of(rows), P);
+    }
     p.prefix_bytes = part_bytes(own.Hkv * p.prefix_splits * rows, own.D);
   }
   const WindowPlan w = window_plan(own, P > 0);
@@ -299,23 +531,27 @@ b200_status qk_norm_rope(const b200_tensor* q, const b200_tensor* k, const void*
   if ((st = check_tensor(who, "k_out", k_out, B, Hkv, S, D, true)) != B200_OK) return st;
   a.p.qy = view_of(q_out);
   a.p.ky = view_of(k_out);
-  const int64_t grid = (a.p.tokens + a.p.block - 1) / a.p.block;
-  if (grid > 0x7fffffffll) return fail(B200_EUNSUPPORTED, "%s: too many tokens", who);
-  using Kernel = void (*)(b200::rope::Params);
-  const Kernel kernel =
-      D == 128 ? (a.interleaved ? b200::rope::norm_rope_kernel<128, true>
-                                : b200::rope::norm_rope_kernel<128, false>)
-               : (a.interleaved ? b200::rope::norm_rope_kernel<64, true>
-                                : b200::rope::norm_rope_kernel<64, false>);
-  kernel<<<static_cast<unsigned>(grid), b200::rope::kThreads, 0,
+  // Slices of a token's heads, so that few tokens still give every SM 24 warps.
+  const int groups = a.groups_q + a.groups_k;
+  const int64_t warps = static_cast<int64_t>(sm_count()) * 24;
+  a.p.slice_groups = static_cast<int>(
+      std::min<int64_t>(groups, (groups * a.token_groups + warps - 1) / warps));
+  a.p.slices = (groups + a.p.slice_groups - 1) / a.p.slice_groups;
+  const int64_t grid =
+      (a.token_groups * a.p.slices + b200::rope::kWarps - 1) / b200::rope::kWarps;
+  return rope_dispatch(D, interleaved != 0, a.per_row, [&](auto d, auto il, auto per_row) {
+    b200::rope::norm_rope_kernel<decltype(d)::value, decltype(il)::value,
+                                 decltype(per_row)::value>
+        <<<static_cast<unsigned>(grid), b200::rope::kThreads, 0,
            reinterpret_cast<cudaStream_t>(stream)>>>(a.p);
-  return check_launch("qk_norm_rope launch");
+    return check_launch("qk_norm_rope launch");
+  });
 }
 
 b200_status qk_norm_rope_bwd_workspace(int B, int S, int D, size_t* bytes) {
   if (!bytes || B < 1 || S < 1) return fail(B200_EINVAL, "qk_norm_rope_bwd_workspace: bad argument");
   // The grid never exceeds its CTAs per SM, whatever the shape.
-  *bytes = static_cast<size_t>(sm_count()) * b200::rope::kGradCtasPerSm * 2 * D * sizeof(float);
+  *bytes = static_cast<size_t>(sm_count()) * b200::rope::kGradCtasPerSm * D * sizeof(float);
   return B200_OK;
 }
 
@@ -337,27 +573,28 @@ b200_status qk_norm_rope_bwd(const b200_tensor* dq_out, const b200_tensor* dk_ou
   if ((st = check_tensor(who, "dq", dq, B, Hq, S, D, true)) != B200_OK) return st;
   if ((st = check_tensor(who, "dk", dk, B, Hkv, S, D, true)) != B200_OK) return st;
   if (!dq_weight || !dk_weight) return fail(B200_EINVAL, "%s: null weight gradient", who);
-  const int grid = rope_bwd_grid(a.p.tokens, a.p.block);
+  const RopeGrid ctas = rope_bwd_grid(a);
+  const int grid = ctas.q + ctas.k;
+  a.p.ctas_q = ctas.q;
   if ((st = check_workspace(who, workspace, workspace_bytes,
-                            static_cast<size_t>(grid) * 2 * D * sizeof(float))) != B200_OK)
+                            static_cast<size_t>(grid) * D * sizeof(float))) != B200_OK)
     return st;
   a.p.qy = view_of(dq_out);
   a.p.ky = view_of(dk_out);
   a.p.qdx = view_of(dq);
   a.p.kdx = view_of(dk);
   a.p.dw_part = static_cast<float*>(workspace);
-  using Kernel = void (*)(b200::rope::Params);
-  const Kernel kernel =
-      D == 128 ? (a.interleaved ? b200::rope::norm_rope_bwd_kernel<128, true>
-                                : b200::rope::norm_rope_bwd_kernel<128, false>)
-               : (a.interleaved ? b200::rope::norm_rope_bwd_kernel<64, true>
-                                : b200::rope::norm_rope_bwd_kernel<64, false>);
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  kernel<<<grid, b200::rope::kThreads, 0, cs>>>(a.p);
-  if ((st = check_launch("qk_norm_rope_bwd launch")) != B200_OK) return st;
-  b200::rope::norm_rope_dw_kernel<<<2 * D / 32, 256, 0, cs>>>(a.p.dw_part, grid, D, dq_weight,
-                                                              dk_weight);
-  return check_launch("qk_norm_rope_bwd weight launch");
+  st = rope_dispatch(D, interleaved != 0, a.per_row, [&](auto d, auto il, auto per_row) {
+    b200::rope::norm_rope_bwd_kernel<decltype(d)::value, decltype(il)::value,
+                                     decltype(per_row)::value>
+        <<<grid, b200::rope::kThreads, 0, cs>>>(a.p);
+    return check_launch("qk_norm_rope_bwd launch");
+  });
+  if (st != B200_OK) return st;
+  return launch_dependent(b200::rope::norm_rope_dw_kernel, 2 * D / 8, 512, cs,
+                          "qk_norm_rope_bwd weight launch", a.p.dw_part, ctas.q, grid, D,
+                          dq_weight, dk_weight);
 }
 
 b200_status attention_window_fwd_workspace(int B, int Hq, int Hkv, int Sq, int Skv, int D,
@@ -384,6 +621,9 @@ b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, con
   const WindowPlan plan = window_plan(s);
   if ((st = check_workspace(who, workspace, workspace_bytes, plan.bytes)) != B200_OK) return st;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+  if (plan.tiles)
+    return D == 128 ? launch_window_tiles<128>(s, q, k, v, o, lse, kv_len, cs)
+                    : launch_window_tiles<64>(s, q, k, v, o, lse, kv_len, cs);
   b200::split::Params p = split_params(s, q, k, v, o, kv_len, plan.nsplit);
   p.lse = lse;
   const int64_t rows = static_cast<int64_t>(B) * Hkv * plan.nsplit * p.rows;
@@ -487,8 +727,9 @@ b200_status attention_shared_prefix_workspace(int B, int Hq, int Hkv, int Sq, in
   WindowShape own;
   const b200_status st = prefix_shape(who, B, Hq, Hkv, Sq, P, S, D, -1.0f, &own);
   if (st != B200_OK) return st;
-  const PrefixPlan plan = prefix_plan(own, P);
-  *bytes = plan.prefix_bytes + plan.own_bytes;
+  const b200_tensor shared{nullptr, 0, 0, 0};  // a q that is broadcast
+  const PrefixPlan plan = prefix_plan(own, P, nullptr), other = prefix_plan(own, P, &shared);
+  *bytes = std::max(plan.prefix_bytes, other.prefix_bytes) + plan.own_bytes;
   return B200_OK;
 }
 
@@ -503,7 +744,7 @@ b200_status attention_shared_prefix(const b200_tensor* q, const b200_tensor* k_p
   b200_status st = prefix_shape(who, B, Hq, Hkv, Sq, P, S, D, softmax_scale, &own);
   if (st != B200_OK) return st;
   if ((st = check_qkvo(who, own, q, k, v, o)) != B200_OK) return st;
-  const PrefixPlan plan = prefix_plan(own, P);
+  const PrefixPlan plan = prefix_plan(own, P, q);
   if (P > 0) {
     if ((st = check_tensor(who, "k_prefix", k_prefix, 1, Hkv, P, D, false)) != B200_OK) return st;
     if ((st = check_tensor(who, "v_prefix", v_prefix, 1, Hkv, P, D, false)) != B200_OK) return st;
@@ -523,20 +764,32 @@ b200_status attention_shared_prefix(const b200_tensor* q, const b200_tensor* k_p
   c.rows = c.group * Sq;
   c.o = view_of(o);
   if (P > 0) {
-    WindowShape shared = own;
-    shared.Skv = shared.window = P;
-    b200::split::Params p =
-        split_params(shared, q, k_prefix, v_prefix, o, nullptr, plan.prefix_splits);
-    p.B = 1;
-    p.step = 0;
-    p.rows = B * c.rows;
-    p.row_tiles = row_tiles_of(p.rows);
-    part_pointers(workspace, static_cast<int64_t>(Hkv) * p.nsplit * p.rows, D, &p.part_o,
-                  &p.part_ml);
-    if ((st = launch(p)) != B200_OK) return st;
-    c.part_b = p.part_o;
-    c.ml_b = p.part_ml;
-    c.nb = p.nsplit;
+    float* part_o;
+    float2* part_ml;
+    part_pointers(workspace, static_cast<int64_t>(Hkv) * plan.prefix_splits * B * c.rows, D,
+                  &part_o, &part_ml);
+    if (plan.tiles) {
+      st = D == 128 ? launch_prefix_tiles<128>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
+                                               part_o, part_ml, cs)
+                    : launch_prefix_tiles<64>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
+                                              part_o, part_ml, cs);
+    } else {
+      WindowShape shared = own;
+      shared.Skv = shared.window = P;
+      b200::split::Params p =
+          split_params(shared, q, k_prefix, v_prefix, o, nullptr, plan.prefix_splits);
+      p.B = 1;
+      p.step = 0;
+      p.rows = B * c.rows;
+      p.row_tiles = row_tiles_of(p.rows);
+      p.part_o = part_o;
+      p.part_ml = part_ml;
+      st = launch(p);
+    }
+    if (st != B200_OK) return st;
+    c.part_b = part_o;
+    c.ml_b = part_ml;
+    c.nb = plan.prefix_splits;
   }
   b200::split::Params p = split_params(own, q, k, v, o, kv_len, plan.own_splits);
   if (plan.own_bytes > 0)

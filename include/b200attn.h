@@ -133,8 +133,9 @@ b200_status attention_fwd_scalar(const void* q, const void* k, const void* v, vo
  * The data is 16-byte aligned and the strides are multiples of 8, so a view
  * of a fused projection's [B, S, heads, D] output, or of a cache with room
  * for more tokens, is a tensor.  The stride of an axis of length 1 is not
- * used.  An input's stride may be 0 (broadcast); the rows of an output may not
- * overlap, and an output overlaps an input only where an entry point allows it.
+ * used.  An input's batch or head stride may be 0 (broadcast); the rows of an
+ * output may not overlap, and an output overlaps an input only where an entry
+ * point allows it.
  */
 typedef struct {
   const void* data;
@@ -148,7 +149,7 @@ typedef struct {
  * (i, i + rotary_dim/2), or (2i, 2i + 1) if interleaved; columns from
  * rotary_dim on are only normalised.  The angle is formed in 64 bits.
  *   q, q_out: [B, Hq, S, D]   k, k_out: [B, Hkv, S, D]   D in {64, 128}
- *   q_weight, k_weight: [D], bf16 or (weight_f32) fp32
+ *   q_weight, k_weight: [D], bf16 or (weight_f32) fp32, 16-byte aligned
  *   inv_freq: [rotary_dim/2]; rotary_dim a multiple of 16, 0..D
  *   positions[b * position_stride_b + s]; stride 0 shares them over the batch
  * An output may be its own input (same data and strides).

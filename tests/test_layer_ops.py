@@ -25,7 +25,7 @@ def window(q=None, k=None, v=None, o=None, B=2, Hq=8, Hkv=2, Sq=64, Skv=1024, D=
     (dict(q=T(0)), 1, "null"), (dict(k=T(24)), 1, "aligned"), (dict(v=T(ss=129)), 1, "multiples"),
     (dict(k=T(sh=-8)), 1, "negative"), (dict(o=T(sh=0)), 1, "overlap"),
     (dict(o=T(ss=64)), 1, "overlap"), (dict(o=T(sb=1024)), 1, "overlap"),
-    (dict(q=T(sb=1 << 39)), 2, "2^39"), (dict(B=0), 1, "shape"), (dict(Sq=0), 1, "shape"),
+    (dict(k=T(ss=0)), 1, "share a row"), (dict(q=T(sb=1 << 39)), 2, "2^39"), (dict(B=0), 1, "shape"), (dict(Sq=0), 1, "shape"),
     (dict(Skv=0), 1, "shape"), (dict(Hq=7), 1, "Hkv"), (dict(D=96), 2, "head_dim"),
     (dict(W=0), 1, "window"), (dict(sinks=-1), 1, "sinks"), (dict(scale=math.inf), 1, "scale"),
     (dict(scale=math.nan), 1, "scale"), (dict(Skv=(1 << 30) + 1), 2, "2^30"),
@@ -82,10 +82,11 @@ def rope(q=None, k=None, qo=None, ko=None, wq=256, wk=256, freq=256, R=128, pos=
 
 @pytest.mark.parametrize("bad,status,word", [
     (dict(q=T(0)), 1, "q"), (dict(ko=T(ss=8)), 1, "k_out"), (dict(k=T(ss=12)), 1, "k"),
-    (dict(wq=None), 1, "weight"), (dict(freq=None), 1, "inv_freq"), (dict(pos=None), 1, "positions"),
+    (dict(wq=None), 1, "weight"), (dict(wk=260), 1, "weights must"), (dict(freq=None), 1, "inv_freq"), (dict(pos=None), 1, "positions"),
     (dict(R=24), 2, "rotary_dim"), (dict(R=144), 2, "rotary_dim"), (dict(R=-16), 2, "rotary_dim"),
     (dict(eps=-1.0), 1, "eps"), (dict(eps=math.nan), 1, "eps"), (dict(D=80), 2, "head_dim"),
-    (dict(S=0), 1, "shape"), (dict(pos_sb=-1), 1, "stride"), (dict(Hq=5000), 2, "heads"),
+    (dict(S=0), 1, "shape"), (dict(pos_sb=-1), 1, "stride"), (dict(S=1 << 30), 2, "tokens"),
+    (dict(Hkv=(1 << 20) + 1), 2, "heads"),
 ])
 def test_norm_rope_refuses(bad, status, word):
     assert rope(**bad) == status

@@ -49,6 +49,9 @@ ROPE = [  # B, S, Hq, Hkv, D, R, interleaved, w32
     (4, 2100, 5, 2, 128, 16, True, False),
     (1, 40, 64, 8, 128, 0, False, False),
     (2, 4500, 32, 8, 128, 128, False, True),
+    (3, 77, 2, 1, 128, 128, False, True),   # few heads: a token to each row of a warp
+    (2, 1301, 2, 2, 64, 64, True, False),
+    (1, 3, 1, 1, 64, 32, False, False),
 ]
 
 
@@ -150,6 +153,13 @@ WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks, lens
     (1, 8, 2, 1111, 1111, 128, 256, 128, None),
     (2, 4, 1, 515, 515, 64, 100, 500, [515, 300]),
     (1, 2, 1, 1024, 4096, 128, 2000, 1000, None),
+    # enough rows for 128-row tiles
+    (6, 8, 2, 300, 517, 128, 128, 4, [517, 200, 0, 300, 299, 1]),
+    (4, 16, 4, 260, 1000, 64, 1 << 40, 0, [1000, 260, 17, 999]),
+    (2, 16, 2, 515, 515, 64, 100, 500, [515, 300]),
+    (1, 32, 8, 1024, 4096, 128, 2000, 1000, None),
+    (16, 32, 8, 64, 700, 128, 300, 5, [700] * 8 + [65, 64, 63, 0, 1, 128, 300, 699]),
+    (1, 8, 1, 2048, 2048, 128, 256, 130, None),
 ]
 
 
@@ -298,6 +308,10 @@ PREFIX = [  # B, Hq, Hkv, Sq, P, S, D, lens
     (5, 16, 1, 4, 129, 2000, 128, [2000, 0, 3, 1500, 64]),
     (70, 8, 2, 1, 3001, 5, 128, None),
     (2, 48, 16, 2, 127, 9, 64, [9, 2]),
+    (40, 16, 16, 1, 5003, 20, 64, None),
+    (25, 40, 8, 3, 3000, 30, 128, None),
+    (3, 64, 1, 2, 9000, 10, 128, None),
+    (2, 192, 2, 2, 9000, 10, 128, [1, 10]),  # more rows of a request than a tile has
 ]
 
 
@@ -316,6 +330,16 @@ def test_shared_prefix(case):
     ops.check()
     U.check_close(o, *U.shared_prefix(q, kp, vp, k, v, n), "o")
     assert torch.equal(o, ops.attention_shared_prefix(q, kp, vp, k, v, kv_len=n))
+
+
+def test_shared_prefix_broadcast_queries():
+    g = gen(14)
+    q = randn(g, 1, 16, 1, 128).expand(40, 16, 1, 128)
+    kp, vp = randn(g, 1, 4000, 128).expand(2, 4000, 128), randn(g, 2, 4000, 128)
+    k, v = randn(g, 40, 2, 9, 128), randn(g, 1, 2, 9, 128).expand(40, 2, 9, 128)
+    o = ops.attention_shared_prefix(q, kp, vp, k, v)
+    ops.check()
+    U.check_close(o, *U.shared_prefix(q, kp, vp, k, v, i32([9] * 40)), "o")
 
 
 def test_shared_prefix_strides_and_default_lengths():
