@@ -405,6 +405,98 @@ b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, cons
   return launch_tiles<D, b200::attn::kWindow>(qm, km, vm, om, p, planes * p.n_qtiles, stream);
 }
 
+// ---- window attention's gradients ----
+struct WindowGrads {
+  const b200_tensor *dout, *q, *k, *v, *o, *dq, *dk, *dv;
+  const float* lse;
+  const int32_t* kv_len;
+};
+
+int64_t padded_queries(int Sq) { return (static_cast<int64_t>(Sq) + 63) / 64 * 64; }
+
+size_t window_bwd_bytes(int B, int Hq, int Sq) {
+  return static_cast<size_t>(B) * Hq * padded_queries(Sq) * 2 * sizeof(float);
+}
+
+template <int D, bool kKeys>
+b200_status launch_bwd_tiles(const CUtensorMap (&m)[4], b200::bwd::TileParams p, int heads,
+                             int rows, cudaStream_t stream) {
+  using C = b200::bwd::TileCfg<D, kKeys>;
+  static unsigned attr_done = 0;
+  auto kernel = b200::bwd::bwd_tile_kernel<D, kKeys>;
+  const b200_status st = ensure_smem_attr(kernel, C::kSmemBytes, &attr_done);
+  if (st != B200_OK) return st;
+  p.tiles = (rows + b200::bwd::kOwn - 1) / b200::bwd::kOwn;
+  const int64_t items = static_cast<int64_t>(p.B) * heads * p.tiles;
+  if (items > 0x3fffffffll) return fail(B200_EUNSUPPORTED, "attention_window_bwd: too many tiles");
+  p.n_items = static_cast<int>(items);
+  // Key tiles differ in length (sinks): a CTA each, so that the next one starts
+  // where one ends.  Query tiles are alike: persistent CTAs.
+  const unsigned grid = static_cast<unsigned>(kKeys ? items : std::min<int64_t>(items, sm_count()));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(b200::bwd::kTileThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = kKeys ? 1 : 0;  // the keys' launch follows the row statistics'
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], p);
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, "attention_window_bwd launch");
+}
+
+template <int D>
+b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* workspace,
+                             cudaStream_t stream) {
+  b200::bwd::TileParams p{};
+  p.sq_pad = static_cast<int>(padded_queries(s.Sq));
+  p.stat_plane = static_cast<int64_t>(s.B) * s.Hq * p.sq_pad;
+  float* stats = static_cast<float*>(workspace);
+  p.stats = stats;
+  p.kv_len = t.kv_len;
+  p.B = s.B;
+  p.Hq = s.Hq;
+  p.Hkv = s.Hkv;
+  p.group = s.Hq / s.Hkv;
+  p.Sq = s.Sq;
+  p.Skv = s.Skv;
+  p.window = s.window;
+  p.sinks = s.sinks;
+  p.scale = s.scale;
+  p.scale_log2 = s.scale * 1.4426950408889634f;
+  // [0]: 128-row boxes, [1]: 64-row boxes of the queries' tensors.
+  CUtensorMap q[2], dout[2], k, v;
+  int q_b, q_h, do_b, do_h, k_b, k_h, v_b, v_h;
+  b200_status st;
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t rows = i ? 64 : 128;
+    if ((st = encode_view(&q[i], t.q, s.B, s.Hq, s.Sq, D, rows, &q_b, &q_h)) != B200_OK ||
+        (st = encode_view(&dout[i], t.dout, s.B, s.Hq, s.Sq, D, rows, &do_b, &do_h)) != B200_OK)
+      return st;
+  }
+  if ((st = encode_view(&k, t.k, s.B, s.Hkv, s.Skv, D, 128, &k_b, &k_h)) != B200_OK ||
+      (st = encode_view(&v, t.v, s.B, s.Hkv, s.Skv, D, 128, &v_b, &v_h)) != B200_OK)
+    return st;
+  const int64_t blocks = (p.stat_plane + 7) / 8;
+  if (blocks > 0x7fffffffll)
+    return fail(B200_EUNSUPPORTED, "attention_window_bwd: too many query rows");
+  b200::bwd::stats_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+      view_of(t.dout), view_of(t.o), t.lse, stats, p.stat_plane, p.sq_pad, s.B, s.Hq, s.Sq);
+  if ((st = check_launch("attention_window_bwd statistics")) != B200_OK) return st;
+  p.out1 = view_of(t.dk);
+  p.out2 = view_of(t.dv);
+  p.o1_b = k_b, p.o1_h = k_h, p.o2_b = v_b, p.o2_h = v_h;
+  p.s1_b = q_b, p.s1_h = q_h, p.s2_b = do_b, p.s2_h = do_h;
+  if ((st = launch_bwd_tiles<D, true>({k, v, q[1], dout[1]}, p, s.Hkv, s.Skv, stream)) != B200_OK)
+    return st;
+  p.out1 = p.out2 = view_of(t.dq);
+  p.o1_b = q_b, p.o1_h = q_h, p.o2_b = do_b, p.o2_h = do_h;
+  p.s1_b = k_b, p.s1_h = k_h, p.s2_b = v_b, p.s2_h = v_h;
+  return launch_bwd_tiles<D, false>({q[0], dout[0], k, v}, p, s.Hq, s.Sq, stream);
+}
+
 // Tiles of the prefix form: whole batches, up to 128 rows.
 struct PrefixTiles {
   int batches, rows, count;  // of a tile; tiles
@@ -647,7 +739,7 @@ b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, con
 b200_status attention_window_bwd_workspace(int B, int Hq, int Sq, size_t* bytes) {
   if (!bytes || B < 1 || Hq < 1 || Sq < 1)
     return fail(B200_EINVAL, "attention_window_bwd_workspace: bad argument");
-  *bytes = static_cast<size_t>(B) * Hq * Sq * sizeof(float);
+  *bytes = window_bwd_bytes(B, Hq, Sq);
   return B200_OK;
 }
 
@@ -671,8 +763,15 @@ b200_status attention_window_bwd(const b200_tensor* dout, const b200_tensor* q,
   if ((st = check_tensor(who, "dk", dk, B, Hkv, Skv, D, true)) != B200_OK) return st;
   if ((st = check_tensor(who, "dv", dv, B, Hkv, Skv, D, true)) != B200_OK) return st;
   if (!lse) return fail(B200_EINVAL, "%s: null lse", who);
-  const size_t need = static_cast<size_t>(B) * Hq * Sq * sizeof(float);
-  if ((st = check_workspace(who, workspace, workspace_bytes, need)) != B200_OK) return st;
+  if ((st = check_workspace(who, workspace, workspace_bytes, window_bwd_bytes(B, Hq, Sq))) !=
+      B200_OK)
+    return st;
+  if (!(std::getenv("B200_TILES") && std::getenv("B200_TILES")[0] == '0')) {
+    const WindowGrads t{dout, q, k, v, o, dq, dk, dv, lse, kv_len};
+    const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+    return D == 128 ? window_bwd_tiles<128>(s, t, workspace, cs)
+                    : window_bwd_tiles<64>(s, t, workspace, cs);
+  }
   namespace bw = b200::bwd;
   bw::Params p{};
   p.dout = view_of(dout);
