@@ -438,7 +438,7 @@ b200_status launch_bwd_tiles(const CUtensorMap (&m)[4], b200::bwd::TileParams p,
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(b200::bwd::kTileThreads, 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -479,7 +479,8 @@ b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* w
   if ((st = encode_view(&k, t.k, s.B, s.Hkv, s.Skv, D, 128, &k_b, &k_h)) != B200_OK ||
       (st = encode_view(&v, t.v, s.B, s.Hkv, s.Skv, D, 128, &v_b, &v_h)) != B200_OK)
     return st;
-  const int64_t blocks = (p.stat_plane + 7) / 8;
+  constexpr int kRowsPerBlock = 4 * 256 / (D / 8);
+  const int64_t blocks = (p.stat_plane + kRowsPerBlock - 1) / kRowsPerBlock;
   if (blocks > 0x7fffffffll)
     return fail(B200_EUNSUPPORTED, "attention_window_bwd: too many query rows");
   b200::bwd::stats_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(

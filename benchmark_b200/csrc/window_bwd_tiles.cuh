@@ -16,9 +16,9 @@
 // step's S and dP run while this step's P is computed.  kKeys steps are 64
 // queries wide: two accumulators of D columns leave no room for 128.
 //
-// Roles: warps 0-7 elementwise (warp w: lanes 32 (w % 4), columns half w / 4)
-// and epilogue; warp 8 TMA; warp 9 issues S and dP; warp 10 the accumulating
-// products.  Waits are bounded as in the forward kernel.
+// Roles: elementwise and epilogue warps (warp w: lanes 32 (w % 4), the w / 4th
+// share of the columns), then a TMA warp, one that issues S and dP and one that
+// issues the accumulating products.  Waits are bounded as in the forward kernel.
 #pragma once
 
 #include "attention_kernel.cuh"
@@ -28,13 +28,23 @@
 namespace b200 {
 namespace bwd {
 
-constexpr int kTileThreads = 384;
 constexpr int kOwn = 128;  // owned rows
 
 template <int D, bool kKeys>
 struct TileCfg {
   static constexpr int kN = kKeys ? 64 : 128;  // streamed rows of a step
-  static constexpr int kStages = (kKeys ? 4 : 2) * (128 / D);
+  static constexpr int kGroups = 4;                 // elementwise warpgroups
+  static constexpr int kWarps = 4 * kGroups;     // elementwise warps
+  static constexpr int kCols = kN / kGroups;     // columns of a step for each
+  static constexpr int kThreads = 32 * (kWarps + 4);
+  // Epilogue: warpgroups of an accumulator, columns for each.
+  static constexpr int kAccGroups = kKeys ? kGroups / 2 : kGroups;
+  static constexpr int kAccCols = D / kAccGroups;
+  // Ring depths of the two streamed tensors.  Both of kKeys' live until the
+  // accumulating products have read them, but V only until dP has: K gets the
+  // odd stage.
+  static constexpr int kStages1 = (kKeys ? 4 : 3) * (128 / D);
+  static constexpr int kStages2 = (kKeys ? 4 : 2) * (128 / D);
   static constexpr int kBoxes = D / 64;
   static constexpr int kOwnBox = kOwn * 128;
   static constexpr int kOwnBytes = kBoxes * kOwnBox;
@@ -42,10 +52,11 @@ struct TileCfg {
   static constexpr int kStrBytes = kBoxes * kStrBox;
   static constexpr int kStatBytes = kKeys ? 2 * kN * 4 : 0;  // -lse, -delta of the queries
   static constexpr int kRingOff = 2 * kOwnBytes;
-  static constexpr int kStatOff = kRingOff + kStages * 2 * kStrBytes;
-  static constexpr int kBarOff = kStatOff + kStages * kStatBytes;
+  static constexpr int kRing2Off = kRingOff + kStages1 * kStrBytes;
+  static constexpr int kStatOff = kRing2Off + kStages2 * kStrBytes;
+  static constexpr int kBarOff = kStatOff + kStages2 * kStatBytes;
   // own_full own_empty s_ready dp_ready s_free p_ready p_free acc_full acc_empty drain
-  static constexpr int kNumBars = 10 + 2 * kStages;
+  static constexpr int kNumBars = 10 + 2 * (kStages1 + kStages2);
   static constexpr int kSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kSlotOff + 16 + 1024;  // + alignment slack
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
@@ -74,38 +85,52 @@ struct TileParams {
 };
 
 enum : uint32_t {
-  kSiteBwdOwn = 0x20, kSiteBwdFull, kSiteBwdEmpty, kSiteBwdS, kSiteBwdDp, kSiteBwdSFree,
+  kSiteBwdOwn = 0x20, kSiteBwdFull, kSiteBwdEmpty, kSiteBwdS, kSiteBwdDp,
   kSiteBwdP, kSiteBwdPFree, kSiteBwdAcc
 };
 
-// -lse and -delta of every query row, padded with zeros; one warp to a row.
+// -lse and -delta of every query row, padded with zeros.  D/8 lanes to a row
+// (16 bytes each of dO and O), four rows of each in flight.
 template <int D>
 __global__ void __launch_bounds__(256)
     stats_kernel(const View dout, const View o, const float* lse, float* stats, int64_t plane,
                  int sq_pad, int B, int Hq, int Sq) {
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = 4;
   pdl_launch_dependents();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + warp_id();
-  if (row >= plane) return;
-  const int64_t bh = row / sq_pad, s = row - bh * sq_pad, b = bh / Hq, h = bh - b * Hq;
-  float sum = 0.0f, l = 0.0f;
-  if (s < Sq) {
-    const uint16_t* x = dout.row(b, h, s);
-    const uint16_t* y = o.row(b, h, s);
+  const int lane = static_cast<int>(threadIdx.x) % kLanes;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kUnroll) +
+                       static_cast<int>(threadIdx.x) / kLanes;
+  uint4 x[kUnroll], y[kUnroll];
+  float l[kUnroll];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const int c = i * 32 + static_cast<int>(lane_id());
-      const uint32_t a = reinterpret_cast<const uint32_t*>(x)[c];
-      const uint32_t e = reinterpret_cast<const uint32_t*>(y)[c];
-      sum = fmaf(__uint_as_float(a << 16), __uint_as_float(e << 16), sum);
-      sum = fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(e & 0xffff0000u), sum);
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t row = row0 + u * kRows;
+    x[u] = y[u] = make_uint4(0u, 0u, 0u, 0u);
+    l[u] = 0.0f;
+    const int64_t bh = row / sq_pad, s = row - bh * sq_pad, b = bh / Hq, h = bh - b * Hq;
+    if (row < plane && s < Sq) {
+      x[u] = __ldg(reinterpret_cast<const uint4*>(dout.row(b, h, s)) + lane);
+      y[u] = __ldg(reinterpret_cast<const uint4*>(o.row(b, h, s)) + lane);
+      l[u] = __ldg(lse + bh * Sq + s);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t row = row0 + u * kRows;
+    const uint32_t a[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+    const uint32_t e[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(e[i] << 16), sum);
+      sum = fmaf(__uint_as_float(a[i] & 0xffff0000u), __uint_as_float(e[i] & 0xffff0000u), sum);
     }
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    l = lse[bh * Sq + s];
-  }
-  if (lane_id() == 0) {
-    stats[row] = l == -INFINITY ? 0.0f : l * -1.4426950408889634f;
-    stats[plane + row] = -sum;
+    for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    if (lane == 0 && row < plane) {
+      stats[row] = l[u] == -INFINITY ? 0.0f : l[u] * -1.4426950408889634f;
+      stats[plane + row] = -sum;
+    }
   }
 }
 
@@ -117,6 +142,18 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
+
+// TMEM loads and stores of a thread's columns.
+__device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t (&r)[16]) {
+  tmem_st16(taddr, r);
+}
+__device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t (&r)[8]) {
+  tmem_st8(taddr, r);
+}
+__device__ __forceinline__ void written_here(uint32_t (&r)[32]) { reg_written_here(r); }
+__device__ __forceinline__ void written_here(uint32_t (&r)[16]) { reg_written_here16(r); }
 
 // One owned tile: where it lies and what it streams.
 template <bool kKeys>
@@ -166,8 +203,53 @@ __device__ __forceinline__ TileItem<kKeys> tile_item(const TileParams& p, int k)
   return it;
 }
 
+// P and dS of kCols columns of this thread's row, as bf16 pairs.  kKeys: -lse and
+// -delta of the columns at st_l and st_l + n; else the row's own.
+template <bool kKeys, bool kMasked, int kCols>
+__device__ __forceinline__ void elementwise(const uint32_t (&s)[kCols], const uint32_t (&d)[kCols],
+                                            uint64_t c2, const float* st_l, int n, float nlse,
+                                            float ndelta, int col0, int va, int vb, int vs,
+                                            uint32_t (&pk)[kCols / 2],
+                                            uint32_t (&dk)[kCols / 2]) {
+#pragma unroll
+  for (int e = 0; e < kCols / 2; ++e) {
+    uint64_t nl2, nd2;
+    if constexpr (kKeys) {
+      nl2 = *reinterpret_cast<const uint64_t*>(st_l + 2 * e);
+      nd2 = *reinterpret_cast<const uint64_t*>(st_l + n + 2 * e);
+    } else {
+      nl2 = f2_pack(nlse, nlse);
+      nd2 = f2_pack(ndelta, ndelta);
+    }
+    const uint64_t x2 =
+        f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, nl2);
+    float x0, x1;
+    f2_unpack(x2, x0, x1);
+    float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+    const uint64_t g2 =
+        f2_mul(f2_pack(p0, p1),
+               f2_add(f2_pack(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1])), nd2));
+    float g0, g1;
+    f2_unpack(g2, g0, g1);
+    if constexpr (kMasked) {
+      const int u = col0 + 2 * e;
+      bool see0 = u >= va && u < vb, see1 = u + 1 >= va && u + 1 < vb;
+      if constexpr (!kKeys) {
+        see0 |= u < vs;
+        see1 |= u + 1 < vs;
+      }
+      p0 = see0 ? p0 : 0.0f;
+      p1 = see1 ? p1 : 0.0f;
+      g0 = see0 ? g0 : 0.0f;
+      g1 = see1 ? g1 : 0.0f;
+    }
+    if constexpr (kKeys) pk[e] = pack_bf16x2(p0, p1);
+    dk[e] = pack_bf16x2(g0, g1);
+  }
+}
+
 template <int D, bool kKeys>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
     bwd_tile_kernel(const __grid_constant__ CUtensorMap own1_map,
                     const __grid_constant__ CUtensorMap own2_map,
                     const __grid_constant__ CUtensorMap str1_map,
@@ -178,13 +260,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* own = smem;
-  uint8_t* ring = smem + C::kRingOff;
+  uint8_t* ring1 = smem + C::kRingOff;
+  uint8_t* ring2 = smem + C::kRing2Off;
   float* stat = reinterpret_cast<float*>(smem + C::kStatOff);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
   uint64_t *own_full = bars, *own_empty = bars + 1, *s_ready = bars + 2, *dp_ready = bars + 3,
            *s_free = bars + 4, *p_ready = bars + 5, *p_free = bars + 6, *acc_full = bars + 7,
-           *acc_empty = bars + 8, *drain = bars + 9, *full = bars + 10,
-           *empty = bars + 10 + C::kStages;
+           *acc_empty = bars + 8, *drain = bars + 9, *full1 = bars + 10,
+           *empty1 = full1 + C::kStages1, *full2 = empty1 + C::kStages1,
+           *empty2 = full2 + C::kStages2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kSlotOff);
   const int warp = static_cast<int>(warp_id()), lane = static_cast<int>(lane_id());
 
@@ -193,19 +277,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(own_empty, 1);
     mbar_init(s_ready, 1);
     mbar_init(dp_ready, 1);
-    mbar_init(s_free, 8);
-    mbar_init(p_ready, 8);
+    mbar_init(s_free, C::kWarps);
+    mbar_init(p_ready, C::kWarps);
     mbar_init(p_free, 1);
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 8);
+    mbar_init(acc_empty, C::kWarps);
     mbar_init(drain, 2);
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
+    for (int i = 0; i < 2 * (C::kStages1 + C::kStages2); ++i) mbar_init(&full1[i], 1);
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == C::kWarps) {
     tmem_alloc(slot, 512);
     tmem_relinquish();
     if (lane == 0) {
@@ -235,11 +316,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       return it.h;
   };
 
-  if (warp == 8) {
+  if (warp == C::kWarps) {
     // ================= TMA producer =================
     if (lane == 0) {
       const uint64_t pol_own = l2_policy_evict_first(), pol_str = l2_policy_evict_last();
-      int t = 0, li = 0;
+      int t = 0, li = 0, n1 = 0, n2 = 0;  // steps; copies issued
       bool ok = true;
       for (int k = static_cast<int>(blockIdx.x); k < p.n_items && ok; k += gridDim.x) {
         const TileItem<kKeys> it = tile_item<kKeys>(p, k);
@@ -256,45 +337,56 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         ++li;
         for (int i = 0; i < it.steps; ++i, ++t) {
-          const int st = t % C::kStages;
-          ok = mbar_wait(&empty[st], (static_cast<uint32_t>(t / C::kStages) & 1u) ^ 1u,
-                         kSiteBwdEmpty, kDefaultWaitLimitNs, 20000u);
-          if (!ok) break;
+          const int st1 = t % C::kStages1, st2 = t % C::kStages2;
           const int row = str_row(it, i), hq = query_head(it, i);
           const int h = kKeys ? hq : it.h / p.group;
-          mbar_arrive_expect_tx(&full[st], 2 * C::kStrBytes + C::kStatBytes);
-          uint8_t* dst = ring + st * 2 * C::kStrBytes;
-          for (int x = 0; x < C::kBoxes; ++x) {
-            tma_load_4d(dst + x * C::kStrBox, &str1_map, &full[st], x * 64, row, h * p.s1_h,
-                        it.b * p.s1_b, pol_str);
-            tma_load_4d(dst + C::kStrBytes + x * C::kStrBox, &str2_map, &full[st], x * 64, row,
-                        h * p.s2_h, it.b * p.s2_b, pol_str);
-          }
+          ok = mbar_wait(&empty1[st1], (static_cast<uint32_t>(t / C::kStages1) & 1u) ^ 1u,
+                         kSiteBwdEmpty, kDefaultWaitLimitNs, 20000u);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full1[st1], C::kStrBytes);
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_4d(ring1 + st1 * C::kStrBytes + x * C::kStrBox, &str1_map, &full1[st1],
+                        x * 64, row, h * p.s1_h, it.b * p.s1_b, pol_str);
+          n1 = t + 1;
+          ok = mbar_wait(&empty2[st2], (static_cast<uint32_t>(t / C::kStages2) & 1u) ^ 1u,
+                         kSiteBwdEmpty, kDefaultWaitLimitNs, 20000u);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full2[st2], C::kStrBytes + C::kStatBytes);
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_4d(ring2 + st2 * C::kStrBytes + x * C::kStrBox, &str2_map, &full2[st2],
+                        x * 64, row, h * p.s2_h, it.b * p.s2_b, pol_str);
           if constexpr (kKeys) {
             const float* src =
                 p.stats + (static_cast<int64_t>(it.b) * p.Hq + hq) * p.sq_pad + row;
-            float* sdst = stat + st * 2 * C::kN;
-            bulk_load(sdst, src, C::kN * 4, &full[st]);
-            bulk_load(sdst + C::kN, src + p.stat_plane, C::kN * 4, &full[st]);
+            float* sdst = stat + st2 * 2 * C::kN;
+            bulk_load(sdst, src, C::kN * 4, &full2[st2]);
+            bulk_load(sdst + C::kN, src + p.stat_plane, C::kN * 4, &full2[st2]);
           }
+          n2 = t + 1;
         }
       }
       if (!ok) {
         // Unwinding: let every copy already issued land before the CTA exits.
         if (li > 0) attn::drain_wait(own_full, static_cast<uint32_t>(li - 1) & 1u);
-        for (int i = max(0, t - C::kStages); i < t; ++i)
-          attn::drain_wait(&full[i % C::kStages], static_cast<uint32_t>(i / C::kStages) & 1u);
+        for (int i = max(0, n1 - C::kStages1); i < n1; ++i)
+          attn::drain_wait(&full1[i % C::kStages1], static_cast<uint32_t>(i / C::kStages1) & 1u);
+        for (int i = max(0, n2 - C::kStages2); i < n2; ++i)
+          attn::drain_wait(&full2[i % C::kStages2], static_cast<uint32_t>(i / C::kStages2) & 1u);
       }
     }
     __syncwarp();
-  } else if (warp == 9 || warp == 10) {
+  } else if (warp == C::kWarps + 1 || warp == C::kWarps + 2) {
     // ================= MMA issuers =================
-    const bool acc = warp == 10;
-    const uint32_t ring_addr = smem_u32(ring), own_addr = smem_u32(own);
+    const bool acc = warp == C::kWarps + 2;
+    const uint32_t own_addr = smem_u32(own);
     const uint64_t d_own1 = sdesc_sw128(own_addr, 16, 1024);
     const uint64_t d_own2 = sdesc_sw128(own_addr + C::kOwnBytes, 16, 1024);
-    const uint64_t d_str = sdesc_sw128(ring_addr, 16, 1024);           // rows as N
-    const uint64_t d_acc = sdesc_sw128(ring_addr, C::kStrBox, 1024);   // rows as K
+    // Streamed tiles with their rows as N (S, dP) and as K (accumulation).
+    const uint64_t d_n1 = sdesc_sw128(smem_u32(ring1), 16, 1024);
+    const uint64_t d_n2 = sdesc_sw128(smem_u32(ring2), 16, 1024);
+    const uint64_t d_k1 = sdesc_sw128(smem_u32(ring1), C::kStrBox, 1024);
+    const uint64_t d_k2 = sdesc_sw128(smem_u32(ring2), C::kStrBox, 1024);
+    constexpr uint32_t kStr16 = C::kStrBytes >> 4;
     auto warp_wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
       const bool ok = attn::warp_wait(bar, parity, site);
       tc_fence_after();
@@ -313,41 +405,47 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       ++li;
       for (int i = 0; i < steps && ok; ++i, ++t) {
-        const int st = t % C::kStages;
-        const uint32_t stage16 = static_cast<uint32_t>(st * 2 * C::kStrBytes) >> 4;
+        const int st1 = t % C::kStages1, st2 = t % C::kStages2;
+        const uint32_t par1 = static_cast<uint32_t>(t / C::kStages1) & 1u;
+        const uint32_t par2 = static_cast<uint32_t>(t / C::kStages2) & 1u;
         if (!acc) {
-          ok = warp_wait(&full[st], static_cast<uint32_t>(t / C::kStages) & 1u, kSiteBwdFull) &&
-               warp_wait(s_free, (static_cast<uint32_t>(t) & 1u) ^ 1u, kSiteBwdSFree);
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait3(smem_u32(&full1[st1]), par1, smem_u32(&full2[st2]), par2,
+                                     smem_u32(s_free), (static_cast<uint32_t>(t) & 1u) ^ 1u,
+                                     kSiteBwdFull));
           if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-          for (int which = 0; which < 2; ++which) {
-            const uint64_t da = which ? d_own2 : d_own1;
-            const uint64_t db = d_str + stage16 + (which ? C::kStrBytes >> 4 : 0);
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss_warp(tmem + C::kColS, d_own1 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
+                        d_n1 + st1 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
+                        C::kIdescS, kk > 0 ? 1u : 0u);
+          mma_commit_warp(s_ready);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              mma_ss_warp(tmem + (which ? C::kColDp : C::kColS),
-                          da + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
-                          db + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2, C::kIdescS,
-                          kk > 0 ? 1u : 0u);
-            mma_commit_warp(which ? dp_ready : s_ready);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss_warp(tmem + C::kColDp, d_own2 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
+                        d_n2 + st2 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
+                        C::kIdescS, kk > 0 ? 1u : 0u);
+          if constexpr (!kKeys) mma_commit_warp(&empty2[st2]);
+          mma_commit_warp(dp_ready);
           if (i + 1 == steps) mma_commit_warp(own_empty);
         } else {
           ok = warp_wait(p_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdP);
           if (!ok) break;
-          const uint64_t db = d_acc + stage16;
           if constexpr (kKeys) {
 #pragma unroll
             for (int kk = 0; kk < C::kN / 16; ++kk)
               mma_ts_warp(tmem + C::kColAcc2, tmem + C::kColP + kk * 8,
-                          db + (C::kStrBytes >> 4) + kk * (2048 >> 4), C::kIdescAcc,
+                          d_k2 + st2 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
                           (i > 0 || kk > 0) ? 1u : 0u);
           }
 #pragma unroll
           for (int kk = 0; kk < C::kN / 16; ++kk)
             mma_ts_warp(tmem + (kKeys ? C::kColAcc1 : C::kColAcc2), tmem + C::kColDs + kk * 8,
-                        db + kk * (2048 >> 4), C::kIdescAcc, (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit_warp(&empty[st]);
+                        d_k1 + st1 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit_warp(&empty1[st1]);
+          if constexpr (kKeys) mma_commit_warp(&empty2[st2]);
           mma_commit_warp(p_free);
           if (i + 1 == steps) mma_commit_warp(acc_full);
         }
@@ -356,9 +454,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mma_commit_warp(drain);
     attn::drain_wait(drain, 0);
     __syncwarp();
-  } else if (warp < 8) {
+  } else if (warp < C::kWarps) {
     // ================= elementwise and epilogue =================
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3, wg = warp >> 2;
+    const int col0 = wg * C::kCols;
     const int row = quad * 32 + lane;
     const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = p.scale_log2;
@@ -375,7 +474,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ndelta = __ldg(src + p.stat_plane);
       }
       for (int i = 0; i < it.steps; ++i, ++t) {
-        const int st = t % C::kStages;
+        const int st1 = t % C::kStages1, st2 = t % C::kStages2;
         const int str0 = str_row(it, i);
         // The streamed columns [va, vb) that this row meets; for queries also
         // those below vs (sinks).  `masked`: some pair of the step is hidden.
@@ -397,77 +496,43 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           masked = it.r0 + kOwn > p.Sq || str0 + 127 > first ||
                    (last - str0 >= p.window && str0 + 128 > p.sinks);
         }
-        ok = attn::warp_wait(s_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdS);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int ch = 0; ch < C::kN / 64; ++ch) {
-          const int col0 = half * (C::kN / 2) + ch * 32;
-          uint32_t s[32], d[32];
-          tmem_ld32(tlane + C::kColS + col0, s);
-          if (ch == 0) {
-            ok = attn::warp_wait(dp_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdDp);
-            if (!ok) {
-              tmem_wait_ld(s);
-              break;
-            }
-            tc_fence_after();
-          }
-          tmem_ld32(tlane + C::kColDp + col0, d);
-          tmem_wait_ld(s);
-          tmem_wait_ld(d);
-          if (ch + 1 == C::kN / 64) {  // the next step's S and dP may overwrite these
-            tc_fence_before();
-            __syncwarp();
-            mbar_arrive_warp(s_free);
-          }
-          const float* st_l = stat + st * 2 * C::kN + col0;
-          uint32_t pk[16], dk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            uint64_t nl2, nd2;
-            if constexpr (kKeys) {
-              nl2 = *reinterpret_cast<const uint64_t*>(st_l + 2 * e);
-              nd2 = *reinterpret_cast<const uint64_t*>(st_l + C::kN + 2 * e);
-            } else {
-              nl2 = f2_pack(nlse, nlse);
-              nd2 = f2_pack(ndelta, ndelta);
-            }
-            const uint64_t x2 = f2_fma(
-                f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, nl2);
-            float x0, x1;
-            f2_unpack(x2, x0, x1);
-            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-            uint64_t g2 = f2_mul(
-                f2_pack(p0, p1),
-                f2_add(f2_pack(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1])), nd2));
-            float g0, g1;
-            f2_unpack(g2, g0, g1);
-            if (masked) {
-              const int u = col0 + 2 * e;
-              bool see0 = u >= va && u < vb, see1 = u + 1 >= va && u + 1 < vb;
-              if constexpr (!kKeys) {
-                see0 |= u < vs;
-                see1 |= u + 1 < vs;
-              }
-              p0 = see0 ? p0 : 0.0f;
-              p1 = see1 ? p1 : 0.0f;
-              g0 = see0 ? g0 : 0.0f;
-              g1 = see1 ? g1 : 0.0f;
-            }
-            if constexpr (kKeys) pk[e] = pack_bf16x2(p0, p1);
-            dk[e] = pack_bf16x2(g0, g1);
-          }
-          if (ch == 0) {
-            // The products of the step before have read P and dS.
-            ok = attn::warp_wait(p_free, (static_cast<uint32_t>(t) & 1u) ^ 1u, kSiteBwdPFree);
-            if (!ok) break;
-            tc_fence_after();
-          }
-          if constexpr (kKeys) tmem_st16(tlane + C::kColP + (col0 >> 1), pk);
-          tmem_st16(tlane + C::kColDs + (col0 >> 1), dk);
+        // kKeys: the columns' statistics came with dO.  (Barriers are polled in
+        // one group: each poll that a branch depends on costs its latency.)
+        {
+          const uint32_t s_bar = smem_u32(s_ready), s_par = static_cast<uint32_t>(t) & 1u;
+          const uint32_t f_bar = kKeys ? smem_u32(&full2[st2]) : s_bar;
+          const uint32_t f_par = kKeys ? static_cast<uint32_t>(t / C::kStages2) & 1u : s_par;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait3(s_bar, s_par, f_bar, f_par, s_bar, s_par, kSiteBwdS));
         }
         if (!ok) break;
+        tc_fence_after();
+        uint32_t s[C::kCols], d[C::kCols];
+        ld_cols(tlane + C::kColS + col0, s);
+        ok = attn::warp_wait(dp_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdDp);
+        tc_fence_after();
+        if (ok) ld_cols(tlane + C::kColDp + col0, d);
+        tmem_wait_ld();
+        written_here(s);
+        if (!ok) break;
+        written_here(d);
+        // The next step's S and dP may overwrite these.
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_warp(s_free);
+        uint32_t pk[C::kCols / 2], dk[C::kCols / 2];
+        const float* st_l = stat + st2 * 2 * C::kN + col0;
+        if (masked)
+          elementwise<kKeys, true>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, va, vb, vs, pk, dk);
+        else
+          elementwise<kKeys, false>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, va, vb, vs, pk,
+                                    dk);
+        // The products of the step before have read P and dS.
+        ok = attn::warp_wait(p_free, (static_cast<uint32_t>(t) & 1u) ^ 1u, kSiteBwdPFree);
+        if (!ok) break;
+        tc_fence_after();
+        if constexpr (kKeys) st_cols(tlane + C::kColP + (col0 >> 1), pk);
+        st_cols(tlane + C::kColDs + (col0 >> 1), dk);
         // Streamed rows that nothing sees may hold anything: zero them before
         // the accumulating products read them (0 * NaN is NaN).
         {
@@ -482,14 +547,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             hi = it.hi;
           }
           if (str0 + C::kN > hi || (str0 < lo && str0 + C::kN > se)) {
-            ok = attn::warp_wait(&full[st], static_cast<uint32_t>(t / C::kStages) & 1u,
+            ok = attn::warp_wait(&full1[st1], static_cast<uint32_t>(t / C::kStages1) & 1u,
                                  kSiteBwdFull);
             if (!ok) break;
-            for (int r = warp * 32 + lane; r < 2 * C::kBoxes * C::kN; r += 256) {
+            for (int r = static_cast<int>(threadIdx.x); r < (kKeys ? 2 : 1) * C::kBoxes * C::kN;
+                 r += 32 * C::kWarps) {
               const int sr = str0 + r % C::kN;
               if (sr >= hi || (sr < lo && sr >= se)) {
-                const uint32_t at = smem_u32(ring + st * 2 * C::kStrBytes) +
-                                    static_cast<uint32_t>(r) * 128u;
+                const int x = r / C::kN;  // boxes of the first tensor, then of the second
+                uint8_t* box = x < C::kBoxes
+                                   ? ring1 + st1 * C::kStrBytes + x * C::kStrBox
+                                   : ring2 + st2 * C::kStrBytes + (x - C::kBoxes) * C::kStrBox;
+                const uint32_t at = smem_u32(box) + static_cast<uint32_t>(r % C::kN) * 128u;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) st_shared_v4(at + e * 16, 0u, 0u, 0u, 0u);
               }
@@ -503,12 +572,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         mbar_arrive_warp(p_ready);
       }
       if (!ok) break;
-      // Epilogue: kKeys, half 0 writes dK and half 1 dV; queries, each half
-      // writes its half of dQ's columns.
-      const View& out = kKeys && half ? p.out2 : p.out1;
-      const float scale = kKeys && half ? 1.0f : p.scale;
-      constexpr int kCols = kKeys ? D : D / 2;
-      const int c0 = kKeys ? 0 : half * kCols;
+      // Epilogue: each warpgroup writes its columns of dQ, or of dK or dV.
+      const bool second = kKeys && wg >= C::kAccGroups;  // dV
+      const View& out = second ? p.out2 : p.out1;
+      const float scale = second ? 1.0f : p.scale;
+      const int c0 = wg % C::kAccGroups * C::kAccCols;
       const bool live = my < (kKeys ? p.Skv : p.Sq);
       uint16_t* dst = out.row(it.b, it.h, live ? my : 0) + c0;
       if (it.steps > 0) {
@@ -517,20 +585,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ++li;
         tc_fence_after();
       }
-      const uint32_t tacc = tlane + (kKeys && !half ? C::kColAcc1 : C::kColAcc2) + c0;
-#pragma unroll 1
-      for (int cc = 0; cc < kCols; cc += 32) {
-        uint32_t v[32];
+      const uint32_t tacc = tlane + (kKeys && !second ? C::kColAcc1 : C::kColAcc2) + c0;
+#pragma unroll
+      for (int cc = 0; cc < C::kAccCols; cc += 16) {
+        uint32_t v[16];
         if (it.steps > 0) {
-          tmem_ld32(tacc + cc, v);
-          tmem_wait_ld(v);
+          tmem_ld16(tacc + cc, v);
+          tmem_wait_ld();
+          written_here(v);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0u;
+          for (int e = 0; e < 16; ++e) v[e] = 0u;
         }
         if (live) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 2; ++e) {
             uint32_t w[4];
 #pragma unroll
             for (int f = 0; f < 4; ++f)
@@ -549,7 +618,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == C::kWarps) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
