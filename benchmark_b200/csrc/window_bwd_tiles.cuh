@@ -11,14 +11,10 @@
 // read along their rows).  Every output element has one owner that adds in a
 // fixed order: no atomics, equal bits from call to call.
 //
-// TMEM (all 512 columns at D = 128): kSBufs buffers of S, one of dP, the
-// accumulators.  P and dS overwrite their S.  A step is a chain of signals of
-// about 300 cycles each (product -> barrier -> TMEM load -> barrier -> next
-// product), longer than its products: with one buffer of S and dP the chain
-// took 2,050 cycles a step where the products need 1,280 (kKeys).  So S runs
-// steps ahead, and dP alone waits for its one buffer, which is free as soon as
-// it is in the registers.  kKeys steps are 64 queries wide: two accumulators
-// of D columns leave no room for 128.
+// TMEM: S, dP, then P and dS, then the accumulators.  S and dP have one buffer
+// each: the registers of the elementwise warps are the second, so the next
+// step's S and dP run while this step's P is computed.  kKeys steps are 64
+// queries wide: two accumulators of D columns leave no room for 128.
 //
 // Roles: elementwise and epilogue warps (warp w: lanes 32 (w % 4), the w / 4th
 // share of the columns), then a TMA warp, one that issues S and dP and one that
@@ -33,7 +29,6 @@ namespace b200 {
 namespace bwd {
 
 constexpr int kOwn = 128;  // owned rows
-constexpr int kBarQuad = 1;  // named barriers 1-4: the warps of a lane quadrant
 
 template <int D, bool kKeys>
 struct TileCfg {
@@ -60,17 +55,16 @@ struct TileCfg {
   static constexpr int kRing2Off = kRingOff + kStages1 * kStrBytes;
   static constexpr int kStatOff = kRing2Off + kStages2 * kStrBytes;
   static constexpr int kBarOff = kStatOff + kStages2 * kStatBytes;
-  // own_full own_empty p_free[3] sd_ready dp_free p_ready[2] acc_full acc_empty drain
-  static constexpr int kNumBars = 12 + 2 * (kStages1 + kStages2);
+  // own_full own_empty s_ready dp_ready s_free p_ready p_free acc_full acc_empty drain
+  static constexpr int kNumBars = 10 + 2 * (kStages1 + kStages2);
   static constexpr int kSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kSlotOff + 16 + 1024;  // + alignment slack
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
   static_assert(kSmemBytes > 116 * 1024, "one CTA per SM: each takes all of TMEM");
-  static constexpr int kSBufs = kKeys ? 3 : 2;
-  static constexpr uint32_t kColDp = kSBufs * kN;
-  static constexpr uint32_t kDs = kKeys ? kN / 2 : 0;  // dS in its S buffer (P at 0)
+  static constexpr uint32_t kColS = 0, kColDp = kN, kColP = 2 * kN;
+  static constexpr uint32_t kColDs = kColP + (kKeys ? kN / 2 : 0);
   static constexpr uint32_t kColAcc1 = 512 - 2 * D, kColAcc2 = 512 - D;
-  static_assert(kColDp + kN <= (kKeys ? kColAcc1 : kColAcc2), "TMEM columns");
+  static_assert(kColDs + kN / 2 <= (kKeys ? kColAcc1 : kColAcc2), "TMEM columns");
   static constexpr uint32_t kIdescS = idesc_bf16_f32(kOwn, kN, false, false);
   static constexpr uint32_t kIdescAcc = idesc_bf16_f32(kOwn, D, false, true);
 };
@@ -91,8 +85,8 @@ struct TileParams {
 };
 
 enum : uint32_t {
-  kSiteBwdOwn = 0x20, kSiteBwdFull, kSiteBwdEmpty, kSiteBwdS, kSiteBwdP,
-  kSiteBwdAcc
+  kSiteBwdOwn = 0x20, kSiteBwdFull, kSiteBwdEmpty, kSiteBwdS, kSiteBwdDp,
+  kSiteBwdP, kSiteBwdPFree, kSiteBwdAcc
 };
 
 // -lse and -delta of every query row, padded with zeros.  D/8 lanes to a row
@@ -202,7 +196,6 @@ __device__ __forceinline__ TileItem<kKeys> tile_item(const TileParams& p, int k)
     if (p.sinks >= it.lo || it.hi == 0) it.lo = 0;
     it.se = it.lo > 0 ? p.sinks : 0;
     const int w0 = it.lo / 128;
-    it.per_head = -1;
     it.n_sink = min((it.se + 127) / 128, w0);
     it.skip = w0 - it.n_sink;
     it.steps = it.n_sink + (it.hi + 127) / 128 - w0;
@@ -271,9 +264,9 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   uint8_t* ring2 = smem + C::kRing2Off;
   float* stat = reinterpret_cast<float*>(smem + C::kStatOff);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t *own_full = bars, *own_empty = bars + 1, *p_free = bars + 2, *sd_ready = bars + 5,
-           *dp_free = bars + 6, *p_ready = bars + 7, *acc_full = bars + 9,
-           *acc_empty = bars + 10, *drain = bars + 11, *full1 = bars + 12,
+  uint64_t *own_full = bars, *own_empty = bars + 1, *s_ready = bars + 2, *dp_ready = bars + 3,
+           *s_free = bars + 4, *p_ready = bars + 5, *p_free = bars + 6, *acc_full = bars + 7,
+           *acc_empty = bars + 8, *drain = bars + 9, *full1 = bars + 10,
            *empty1 = full1 + C::kStages1, *full2 = empty1 + C::kStages1,
            *empty2 = full2 + C::kStages2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kSlotOff);
@@ -282,12 +275,11 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(own_full, 1);
     mbar_init(own_empty, 1);
-    for (int i = 0; i < 3; ++i) mbar_init(&p_free[i], 1);
-    mbar_init(sd_ready, 1);
-    mbar_init(dp_free, C::kWarps);
-    // Two: a warp may be a step ahead of another, but not two (dP's buffer).
-    mbar_init(&p_ready[0], C::kWarps);
-    mbar_init(&p_ready[1], C::kWarps);
+    mbar_init(s_ready, 1);
+    mbar_init(dp_ready, 1);
+    mbar_init(s_free, C::kWarps);
+    mbar_init(p_ready, C::kWarps);
+    mbar_init(p_free, 1);
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, C::kWarps);
     mbar_init(drain, 2);
@@ -310,12 +302,18 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   const uint32_t tmem = *slot;
   pdl_wait();  // the row statistics
 
-  // First streamed row of a query head's step i.
+  // Streamed row 0 and the query head of step i.
   auto str_row = [&](const TileItem<kKeys>& it, int i) {
     if constexpr (kKeys)
-      return (it.t0 + i) * 64;
+      return (it.t0 + i % it.per_head) * 64;
     else
       return (i < it.n_sink ? i : i + it.skip) * 128;
+  };
+  auto query_head = [&](const TileItem<kKeys>& it, int i) {
+    if constexpr (kKeys)
+      return it.h * p.group + i / it.per_head;
+    else
+      return it.h;
   };
 
   if (warp == C::kWarps) {
@@ -338,10 +336,9 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
                       it.h * p.o2_h, it.b * p.o2_b, pol_own);
         }
         ++li;
-        int hi = 0, hq = kKeys ? it.h * p.group : it.h;  // step of a head; the head
         for (int i = 0; i < it.steps; ++i, ++t) {
           const int st1 = t % C::kStages1, st2 = t % C::kStages2;
-          const int row = str_row(it, hi);
+          const int row = str_row(it, i), hq = query_head(it, i);
           const int h = kKeys ? hq : it.h / p.group;
           ok = mbar_wait(&empty1[st1], (static_cast<uint32_t>(t / C::kStages1) & 1u) ^ 1u,
                          kSiteBwdEmpty, kDefaultWaitLimitNs, 20000u);
@@ -366,11 +363,6 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
             bulk_load(sdst + C::kN, src + p.stat_plane, C::kN * 4, &full2[st2]);
           }
           n2 = t + 1;
-          ++hi;
-          if (kKeys && hi == it.per_head) {
-            hi = 0;
-            ++hq;
-          }
         }
       }
       if (!ok) {
@@ -416,60 +408,45 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
         const int st1 = t % C::kStages1, st2 = t % C::kStages2;
         const uint32_t par1 = static_cast<uint32_t>(t / C::kStages1) & 1u;
         const uint32_t par2 = static_cast<uint32_t>(t / C::kStages2) & 1u;
-        const int sb = t % C::kSBufs;  // S buffer
-        const uint32_t t_s = tmem + static_cast<uint32_t>(sb * C::kN);
         if (!acc) {
-          // S(t), once the products of step t - kSBufs have read P and dS there.
-          {
-            const uint32_t f = smem_u32(&full1[st1]);
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait3(f, par1, smem_u32(&p_free[sb]),
-                                       (static_cast<uint32_t>(t / C::kSBufs) & 1u) ^ 1u, f, par1,
-                                       kSiteBwdFull));
-          }
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait3(smem_u32(&full1[st1]), par1, smem_u32(&full2[st2]), par2,
+                                     smem_u32(s_free), (static_cast<uint32_t>(t) & 1u) ^ 1u,
+                                     kSiteBwdFull));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss_warp(t_s, d_own1 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
+            mma_ss_warp(tmem + C::kColS, d_own1 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
                         d_n1 + st1 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
                         C::kIdescS, kk > 0 ? 1u : 0u);
-          // dP(t), once dP(t - 1) is in the registers.
-          {
-            const uint32_t f = smem_u32(&full2[st2]);
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait3(f, par2, smem_u32(dp_free),
-                                       (static_cast<uint32_t>(t) & 1u) ^ 1u, f, par2,
-                                       kSiteBwdFull));
-          }
-          if (!ok) break;
-          tc_fence_after();
+          mma_commit_warp(s_ready);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             mma_ss_warp(tmem + C::kColDp, d_own2 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
                         d_n2 + st2 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
                         C::kIdescS, kk > 0 ? 1u : 0u);
           if constexpr (!kKeys) mma_commit_warp(&empty2[st2]);
-          mma_commit_warp(sd_ready);
+          mma_commit_warp(dp_ready);
           if (i + 1 == steps) mma_commit_warp(own_empty);
         } else {
-          ok = warp_wait(&p_ready[t & 1], static_cast<uint32_t>(t >> 1) & 1u, kSiteBwdP);
+          ok = warp_wait(p_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdP);
           if (!ok) break;
           if constexpr (kKeys) {
 #pragma unroll
             for (int kk = 0; kk < C::kN / 16; ++kk)
-              mma_ts_warp(tmem + C::kColAcc2, t_s + kk * 8,
+              mma_ts_warp(tmem + C::kColAcc2, tmem + C::kColP + kk * 8,
                           d_k2 + st2 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
                           (i > 0 || kk > 0) ? 1u : 0u);
           }
 #pragma unroll
           for (int kk = 0; kk < C::kN / 16; ++kk)
-            mma_ts_warp(tmem + (kKeys ? C::kColAcc1 : C::kColAcc2), t_s + C::kDs + kk * 8,
+            mma_ts_warp(tmem + (kKeys ? C::kColAcc1 : C::kColAcc2), tmem + C::kColDs + kk * 8,
                         d_k1 + st1 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
                         (i > 0 || kk > 0) ? 1u : 0u);
           mma_commit_warp(&empty1[st1]);
           if constexpr (kKeys) mma_commit_warp(&empty2[st2]);
-          mma_commit_warp(&p_free[sb]);
+          mma_commit_warp(p_free);
           if (i + 1 == steps) mma_commit_warp(acc_full);
         }
       }
@@ -496,10 +473,9 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
         nlse = __ldg(src);
         ndelta = __ldg(src + p.stat_plane);
       }
-      for (int i = 0, hi = 0; i < it.steps; ++i, ++t) {
+      for (int i = 0; i < it.steps; ++i, ++t) {
         const int st1 = t % C::kStages1, st2 = t % C::kStages2;
-        const int str0 = str_row(it, hi);
-        if (++hi == it.per_head) hi = 0;  // (queries have no per_head: -1)
+        const int str0 = str_row(it, i);
         // The streamed columns [va, vb) that this row meets; for queries also
         // those below vs (sinks).  `masked`: some pair of the step is hidden.
         int va, vb, vs = 0;
@@ -520,36 +496,30 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
           masked = it.r0 + kOwn > p.Sq || str0 + 127 > first ||
                    (last - str0 >= p.window && str0 + 128 > p.sinks);
         }
-        // S and dP; kKeys: the columns' statistics, which came with dO.
+        // kKeys: the columns' statistics came with dO.  (Barriers are polled in
+        // one group: each poll that a branch depends on costs its latency.)
         {
-          const uint32_t s_bar = smem_u32(sd_ready), s_par = static_cast<uint32_t>(t) & 1u;
-          ok = __all_sync(
-              0xffffffffu,
-              mbar_wait3(s_bar, s_par, kKeys ? smem_u32(&full2[st2]) : s_bar,
-                         kKeys ? static_cast<uint32_t>(t / C::kStages2) & 1u : s_par, s_bar,
-                         s_par, kSiteBwdS));
+          const uint32_t s_bar = smem_u32(s_ready), s_par = static_cast<uint32_t>(t) & 1u;
+          const uint32_t f_bar = kKeys ? smem_u32(&full2[st2]) : s_bar;
+          const uint32_t f_par = kKeys ? static_cast<uint32_t>(t / C::kStages2) & 1u : s_par;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait3(s_bar, s_par, f_bar, f_par, s_bar, s_par, kSiteBwdS));
         }
-        if (!ok) {
-          // Another warp of the quadrant may have seen the barrier: it must not
-          // wait for this one.  (It gets no further: dP stays taken.)
-          named_bar_arrive(kBarQuad + quad, 32 * C::kGroups);
-          break;
-        }
+        if (!ok) break;
         tc_fence_after();
         uint32_t s[C::kCols], d[C::kCols];
-        const uint32_t t_s = tlane + static_cast<uint32_t>(t % C::kSBufs * C::kN);
-        ld_cols(t_s + col0, s);
-        ld_cols(tlane + C::kColDp + col0, d);
+        ld_cols(tlane + C::kColS + col0, s);
+        ok = attn::warp_wait(dp_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdDp);
+        tc_fence_after();
+        if (ok) ld_cols(tlane + C::kColDp + col0, d);
         tmem_wait_ld();
         written_here(s);
+        if (!ok) break;
         written_here(d);
-        // The next step's dP may overwrite this one's, and, once the warps of
-        // this quadrant have all loaded S, P and dS may overwrite that.
+        // The next step's S and dP may overwrite these.
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_warp(dp_free);
-        named_bar_sync(kBarQuad + quad, 32 * C::kGroups);
-        tc_fence_after();
+        mbar_arrive_warp(s_free);
         uint32_t pk[C::kCols / 2], dk[C::kCols / 2];
         const float* st_l = stat + st2 * 2 * C::kN + col0;
         if (masked)
@@ -557,8 +527,12 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
         else
           elementwise<kKeys, false>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, va, vb, vs, pk,
                                     dk);
-        if constexpr (kKeys) st_cols(t_s + (col0 >> 1), pk);
-        st_cols(t_s + C::kDs + (col0 >> 1), dk);
+        // The products of the step before have read P and dS.
+        ok = attn::warp_wait(p_free, (static_cast<uint32_t>(t) & 1u) ^ 1u, kSiteBwdPFree);
+        if (!ok) break;
+        tc_fence_after();
+        if constexpr (kKeys) st_cols(tlane + C::kColP + (col0 >> 1), pk);
+        st_cols(tlane + C::kColDs + (col0 >> 1), dk);
         // Streamed rows that nothing sees may hold anything: zero them before
         // the accumulating products read them (0 * NaN is NaN).
         {
@@ -595,7 +569,7 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_warp(&p_ready[t & 1]);
+        mbar_arrive_warp(p_ready);
       }
       if (!ok) break;
       // Epilogue: each warpgroup writes its columns of dQ, or of dK or dV.
