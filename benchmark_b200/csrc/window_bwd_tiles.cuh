@@ -11,10 +11,14 @@
 // read along their rows).  Every output element has one owner that adds in a
 // fixed order: no atomics, equal bits from call to call.
 //
-// TMEM: S, dP, then P and dS, then the accumulators.  S and dP have one buffer
-// each: the registers of the elementwise warps are the second, so the next
-// step's S and dP run while this step's P is computed.  kKeys steps are 64
-// queries wide: two accumulators of D columns leave no room for 128.
+// TMEM (all 512 columns at D = 128): kSBufs buffers of S, one of dP, the
+// accumulators.  P and dS overwrite their S.  A step is a chain of signals of
+// about 300 cycles each (product -> barrier -> TMEM load -> barrier -> next
+// product), longer than its products: with one buffer of S and dP the chain
+// took 2,050 cycles a step where the products need 1,280 (kKeys).  So S runs
+// steps ahead, and dP alone waits for its one buffer, which is free as soon as
+// it is in the registers.  kKeys steps are 64 queries wide: two accumulators
+// of D columns leave no room for 128.
 //
 // Roles: elementwise and epilogue warps (warp w: lanes 32 (w % 4), the w / 4th
 // share of the columns), then a TMA warp, one that issues S and dP and one that
@@ -29,6 +33,7 @@ namespace b200 {
 namespace bwd {
 
 constexpr int kOwn = 128;  // owned rows
+constexpr int kBarQuad = 1;  // named barriers 1-4: the warps of a lane quadrant
 
 template <int D, bool kKeys>
 struct TileCfg {
@@ -55,16 +60,17 @@ struct TileCfg {
   static constexpr int kRing2Off = kRingOff + kStages1 * kStrBytes;
   static constexpr int kStatOff = kRing2Off + kStages2 * kStrBytes;
   static constexpr int kBarOff = kStatOff + kStages2 * kStatBytes;
-  // own_full own_empty s_ready dp_ready s_free p_ready p_free acc_full acc_empty drain
-  static constexpr int kNumBars = 10 + 2 * (kStages1 + kStages2);
+  // own_full own_empty p_free[3] sd_ready dp_free p_ready[2] acc_full acc_empty drain
+  static constexpr int kNumBars = 12 + 2 * (kStages1 + kStages2);
   static constexpr int kSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kSlotOff + 16 + 1024;  // + alignment slack
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
   static_assert(kSmemBytes > 116 * 1024, "one CTA per SM: each takes all of TMEM");
-  static constexpr uint32_t kColS = 0, kColDp = kN, kColP = 2 * kN;
-  static constexpr uint32_t kColDs = kColP + (kKeys ? kN / 2 : 0);
+  static constexpr int kSBufs = kKeys ? 3 : 2;
+  static constexpr uint32_t kColDp = kSBufs * kN;
+  static constexpr uint32_t kDs = kKeys ? kN / 2 : 0;  // dS in its S buffer (P at 0)
   static constexpr uint32_t kColAcc1 = 512 - 2 * D, kColAcc2 = 512 - D;
-  static_assert(kColDs + kN / 2 <= (kKeys ? kColAcc1 : kColAcc2), "TMEM columns");
+  static_assert(kColDp + kN <= (kKeys ? kColAcc1 : kColAcc2), "TMEM columns");
   static constexpr uint32_t kIdescS = idesc_bf16_f32(kOwn, kN, false, false);
   static constexpr uint32_t kIdescAcc = idesc_bf16_f32(kOwn, D, false, true);
 };
@@ -85,8 +91,8 @@ struct TileParams {
 };
 
 enum : uint32_t {
-  kSiteBwdOwn = 0x20, kSiteBwdFull, kSiteBwdEmpty, kSiteBwdS, kSiteBwdDp,
-  kSiteBwdP, kSiteBwdPFree, kSiteBwdAcc
+  kSiteBwdOwn = 0x20, kSiteBwdFull, kSiteBwdEmpty, kSiteBwdS, kSiteBwdP,
+  kSiteBwdAcc
 };
 
 // -lse and -delta of every query row, padded with zeros.  D/8 lanes to a row
@@ -155,6 +161,30 @@ __device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t (&r)[8]) 
 __device__ __forceinline__ void written_here(uint32_t (&r)[32]) { reg_written_here(r); }
 __device__ __forceinline__ void written_here(uint32_t (&r)[16]) { reg_written_here16(r); }
 
+// Transposes 16-byte pieces among groups of kShare lanes: afterwards piece e of
+// lane q is what piece q of lane e was.
+template <int kShare>
+__device__ __forceinline__ void exchange(uint32_t (&x)[4 * kShare], int lane) {
+#pragma unroll
+  for (int m = 1; m < kShare; m <<= 1) {
+    const bool up = lane & m;
+#pragma unroll
+    for (int e = 0; e < kShare; ++e) {
+      if (e & m) continue;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t& a = x[4 * e + u];
+        uint32_t& b = x[4 * (e | m) + u];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? a : b, m);
+        if (up)
+          a = got;
+        else
+          b = got;
+      }
+    }
+  }
+}
+
 // One owned tile: where it lies and what it streams.
 template <bool kKeys>
 struct TileItem {
@@ -196,6 +226,7 @@ __device__ __forceinline__ TileItem<kKeys> tile_item(const TileParams& p, int k)
     if (p.sinks >= it.lo || it.hi == 0) it.lo = 0;
     it.se = it.lo > 0 ? p.sinks : 0;
     const int w0 = it.lo / 128;
+    it.per_head = -1;
     it.n_sink = min((it.se + 127) / 128, w0);
     it.skip = w0 - it.n_sink;
     it.steps = it.n_sink + (it.hi + 127) / 128 - w0;
@@ -264,9 +295,9 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   uint8_t* ring2 = smem + C::kRing2Off;
   float* stat = reinterpret_cast<float*>(smem + C::kStatOff);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t *own_full = bars, *own_empty = bars + 1, *s_ready = bars + 2, *dp_ready = bars + 3,
-           *s_free = bars + 4, *p_ready = bars + 5, *p_free = bars + 6, *acc_full = bars + 7,
-           *acc_empty = bars + 8, *drain = bars + 9, *full1 = bars + 10,
+  uint64_t *own_full = bars, *own_empty = bars + 1, *p_free = bars + 2, *sd_ready = bars + 5,
+           *dp_free = bars + 6, *p_ready = bars + 7, *acc_full = bars + 9,
+           *acc_empty = bars + 10, *drain = bars + 11, *full1 = bars + 12,
            *empty1 = full1 + C::kStages1, *full2 = empty1 + C::kStages1,
            *empty2 = full2 + C::kStages2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kSlotOff);
@@ -275,11 +306,12 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(own_full, 1);
     mbar_init(own_empty, 1);
-    mbar_init(s_ready, 1);
-    mbar_init(dp_ready, 1);
-    mbar_init(s_free, C::kWarps);
-    mbar_init(p_ready, C::kWarps);
-    mbar_init(p_free, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&p_free[i], 1);
+    mbar_init(sd_ready, 1);
+    mbar_init(dp_free, C::kWarps);
+    // Two: a warp may be a step ahead of another, but not two (dP's buffer).
+    mbar_init(&p_ready[0], C::kWarps);
+    mbar_init(&p_ready[1], C::kWarps);
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, C::kWarps);
     mbar_init(drain, 2);
@@ -302,18 +334,12 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   const uint32_t tmem = *slot;
   pdl_wait();  // the row statistics
 
-  // Streamed row 0 and the query head of step i.
+  // First streamed row of a query head's step i.
   auto str_row = [&](const TileItem<kKeys>& it, int i) {
     if constexpr (kKeys)
-      return (it.t0 + i % it.per_head) * 64;
+      return (it.t0 + i) * 64;
     else
       return (i < it.n_sink ? i : i + it.skip) * 128;
-  };
-  auto query_head = [&](const TileItem<kKeys>& it, int i) {
-    if constexpr (kKeys)
-      return it.h * p.group + i / it.per_head;
-    else
-      return it.h;
   };
 
   if (warp == C::kWarps) {
@@ -336,9 +362,10 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
                       it.h * p.o2_h, it.b * p.o2_b, pol_own);
         }
         ++li;
+        int hi = 0, hq = kKeys ? it.h * p.group : it.h;  // step of a head; the head
         for (int i = 0; i < it.steps; ++i, ++t) {
           const int st1 = t % C::kStages1, st2 = t % C::kStages2;
-          const int row = str_row(it, i), hq = query_head(it, i);
+          const int row = str_row(it, hi);
           const int h = kKeys ? hq : it.h / p.group;
           ok = mbar_wait(&empty1[st1], (static_cast<uint32_t>(t / C::kStages1) & 1u) ^ 1u,
                          kSiteBwdEmpty, kDefaultWaitLimitNs, 20000u);
@@ -363,6 +390,11 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
             bulk_load(sdst + C::kN, src + p.stat_plane, C::kN * 4, &full2[st2]);
           }
           n2 = t + 1;
+          ++hi;
+          if (kKeys && hi == it.per_head) {
+            hi = 0;
+            ++hq;
+          }
         }
       }
       if (!ok) {
@@ -408,45 +440,60 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
         const int st1 = t % C::kStages1, st2 = t % C::kStages2;
         const uint32_t par1 = static_cast<uint32_t>(t / C::kStages1) & 1u;
         const uint32_t par2 = static_cast<uint32_t>(t / C::kStages2) & 1u;
+        const int sb = t % C::kSBufs;  // S buffer
+        const uint32_t t_s = tmem + static_cast<uint32_t>(sb * C::kN);
         if (!acc) {
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait3(smem_u32(&full1[st1]), par1, smem_u32(&full2[st2]), par2,
-                                     smem_u32(s_free), (static_cast<uint32_t>(t) & 1u) ^ 1u,
-                                     kSiteBwdFull));
+          // S(t), once the products of step t - kSBufs have read P and dS there.
+          {
+            const uint32_t f = smem_u32(&full1[st1]);
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait3(f, par1, smem_u32(&p_free[sb]),
+                                       (static_cast<uint32_t>(t / C::kSBufs) & 1u) ^ 1u, f, par1,
+                                       kSiteBwdFull));
+          }
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss_warp(tmem + C::kColS, d_own1 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
+            mma_ss_warp(t_s, d_own1 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
                         d_n1 + st1 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
                         C::kIdescS, kk > 0 ? 1u : 0u);
-          mma_commit_warp(s_ready);
+          // dP(t), once dP(t - 1) is in the registers.
+          {
+            const uint32_t f = smem_u32(&full2[st2]);
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait3(f, par2, smem_u32(dp_free),
+                                       (static_cast<uint32_t>(t) & 1u) ^ 1u, f, par2,
+                                       kSiteBwdFull));
+          }
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             mma_ss_warp(tmem + C::kColDp, d_own2 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
                         d_n2 + st2 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
                         C::kIdescS, kk > 0 ? 1u : 0u);
           if constexpr (!kKeys) mma_commit_warp(&empty2[st2]);
-          mma_commit_warp(dp_ready);
+          mma_commit_warp(sd_ready);
           if (i + 1 == steps) mma_commit_warp(own_empty);
         } else {
-          ok = warp_wait(p_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdP);
+          ok = warp_wait(&p_ready[t & 1], static_cast<uint32_t>(t >> 1) & 1u, kSiteBwdP);
           if (!ok) break;
           if constexpr (kKeys) {
 #pragma unroll
             for (int kk = 0; kk < C::kN / 16; ++kk)
-              mma_ts_warp(tmem + C::kColAcc2, tmem + C::kColP + kk * 8,
+              mma_ts_warp(tmem + C::kColAcc2, t_s + kk * 8,
                           d_k2 + st2 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
                           (i > 0 || kk > 0) ? 1u : 0u);
           }
 #pragma unroll
           for (int kk = 0; kk < C::kN / 16; ++kk)
-            mma_ts_warp(tmem + (kKeys ? C::kColAcc1 : C::kColAcc2), tmem + C::kColDs + kk * 8,
+            mma_ts_warp(tmem + (kKeys ? C::kColAcc1 : C::kColAcc2), t_s + C::kDs + kk * 8,
                         d_k1 + st1 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
                         (i > 0 || kk > 0) ? 1u : 0u);
           mma_commit_warp(&empty1[st1]);
           if constexpr (kKeys) mma_commit_warp(&empty2[st2]);
-          mma_commit_warp(p_free);
+          mma_commit_warp(&p_free[sb]);
           if (i + 1 == steps) mma_commit_warp(acc_full);
         }
       }
@@ -462,134 +509,153 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
     const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = p.scale_log2;
     const uint64_t c2 = f2_pack(c, c);
-    int t = 0, li = 0;
+    const uint32_t sd_bar = smem_u32(sd_ready), full2_bar = smem_u32(full2);
+    // Epilogue: this warpgroup's columns of dQ, or of dK or dV (`second`).
+    const bool second = kKeys && wg >= C::kAccGroups;
+    const View& out = second ? p.out2 : p.out1;
+    const float out_scale = second ? 1.0f : p.scale;
+    const int c0 = wg % C::kAccGroups * C::kAccCols;
+    const uint32_t tacc = tlane + (kKeys && !second ? C::kColAcc1 : C::kColAcc2) + c0;
+    int t = 0, sb = 0, li = 0;  // steps, t % kSBufs, items with steps
     bool ok = true;
-    for (int k = static_cast<int>(blockIdx.x); k < p.n_items && ok; k += gridDim.x) {
-      const TileItem<kKeys> it = tile_item<kKeys>(p, k);
-      const int my = it.r0 + row;  // this thread's key or query
-      float nlse = 0.0f, ndelta = 0.0f;
-      if (!kKeys && my < p.Sq) {
-        const float* src = p.stats + (static_cast<int64_t>(it.b) * p.Hq + it.h) * p.sq_pad + my;
+    TileItem<kKeys> it{};
+    float nlse = 0.0f, ndelta = 0.0f;
+    auto open_item = [&](int k) {
+      it = tile_item<kKeys>(p, k);
+      if (!kKeys && it.r0 + row < p.Sq) {
+        const float* src =
+            p.stats + (static_cast<int64_t>(it.b) * p.Hq + it.h) * p.sq_pad + it.r0 + row;
         nlse = __ldg(src);
         ndelta = __ldg(src + p.stat_plane);
       }
-      for (int i = 0; i < it.steps; ++i, ++t) {
-        const int st1 = t % C::kStages1, st2 = t % C::kStages2;
-        const int str0 = str_row(it, i);
-        // The streamed columns [va, vb) that this row meets; for queries also
-        // those below vs (sinks).  `masked`: some pair of the step is hidden.
-        int va, vb, vs = 0;
-        bool masked;
-        if constexpr (kKeys) {
-          va = my - it.off - str0;
-          vb = min(p.Sq - str0, my < p.sinks ? 64 : my + p.window - it.off - str0);
-          const int first = it.off + str0, last = first + 63;  // positions of the step
-          masked = str0 + 64 > p.Sq || first < it.r0 + kOwn - 1 ||
-                   (last - it.r0 >= p.window && it.r0 + kOwn > p.sinks);
-        } else {
-          const int pos = it.off + my;
-          va = pos - p.window + 1 - str0;
-          vb = (my < p.Sq ? pos : -1) + 1 - str0;
-          vs = min(p.sinks, pos + 1) - str0;
-          if (my >= p.Sq) vs = va = vb = -1;
-          const int first = it.off + it.r0, last = first + kOwn - 1;
-          masked = it.r0 + kOwn > p.Sq || str0 + 127 > first ||
-                   (last - str0 >= p.window && str0 + 128 > p.sinks);
-        }
-        // kKeys: the columns' statistics came with dO.  (Barriers are polled in
-        // one group: each poll that a branch depends on costs its latency.)
+    };
+    if (static_cast<int>(blockIdx.x) < p.n_items) open_item(static_cast<int>(blockIdx.x));
+    for (int k = static_cast<int>(blockIdx.x); k < p.n_items && ok; k += gridDim.x) {
+      const int my = it.r0 + row;  // this thread's key or query
+      // Steps whose pairs are all visible: those with str0 in [clear0, clear1],
+      // or (queries) below clear1 and within the sinks.
+      int clear0, clear1;
+      // The streamed positions [va, vb) that this row meets; queries also
+      // those below vs (sinks).
+      int va, vb, vs = 0;
+      // Live streamed rows: [0, se) and [lo, hi).  The others may hold anything.
+      int se, lo, hi;
+      if constexpr (kKeys) {
+        const bool sinks_only = it.r0 + kOwn <= p.sinks;
+        clear0 = it.r0 + kOwn - 1 - it.off;
+        clear1 = min(p.Sq - 64, sinks_only ? p.Sq : p.window - 64 + it.r0 - it.off);
+        va = my - it.off;
+        vb = min(p.Sq, my < p.sinks ? p.Sq : my + p.window - it.off);
+        se = 0;
+        lo = max(0, -it.off);
+        hi = 0x7fffffff;
+      } else {
+        const int first = it.off + it.r0, pos = it.off + my;
+        clear0 = first + kOwn - p.window;
+        clear1 = it.r0 + kOwn <= p.Sq ? first - 127 : -1;
+        va = pos - p.window + 1;
+        vb = pos + 1;
+        vs = min(p.sinks, pos + 1);
+        if (my >= p.Sq) va = vb = vs = 0;
+        se = it.se;
+        lo = it.lo;
+        hi = it.hi;
+      }
+      int str0 = str_row(it, 0);
+      for (int i = 0, head_i = 0; i < it.steps; ++i, ++t) {
+        const bool masked =
+            str0 > clear1 || (str0 < clear0 && (kKeys || str0 + 128 > p.sinks));
+        // S and dP; kKeys: the columns' statistics, which came with dO.
         {
-          const uint32_t s_bar = smem_u32(s_ready), s_par = static_cast<uint32_t>(t) & 1u;
-          const uint32_t f_bar = kKeys ? smem_u32(&full2[st2]) : s_bar;
-          const uint32_t f_par = kKeys ? static_cast<uint32_t>(t / C::kStages2) & 1u : s_par;
+          const uint32_t par = static_cast<uint32_t>(t) & 1u;
+          const uint32_t f_bar = kKeys ? full2_bar + 8u * (t % C::kStages2) : sd_bar;
+          const uint32_t f_par = kKeys ? static_cast<uint32_t>(t / C::kStages2) & 1u : par;
           ok = __all_sync(0xffffffffu,
-                          mbar_wait3(s_bar, s_par, f_bar, f_par, s_bar, s_par, kSiteBwdS));
+                          mbar_wait3(sd_bar, par, f_bar, f_par, sd_bar, par, kSiteBwdS));
         }
-        if (!ok) break;
+        if (!ok) {
+          // Another warp of the quadrant may have seen the barrier: it must not
+          // wait for this one.  (It gets no further: dP stays taken.)
+          named_bar_arrive(kBarQuad + quad, 32 * C::kGroups);
+          break;
+        }
         tc_fence_after();
         uint32_t s[C::kCols], d[C::kCols];
-        ld_cols(tlane + C::kColS + col0, s);
-        ok = attn::warp_wait(dp_ready, static_cast<uint32_t>(t) & 1u, kSiteBwdDp);
-        tc_fence_after();
-        if (ok) ld_cols(tlane + C::kColDp + col0, d);
+        const uint32_t t_s = tlane + static_cast<uint32_t>(sb * C::kN);
+        if (++sb == C::kSBufs) sb = 0;
+        ld_cols(t_s + col0, s);
+        ld_cols(tlane + C::kColDp + col0, d);
         tmem_wait_ld();
         written_here(s);
-        if (!ok) break;
         written_here(d);
-        // The next step's S and dP may overwrite these.
+        // The next step's dP may overwrite this one's, and, once the warps of
+        // this quadrant have all loaded S, P and dS may overwrite that.
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_warp(s_free);
-        uint32_t pk[C::kCols / 2], dk[C::kCols / 2];
-        const float* st_l = stat + st2 * 2 * C::kN + col0;
-        if (masked)
-          elementwise<kKeys, true>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, va, vb, vs, pk, dk);
-        else
-          elementwise<kKeys, false>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, va, vb, vs, pk,
-                                    dk);
-        // The products of the step before have read P and dS.
-        ok = attn::warp_wait(p_free, (static_cast<uint32_t>(t) & 1u) ^ 1u, kSiteBwdPFree);
-        if (!ok) break;
+        mbar_arrive_warp(dp_free);
+        named_bar_sync(kBarQuad + quad, 32 * C::kGroups);
         tc_fence_after();
-        if constexpr (kKeys) st_cols(tlane + C::kColP + (col0 >> 1), pk);
-        st_cols(tlane + C::kColDs + (col0 >> 1), dk);
-        // Streamed rows that nothing sees may hold anything: zero them before
-        // the accumulating products read them (0 * NaN is NaN).
-        {
-          int se, lo, hi;  // live rows: [0, se) and [lo, hi)
-          if constexpr (kKeys) {
-            se = 0;
-            lo = max(0, -it.off);
-            hi = 0x7fffffff;
-          } else {
-            se = it.se;
-            lo = it.lo;
-            hi = it.hi;
-          }
-          if (str0 + C::kN > hi || (str0 < lo && str0 + C::kN > se)) {
-            ok = attn::warp_wait(&full1[st1], static_cast<uint32_t>(t / C::kStages1) & 1u,
-                                 kSiteBwdFull);
-            if (!ok) break;
-            for (int r = static_cast<int>(threadIdx.x); r < (kKeys ? 2 : 1) * C::kBoxes * C::kN;
-                 r += 32 * C::kWarps) {
-              const int sr = str0 + r % C::kN;
-              if (sr >= hi || (sr < lo && sr >= se)) {
-                const int x = r / C::kN;  // boxes of the first tensor, then of the second
-                uint8_t* box = x < C::kBoxes
-                                   ? ring1 + st1 * C::kStrBytes + x * C::kStrBox
-                                   : ring2 + st2 * C::kStrBytes + (x - C::kBoxes) * C::kStrBox;
-                const uint32_t at = smem_u32(box) + static_cast<uint32_t>(r % C::kN) * 128u;
+        uint32_t pk[C::kCols / 2], dk[C::kCols / 2];
+        const float* st_l = stat + t % C::kStages2 * 2 * C::kN + col0;
+        if (masked)
+          elementwise<kKeys, true>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, va - str0, vb - str0,
+                                   vs - str0, pk, dk);
+        else
+          elementwise<kKeys, false>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, 0, 0, 0, pk, dk);
+        if constexpr (kKeys) st_cols(t_s + (col0 >> 1), pk);
+        st_cols(t_s + C::kDs + (col0 >> 1), dk);
+        // Streamed rows that nothing sees: zeroed before the accumulating
+        // products read them (0 * NaN is NaN).
+        if (str0 + C::kN > hi || (str0 < lo && str0 + C::kN > se)) {
+          const int st1 = t % C::kStages1, st2 = t % C::kStages2;
+          ok = attn::warp_wait(&full1[st1], static_cast<uint32_t>(t / C::kStages1) & 1u,
+                               kSiteBwdFull);
+          if (!ok) break;
+          for (int r = static_cast<int>(threadIdx.x); r < (kKeys ? 2 : 1) * C::kBoxes * C::kN;
+               r += 32 * C::kWarps) {
+            const int sr = str0 + r % C::kN;
+            if (sr >= hi || (sr < lo && sr >= se)) {
+              const int x = r / C::kN;  // boxes of the first tensor, then of the second
+              uint8_t* box = x < C::kBoxes
+                                 ? ring1 + st1 * C::kStrBytes + x * C::kStrBox
+                                 : ring2 + st2 * C::kStrBytes + (x - C::kBoxes) * C::kStrBox;
+              const uint32_t at = smem_u32(box) + static_cast<uint32_t>(r % C::kN) * 128u;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) st_shared_v4(at + e * 16, 0u, 0u, 0u, 0u);
-              }
+              for (int e = 0; e < 8; ++e) st_shared_v4(at + e * 16, 0u, 0u, 0u, 0u);
             }
-            fence_proxy_async_smem();
           }
+          fence_proxy_async_smem();
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_warp(p_ready);
+        mbar_arrive_warp(&p_ready[t & 1]);
+        if constexpr (kKeys) {
+          str0 += 64;
+          if (++head_i == it.per_head) {
+            head_i = 0;
+            str0 = str_row(it, 0);
+          }
+        } else {
+          str0 = i + 1 == it.n_sink ? str_row(it, i + 1) : str0 + 128;
+        }
       }
       if (!ok) break;
-      // Epilogue: each warpgroup writes its columns of dQ, or of dK or dV.
-      const bool second = kKeys && wg >= C::kAccGroups;  // dV
-      const View& out = second ? p.out2 : p.out1;
-      const float scale = second ? 1.0f : p.scale;
-      const int c0 = wg % C::kAccGroups * C::kAccCols;
-      const bool live = my < (kKeys ? p.Skv : p.Sq);
-      uint16_t* dst = out.row(it.b, it.h, live ? my : 0) + c0;
-      if (it.steps > 0) {
+      const bool any = it.steps > 0;
+      const int b = it.b, h = it.h, r0 = it.r0;
+      // The next item's request length and statistics, under this one's end.
+      if (k + static_cast<int>(gridDim.x) < p.n_items) open_item(k + gridDim.x);
+      if (any) {
         ok = attn::warp_wait(acc_full, static_cast<uint32_t>(li) & 1u, kSiteBwdAcc);
         if (!ok) break;
         ++li;
         tc_fence_after();
       }
-      const uint32_t tacc = tlane + (kKeys && !second ? C::kColAcc1 : C::kColAcc2) + c0;
+      uint32_t w[C::kAccCols / 2];
 #pragma unroll
       for (int cc = 0; cc < C::kAccCols; cc += 16) {
         uint32_t v[16];
-        if (it.steps > 0) {
+        if (any) {
           tmem_ld16(tacc + cc, v);
           tmem_wait_ld();
           written_here(v);
@@ -597,22 +663,33 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = 0u;
         }
-        if (live) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t w[4];
-#pragma unroll
-            for (int f = 0; f < 4; ++f)
-              w[f] = pack_bf16x2(__uint_as_float(v[8 * e + 2 * f]) * scale,
-                                 __uint_as_float(v[8 * e + 2 * f + 1]) * scale);
-            *reinterpret_cast<uint4*>(dst + cc + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
+        for (int e = 0; e < 8; ++e)
+          w[cc / 2 + e] = pack_bf16x2(__uint_as_float(v[2 * e]) * out_scale,
+                                      __uint_as_float(v[2 * e + 1]) * out_scale);
       }
-      if (it.steps > 0) {
+      if (any) {
         tc_fence_before();
         __syncwarp();
         mbar_arrive_warp(acc_empty);
+      }
+      // A thread holds kAccCols columns of its row; kShare threads exchange
+      // 16-byte pieces so that together they store 64 bytes of a row at a time.
+      constexpr int kShare = C::kAccCols >= 32 ? 4 : 2;
+      const int rows = kKeys ? p.Skv : p.Sq;
+#pragma unroll
+      for (int cc = 0; cc < C::kAccCols / 2; cc += 4 * kShare) {
+        uint32_t(&x)[4 * kShare] = *reinterpret_cast<uint32_t(*)[4 * kShare]>(&w[cc]);
+        exchange<kShare>(x, lane);
+        // Now piece e of x is piece lane % kShare of row e of the kShare rows.
+#pragma unroll
+        for (int e = 0; e < kShare; ++e) {
+          const int r = r0 + quad * 32 + (lane & ~(kShare - 1)) + e;
+          if (r < rows)
+            *reinterpret_cast<uint4*>(out.row(b, h, r) + c0 + 2 * cc +
+                                      8 * (lane & (kShare - 1))) =
+                make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        }
       }
     }
   }
