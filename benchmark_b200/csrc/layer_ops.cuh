@@ -196,12 +196,24 @@ b200_status window_shape(const char* who, int B, int Hq, int Hkv, int Sq, int Sk
 }
 
 // Splits of the keys of a row tile: two CTAs per SM, at least two blocks for
-// each of a split's warps.
-int split_plan(int64_t units, int64_t keys) {
+// each of a split's warps.  Up to kMaxCluster of them merge as a cluster; more
+// go through a workspace and a second kernel, which pays from twice as many
+// on.  Measured (us, second kernel / cluster of 8): 32 splits, B 1, 8 kv heads,
+// 8192 keys: 12.7 / 17.6; 9 splits, B 4, 32768 keys: 87.8 / 81.7; 8 splits, B 4,
+// 8192 keys: 27.1 / 26.1.
+struct SplitPlan {
+  int nsplit;
+  bool cluster;
+};
+
+SplitPlan split_plan(int64_t units, int64_t keys, bool partial) {
+  namespace sp = b200::split;
   const int64_t want = 2 * static_cast<int64_t>(sm_count()) / std::max<int64_t>(units, 1);
-  const int64_t most = keys / (2 * b200::split::kWarps * b200::split::kKeys);
-  return static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>({want, most, b200::split::kMaxSplits})));
+  const int64_t most = keys / (2 * sp::kWarps * sp::kKeys);
+  const int n =
+      static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, sp::kMaxSplits})));
+  if (partial || n >= 2 * sp::kMaxCluster) return SplitPlan{n, false};
+  return SplitPlan{std::min(n, sp::kMaxCluster), true};
 }
 
 int row_tiles_of(int64_t rows) {
@@ -240,18 +252,20 @@ size_t part_bytes(int64_t rows, int D) {
 struct WindowPlan {
   bool tiles;   // 128-row tiles (tcgen05); else 16-row tiles that split the keys
   int nsplit;
-  size_t bytes;
+  size_t bytes;  // of the splits' partial sums; 0: a cluster merges them
 };
 
-WindowPlan window_plan(const WindowShape& s, bool partial = false) {
-  if (!partial && window_by_tiles(s)) return WindowPlan{true, 1, 0};
+size_t split_bytes(int64_t rows, const SplitPlan& p, int D) {
+  return p.cluster ? 0 : part_bytes(rows * p.nsplit, D);
+}
+
+WindowPlan window_plan(const WindowShape& s) {
+  if (window_by_tiles(s)) return WindowPlan{true, 1, 0};
   const int64_t rows = static_cast<int64_t>(s.Hq / s.Hkv) * s.Sq;
-  const int64_t units = static_cast<int64_t>(s.B) * s.Hkv * row_tiles_of(rows);
+  const int64_t heads = static_cast<int64_t>(s.B) * s.Hkv;
   const int64_t keys = std::min<int64_t>(s.Skv, static_cast<int64_t>(s.window) + s.sinks);
-  WindowPlan p{false, split_plan(units, keys), 0};
-  if (p.nsplit > 1 || partial)
-    p.bytes = part_bytes(static_cast<int64_t>(s.B) * s.Hkv * p.nsplit * rows, s.D);
-  return p;
+  const SplitPlan p = split_plan(heads * row_tiles_of(rows), keys, false);
+  return WindowPlan{false, p.nsplit, split_bytes(heads * rows, p, s.D)};
 }
 
 template <int D>
@@ -263,19 +277,29 @@ b200_status launch_split(const b200::split::Params& p, cudaStream_t stream) {
   if (st != B200_OK) return st;
   const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * p.row_tiles * p.nsplit;
   if (grid > 0x7fffffffll) return fail(B200_EUNSUPPORTED, "attention: too many work units");
-  kernel<<<static_cast<unsigned>(grid), b200::split::kThreads, C::kSmemBytes, stream>>>(p);
-  return check_launch("split attention launch");
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.nsplit);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(b200::split::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = !p.part_o && p.nsplit > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, "split attention launch");
 }
 
 b200_status launch_combine(const b200::split::CombineParams& p, int D, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.rows;
   const int64_t grid = (rows + 3) / 4;
   if (grid > 0x7fffffffll) return fail(B200_EUNSUPPORTED, "attention: too many rows");
-  if (D == 128)
-    b200::split::combine_kernel<128><<<static_cast<unsigned>(grid), 128, 0, stream>>>(p);
-  else
-    b200::split::combine_kernel<64><<<static_cast<unsigned>(grid), 128, 0, stream>>>(p);
-  return check_launch("combine launch");
+  return launch_dependent(
+      D == 128 ? b200::split::combine_kernel<128> : b200::split::combine_kernel<64>,
+      static_cast<unsigned>(grid), 128, stream, "combine launch", p);
 }
 
 b200::split::Params split_params(const WindowShape& s, const b200_tensor* q, const b200_tensor* k,
@@ -297,7 +321,6 @@ b200::split::Params split_params(const WindowShape& s, const b200_tensor* q, con
   p.nsplit = nsplit;
   p.window = s.window;
   p.sinks = s.sinks;
-  p.step = 1;
   p.scale_log2 = s.scale * 1.4426950408889634f;
   return p;
 }
@@ -543,54 +566,58 @@ b200_status launch_prefix_tiles(const WindowShape& own, int P, const b200_tensor
       qm, km, vm, qm, p, static_cast<long long>(own.Hkv) * t.count * nsplit, stream);
 }
 
-// The prefix as one batch whose rows are those of every request's queries.
+// A shared prefix: by 128-row tiles for the whole batch, beside the requests'
+// own keys by 16-row tiles, and combined; or all by 16-row tiles, each request
+// reading the prefix.
 struct PrefixPlan {
-  bool tiles;         // the prefix by 128-row tiles (tcgen05); else 16-row tiles
-  int prefix_splits;  // 0: no prefix
-  int own_splits;
+  bool tiles;
+  int prefix_splits;  // tiles: of the prefix
+  int own_splits;     // of the requests' keys (not tiles: after the prefix)
   size_t prefix_bytes, own_bytes;
 };
 
-// Whether the prefix goes by 128-row tiles: where the 16-row kernel's work
-// would take more than 4 us (the tiles' later start and larger partial sums).
-// Measured (us of a call, 16-row / 128-row): heads 32/8, 2048 keys, 16 requests:
-// 16.3 / 17.6, 32: 20.5 / 19.8; 8192 keys, 4: 18.4 / 19.2, 8: 20.7 / 19.6, 64:
-// 69.8 / 30.1; D 64, 8192 keys, 8: 17.5 / 18.2, 16: 19.8 / 19.0.  A tile holds
-// whole requests, and the queries' map cannot broadcast.
-bool prefix_by_tiles(const WindowShape& own, int P, const b200_tensor* q) {
-  const int64_t rows = static_cast<int64_t>(own.Hq / own.Hkv) * own.Sq;
-  if (rows > b200::attn::kBM) return false;
-  if (q && ((own.B > 1 && q->stride_b == 0) || (own.Hq > 1 && q->stride_h == 0))) return false;
-  return own.B * rows > b200::split::kRows &&
-         split_us(own.Hkv * static_cast<int64_t>(row_tiles_of(own.B * rows)), P, own.D) > 4.0;
-}
-
-// q's strides decide too; null: they do not.
+// The second form starts one kernel instead of three, and reads the prefix
+// (from L2) for each request: it is chosen up to 6 us more work.  Measured (us,
+// tiles / 16-row, 128 own keys): heads 32/8, P 512, B 2: 14.0 / 6.7, B 64: 23.3 /
+// 26.0; P 2048, B 8: 16.2 / 14.3, B 16: 17.3 / 21.1; P 32768, B 2: 35.0 / 34.6,
+// B 4: 35.6 / 62.5; D 64, P 8192, B 4: 17.8 / 15.8, B 8: 18.0 / 24.8.  A tile
+// holds whole requests, and the queries' map cannot broadcast; q's strides
+// decide that (null: they do not).
 PrefixPlan prefix_plan(const WindowShape& own, int P, const b200_tensor* q) {
+  const int64_t rows = static_cast<int64_t>(own.Hq / own.Hkv) * own.Sq;
+  const int64_t heads = static_cast<int64_t>(own.B) * own.Hkv;
+  const int64_t units = heads * row_tiles_of(rows);
   PrefixPlan p{};
-  if (P > 0) {
-    const int64_t rows = static_cast<int64_t>(own.B) * (own.Hq / own.Hkv) * own.Sq;
-    p.tiles = prefix_by_tiles(own, P, q);
-    if (p.tiles) {
-      // Least rounds x (tiles of K/V per unit + a unit's fixed cost of about 3).
-      const int64_t units = static_cast<int64_t>(own.Hkv) * prefix_tiles(own).count;
-      const int64_t kv = (P + b200::attn::kBN - 1) / b200::attn::kBN, sms = sm_count();
-      int64_t best = INT64_MAX;
-      for (int ns = 1; ns <= std::min<int64_t>(kv, b200::split::kMaxSplits); ++ns) {
-        const int64_t cost = (units * ns + sms - 1) / sms * ((kv + ns - 1) / ns + 3);
-        if (cost < best) {
-          best = cost;
-          p.prefix_splits = ns;
-        }
+  bool tiles = P > 0 && rows <= b200::attn::kBM &&
+               !(q && ((own.B > 1 && q->stride_b == 0) || (own.Hq > 1 && q->stride_h == 0)));
+  if (tiles) {
+    // Least rounds x (tiles of K/V per unit + a unit's fixed cost of about 3);
+    // a tile takes about 1 us.
+    const int64_t items = static_cast<int64_t>(own.Hkv) * prefix_tiles(own).count;
+    const int64_t kv = (P + b200::attn::kBN - 1) / b200::attn::kBN, sms = sm_count();
+    int64_t best = INT64_MAX;
+    for (int ns = 1; ns <= std::min<int64_t>(kv, b200::split::kMaxSplits); ++ns) {
+      const int64_t cost = (items * ns + sms - 1) / sms * ((kv + ns - 1) / ns + 3);
+      if (cost < best) {
+        best = cost;
+        p.prefix_splits = ns;
       }
-    } else {
-      p.prefix_splits = split_plan(static_cast<int64_t>(own.Hkv) * row_tiles_of(rows), P);
     }
-    p.prefix_bytes = part_bytes(own.Hkv * p.prefix_splits * rows, own.D);
+    tiles = split_us(units, static_cast<int64_t>(P) + own.Skv, own.D) >
+            static_cast<double>(best) + split_us(units, own.Skv, own.D) + 6.0;
   }
-  const WindowPlan w = window_plan(own, P > 0);
-  p.own_splits = w.nsplit;
-  p.own_bytes = w.bytes;
+  p.tiles = tiles;
+  if (tiles) {
+    const SplitPlan o = split_plan(units, own.Skv, true);
+    p.own_splits = o.nsplit;
+    p.own_bytes = split_bytes(heads * rows, o, own.D);
+    p.prefix_bytes = part_bytes(heads * rows * p.prefix_splits, own.D);
+  } else {
+    const SplitPlan o = split_plan(units, static_cast<int64_t>(P) + own.Skv, false);
+    p.own_splits = o.nsplit;
+    p.own_bytes = split_bytes(heads * rows, o, own.D);
+    p.prefix_bytes = 0;
+  }
   return p;
 }
 
@@ -720,9 +747,9 @@ b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, con
   b200::split::Params p = split_params(s, q, k, v, o, kv_len, plan.nsplit);
   p.lse = lse;
   const int64_t rows = static_cast<int64_t>(B) * Hkv * plan.nsplit * p.rows;
-  if (plan.nsplit > 1) part_pointers(workspace, rows, D, &p.part_o, &p.part_ml);
+  if (plan.bytes > 0) part_pointers(workspace, rows, D, &p.part_o, &p.part_ml);
   if ((st = D == 128 ? launch_split<128>(p, cs) : launch_split<64>(p, cs)) != B200_OK) return st;
-  if (plan.nsplit == 1) return B200_OK;
+  if (plan.bytes == 0) return B200_OK;
   b200::split::CombineParams c{};
   c.o = p.o;
   c.part_a = p.part_o;
@@ -829,7 +856,7 @@ b200_status attention_shared_prefix_workspace(int B, int Hq, int Hkv, int Sq, in
   if (st != B200_OK) return st;
   const b200_tensor shared{nullptr, 0, 0, 0};  // a q that is broadcast
   const PrefixPlan plan = prefix_plan(own, P, nullptr), other = prefix_plan(own, P, &shared);
-  *bytes = std::max(plan.prefix_bytes, other.prefix_bytes) + plan.own_bytes;
+  *bytes = std::max(plan.prefix_bytes + plan.own_bytes, other.prefix_bytes + other.own_bytes);
   return B200_OK;
 }
 
@@ -853,49 +880,36 @@ b200_status attention_shared_prefix(const b200_tensor* q, const b200_tensor* k_p
                             plan.prefix_bytes + plan.own_bytes)) != B200_OK)
     return st;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  auto launch = [&](const b200::split::Params& p) {
-    return D == 128 ? launch_split<128>(p, cs) : launch_split<64>(p, cs);
-  };
+  b200::split::Params p = split_params(own, q, k, v, o, kv_len, plan.own_splits);
   b200::split::CombineParams c{};
   c.B = B;
   c.Hkv = Hkv;
-  c.group = Hq / Hkv;
+  c.group = p.group;
   c.Sq = Sq;
-  c.rows = c.group * Sq;
-  c.o = view_of(o);
-  if (P > 0) {
+  c.rows = p.rows;
+  c.o = p.o;
+  if (plan.tiles) {
     float* part_o;
     float2* part_ml;
-    part_pointers(workspace, static_cast<int64_t>(Hkv) * plan.prefix_splits * B * c.rows, D,
+    part_pointers(workspace, static_cast<int64_t>(B) * Hkv * plan.prefix_splits * p.rows, D,
                   &part_o, &part_ml);
-    if (plan.tiles) {
-      st = D == 128 ? launch_prefix_tiles<128>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
-                                               part_o, part_ml, cs)
-                    : launch_prefix_tiles<64>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
-                                              part_o, part_ml, cs);
-    } else {
-      WindowShape shared = own;
-      shared.Skv = shared.window = P;
-      b200::split::Params p =
-          split_params(shared, q, k_prefix, v_prefix, o, nullptr, plan.prefix_splits);
-      p.B = 1;
-      p.step = 0;
-      p.rows = B * c.rows;
-      p.row_tiles = row_tiles_of(p.rows);
-      p.part_o = part_o;
-      p.part_ml = part_ml;
-      st = launch(p);
-    }
+    st = D == 128 ? launch_prefix_tiles<128>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
+                                             part_o, part_ml, cs)
+                  : launch_prefix_tiles<64>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
+                                            part_o, part_ml, cs);
     if (st != B200_OK) return st;
     c.part_b = part_o;
     c.ml_b = part_ml;
     c.nb = plan.prefix_splits;
+  } else if (P > 0) {
+    p.kp = view_of(k_prefix);
+    p.vp = view_of(v_prefix);
+    p.P = P;
   }
-  b200::split::Params p = split_params(own, q, k, v, o, kv_len, plan.own_splits);
   if (plan.own_bytes > 0)
     part_pointers(static_cast<unsigned char*>(workspace) + plan.prefix_bytes,
                   static_cast<int64_t>(B) * Hkv * p.nsplit * p.rows, D, &p.part_o, &p.part_ml);
-  if ((st = launch(p)) != B200_OK) return st;
+  if ((st = D == 128 ? launch_split<128>(p, cs) : launch_split<64>(p, cs)) != B200_OK) return st;
   if (plan.own_bytes == 0) return B200_OK;
   c.part_a = p.part_o;
   c.ml_a = p.part_ml;

@@ -3,19 +3,25 @@
 //   O_i = softmax_j(q_i k_j scale) v_j over the keys that row i sees: with
 //   p_i its position, j <= p_i and (p_i - j < window or j < sinks)
 //
+// after the P keys of a prefix that all requests share (P may be 0), which
+// every row sees.
+//
 // The rows of one (batch, kv head) -- its `group` query heads x Sq tokens --
 // are packed into tiles of 16, so that a K/V row is read once for all heads
 // that share it.  A unit (batch, kv head, row tile, split) takes a share of
-// the 16-key blocks of [0, sinks) and of the window; each of its four warps
-// walks its own blocks with its own ring of cp.async stages, running maximum,
-// sum and O in registers, and nothing synchronises the warps until they merge
-// at the end.  With one split the unit writes O; with more, the unnormalised
-// O (fp32) and (m, l) of the splits meet in combine_kernel.
+// the 16-key blocks of the prefix, of [0, sinks) and of the window; each of
+// its four warps walks its own blocks with its own ring of cp.async stages,
+// running maximum, sum and O in registers, and nothing synchronises the warps
+// until they merge at the end.  The splits of a row tile are a thread-block
+// cluster and merge through distributed shared memory; where more than
+// kMaxCluster are needed to fill the GPU, their unnormalised O (fp32) and
+// (m, l) go through global memory to combine_kernel instead.
 //
 // Bound by memory: 4 D flops per row and key against 4 D bytes per key, so
 // 16 rows need 16 flops per byte, about 100 TFLOP/s at the card's bandwidth.
 // mma.sync (m16n8k16) carries that with a tile that fits the rows; a tcgen05
-// tile is at least 64 rows high.
+// tile is at least 64 rows high.  64 tokens, 64/8 heads, windows of 4096:
+// 157 us, 6.8 TB/s.
 #pragma once
 
 #include "mma_sync.cuh"
@@ -29,6 +35,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16;    // query rows of a tile
 constexpr int kKeys = 16;    // keys of a block
+constexpr int kMaxCluster = 8;
 constexpr int kMaxSplits = 32;  // the combining warp holds one split's (m, l) per lane
 
 template <int D>
@@ -45,18 +52,16 @@ struct Cfg {
 
 struct Params {
   View q, k, v, o;
+  View kp, vp;            // the prefix, [1, Hkv, P, D]
+  int P;
   const int32_t* kv_len;  // [B], or null: Skv
   int B, Hkv, group, Sq, Skv;
   int rows;       // group * Sq
   int row_tiles;  // ceil(rows / 16)
   int nsplit;
   int window, sinks;  // at most Skv
-  // 1: token s is at position n - Sq + s.  0 (a prefix that all share): every
-  // row sees all n keys, and the rows go on through the batches (B is 1, rows
-  // counts those of all batches).
-  int step;
   float scale_log2;
-  float* part_o;    // [B * Hkv][nsplit][rows][D], or null (nsplit = 1): O is written
+  float* part_o;    // [B * Hkv][nsplit][rows][D], or null: the nsplit CTAs are a cluster
   float2* part_ml;  // [B * Hkv][nsplit][rows] (m in log2 units, l)
   float* lse;       // [B, Hq, Sq] natural log of each row's sum, or null
 };
@@ -78,6 +83,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     split_attention_kernel(const __grid_constant__ Params p) {
   using C = Cfg<D>;
   extern __shared__ __align__(128) uint8_t smem[];
+  pdl_launch_dependents();
   const int lane = static_cast<int>(lane_id());
   const int warp = static_cast<int>(warp_id());
   int unit = static_cast<int>(blockIdx.x);
@@ -90,26 +96,29 @@ __global__ void __launch_bounds__(kThreads, 2)
   // The tile's rows and the keys that some of them see.
   const int n = p.kv_len ? max(0, min(p.kv_len[b], p.Skv)) : p.Skv;
   const int r_last = min(rt * kRows + kRows - 1, p.rows - 1);
-  auto position = [&](int r) { return n - 1 - (p.Sq - 1 - r / p.group) * p.step; };
+  auto position = [&](int r) { return n - p.Sq + r / p.group; };
   const int p_first = position(rt * kRows), p_last = position(r_last);
   const int hi = max(p_last + 1, 0);
   int lo = max(p_first - p.window + 1, 0);
   if (p.sinks >= lo || hi == 0) lo = 0;   // one range
   const int se = lo > 0 ? p.sinks : 0;    // the sinks before the window's range
+  const int nb_p = (p.P + kKeys - 1) / kKeys;
   const int nb_s = (se + kKeys - 1) / kKeys;
-  const int nb = nb_s + (hi - lo + kKeys - 1) / kKeys;
+  const int nb = nb_p + nb_s + (hi - lo + kKeys - 1) / kKeys;
   const int b0 = static_cast<int>(static_cast<int64_t>(nb) * split / p.nsplit);
   const int b1 = static_cast<int>(static_cast<int64_t>(nb) * (split + 1) / p.nsplit);
 
   const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStageBytes;
-  const uint16_t* kbase = p.k.row(b, h, 0);
-  const uint16_t* vbase = p.v.row(b, h, 0);
+  // Keys [j0, j1) of block i, of the prefix or of the request.
   auto block_keys = [&](int i, int* j0, int* j1) {
-    if (i < nb_s) {
+    if (i < nb_p) {
       *j0 = i * kKeys;
+      *j1 = min(*j0 + kKeys, p.P);
+    } else if (i < nb_p + nb_s) {
+      *j0 = (i - nb_p) * kKeys;
       *j1 = min(*j0 + kKeys, se);
     } else {
-      *j0 = lo + (i - nb_s) * kKeys;
+      *j0 = lo + (i - nb_p - nb_s) * kKeys;
       *j1 = min(*j0 + kKeys, hi);
     }
   };
@@ -120,16 +129,20 @@ __global__ void __launch_bounds__(kThreads, 2)
       int j0, j1;
       block_keys(i, &j0, &j1);
       constexpr int kChunks = D / 8;  // per row
+      const bool shared = i < nb_p;
+      const int64_t k_ss = shared ? p.kp.ss : p.k.ss, v_ss = shared ? p.vp.ss : p.v.ss;
+      const uint16_t* kbase = shared ? p.kp.row(0, h, j0) : p.k.row(b, h, j0);
+      const uint16_t* vbase = shared ? p.vp.row(0, h, j0) : p.v.row(b, h, j0);
       const uint32_t dst = ring + stage * C::kStageBytes;
 #pragma unroll
       for (int u = 0; u < kKeys * kChunks / 32; ++u) {
         const int idx = u * 32 + lane;
         const int r = idx / kChunks, c = idx % kChunks;
         const bool live = j0 + r < j1;
-        const int64_t j = live ? j0 + r : j0;
+        const int64_t j = live ? r : 0;
         const uint32_t at = dst + swz<C::kRowBytes>(r, c);
-        cp_async16(at, kbase + j * p.k.ss + c * 8, live);
-        cp_async16(at + C::kTileBytes, vbase + j * p.v.ss + c * 8, live);
+        cp_async16(at, kbase + j * k_ss + c * 8, live);
+        cp_async16(at + C::kTileBytes, vbase + j * v_ss + c * 8, live);
       }
     }
     cp_async_commit();
@@ -146,8 +159,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = min(half ? rb : ra, p.rows - 1);
-    const int t = r / p.group;
-    const uint16_t* src = p.q.row(b + t / p.Sq, h * p.group + r % p.group, t % p.Sq) + ca;
+    const uint16_t* src = p.q.row(b, h * p.group + r % p.group, r / p.group) + ca;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       qa[kk][half] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
@@ -193,15 +205,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     int j0, j1;
     block_keys(i, &j0, &j1);
     // A block that every row sees whole needs no mask.
-    if (!(j1 == j0 + kKeys && j1 - 1 <= p_first &&
-          (p_last - j0 < p.window || j1 <= p.sinks))) {
+    const bool shared = i < nb_p;
+    if (!(j1 == j0 + kKeys &&
+          (shared || (j1 - 1 <= p_first && (p_last - j0 < p.window || j1 <= p.sinks))))) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = j0 + 8 * t + ca + (e & 1);
           const int pos = e < 2 ? pos_a : pos_b;
-          if (!(j < j1 && j <= pos && (pos - j < p.window || j < p.sinks))) s[t][e] = -INFINITY;
+          if (!(j < j1 && (shared || (j <= pos && (pos - j < p.window || j < p.sinks)))))
+            s[t][e] = -INFINITY;
         }
     }
     float x_a = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
@@ -275,7 +289,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   const int row = static_cast<int>(threadIdx.x) >> 3;  // eight threads to a row
   const int r = rt * kRows + row;
-  if (r >= p.rows) return;
   float mx = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml_sh[w * kRows + row].x);
@@ -287,43 +300,102 @@ __global__ void __launch_bounds__(kThreads, 2)
     l = fmaf(ml.y, wt[w], l);
   }
   const int t8 = static_cast<int>(threadIdx.x) & 7;
-  const int64_t part = (static_cast<int64_t>(bh) * p.nsplit + split) * p.rows + r;
-  if (p.part_o && t8 == 0) p.part_ml[part] = make_float2(mx, l);
-  if (!p.part_o && p.lse && t8 == 0)
-    p.lse[(static_cast<int64_t>(bh) * p.group + r % p.group) * p.Sq + r / p.group] =
-        row_lse(mx, l);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  float a[D / 64][8];
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) {
-    const int col = c * 64 + t8 * 8;
-    float a[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = 0.0f;
+    for (int e = 0; e < 8; ++e) a[c][e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float4* src =
-          reinterpret_cast<const float4*>(o_sh + (w * kRows + row) * C::kOStride + col);
+      const float4* src = reinterpret_cast<const float4*>(
+          o_sh + (w * kRows + row) * C::kOStride + c * 64 + t8 * 8);
       const float4 x = src[0], y = src[1];
-      a[0] = fmaf(x.x, wt[w], a[0]);
-      a[1] = fmaf(x.y, wt[w], a[1]);
-      a[2] = fmaf(x.z, wt[w], a[2]);
-      a[3] = fmaf(x.w, wt[w], a[3]);
-      a[4] = fmaf(y.x, wt[w], a[4]);
-      a[5] = fmaf(y.y, wt[w], a[5]);
-      a[6] = fmaf(y.z, wt[w], a[6]);
-      a[7] = fmaf(y.w, wt[w], a[7]);
-    }
-    if (p.part_o) {
-      float4* dst = reinterpret_cast<float4*>(p.part_o + part * D + col);
-      dst[0] = make_float4(a[0], a[1], a[2], a[3]);
-      dst[1] = make_float4(a[4], a[5], a[6], a[7]);
-    } else {
-      uint16_t* dst = p.o.row(b, h * p.group + r % p.group, r / p.group) + col;
-      *reinterpret_cast<uint4*>(dst) =
-          make_uint4(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv),
-                     pack_bf16x2(a[4] * inv, a[5] * inv), pack_bf16x2(a[6] * inv, a[7] * inv));
+      a[c][0] = fmaf(x.x, wt[w], a[c][0]);
+      a[c][1] = fmaf(x.y, wt[w], a[c][1]);
+      a[c][2] = fmaf(x.z, wt[w], a[c][2]);
+      a[c][3] = fmaf(x.w, wt[w], a[c][3]);
+      a[c][4] = fmaf(y.x, wt[w], a[c][4]);
+      a[c][5] = fmaf(y.y, wt[w], a[c][5]);
+      a[c][6] = fmaf(y.z, wt[w], a[c][6]);
+      a[c][7] = fmaf(y.w, wt[w], a[c][7]);
     }
   }
+  if (p.part_o) {
+    if (r >= p.rows) return;
+    const int64_t part = (static_cast<int64_t>(bh) * p.nsplit + split) * p.rows + r;
+    if (t8 == 0) p.part_ml[part] = make_float2(mx, l);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      float4* dst = reinterpret_cast<float4*>(p.part_o + part * D + c * 64 + t8 * 8);
+      dst[0] = make_float4(a[c][0], a[c][1], a[c][2], a[c][3]);
+      dst[1] = make_float4(a[c][4], a[c][5], a[c][6], a[c][7]);
+    }
+    return;
+  }
+  if (p.nsplit > 1) {
+    // The cluster's splits: each CTA leaves its rows in its shared memory and
+    // merges every nsplit-th row of all of them, in split order.
+    __syncthreads();  // the warps' parts have been read
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      float4* dst = reinterpret_cast<float4*>(o_sh + row * C::kOStride + c * 64 + t8 * 8);
+      dst[0] = make_float4(a[c][0], a[c][1], a[c][2], a[c][3]);
+      dst[1] = make_float4(a[c][4], a[c][5], a[c][6], a[c][7]);
+    }
+    if (t8 == 0) ml_sh[row] = make_float2(mx, l);
+    cluster_sync_all();
+    constexpr int kCols = D / 32;  // of a lane; a warp to a row
+    for (int i = split + warp * p.nsplit; i < kRows; i += kWarps * p.nsplit) {
+      const int r_all = rt * kRows + i;
+      if (r_all >= p.rows) break;
+      const uint32_t at = smem_u32(o_sh + i * C::kOStride + lane * kCols);
+      const float2 ml = lane < p.nsplit
+                            ? ld_cluster2(mapa_shared(smem_u32(ml_sh + i), lane))
+                            : make_float2(-INFINITY, 0.0f);
+      float m_all = ml.x;
+#pragma unroll
+      for (int m = kMaxCluster / 2; m > 0; m >>= 1)
+        m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, m));
+      m_all = __shfl_sync(0xffffffffu, m_all, 0);
+      const float w_own = part_weight(ml, m_all);
+      float l_all = 0.0f, acc[kCols];
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+      for (int s2 = 0; s2 < p.nsplit; ++s2) {
+        const float w = __shfl_sync(0xffffffffu, w_own, s2);
+        l_all = fmaf(__shfl_sync(0xffffffffu, ml.y, s2), w, l_all);
+        const uint32_t src = mapa_shared(at, static_cast<uint32_t>(s2));
+#pragma unroll
+        for (int e = 0; e < kCols; e += 2) {
+          const float2 x = ld_cluster2(src + 4 * e);
+          acc[e] = fmaf(x.x, w, acc[e]);
+          acc[e + 1] = fmaf(x.y, w, acc[e + 1]);
+        }
+      }
+      const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+      const int head = h * p.group + r_all % p.group, tok = r_all / p.group;
+      if (p.lse && lane == 0)
+        p.lse[(static_cast<int64_t>(b) * p.Hkv * p.group + head) * p.Sq + tok] =
+            row_lse(m_all, l_all);
+      uint16_t* dst = p.o.row(b, head, tok) + lane * kCols;
+#pragma unroll
+      for (int e = 0; e < kCols; e += 2)
+        reinterpret_cast<uint32_t*>(dst)[e / 2] = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+    }
+    cluster_sync_all();  // the other CTAs have read this one's rows
+    return;
+  }
+  if (r >= p.rows) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int head = h * p.group + r % p.group, tok = r / p.group;
+  if (p.lse && t8 == 0)
+    p.lse[(static_cast<int64_t>(b) * p.Hkv * p.group + head) * p.Sq + tok] = row_lse(mx, l);
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+    *reinterpret_cast<uint4*>(p.o.row(b, head, tok) + c * 64 + t8 * 8) = make_uint4(
+        pack_bf16x2(a[c][0] * inv, a[c][1] * inv), pack_bf16x2(a[c][2] * inv, a[c][3] * inv),
+        pack_bf16x2(a[c][4] * inv, a[c][5] * inv), pack_bf16x2(a[c][6] * inv, a[c][7] * inv));
 }
 
 // O = sum_s w_s O_s / sum_s w_s l_s over the splits' partial sums, added in
@@ -354,6 +426,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Co
   const int64_t a0 = bh * p.na * p.rows + r;  // + s * rows
   const int64_t rows_b = static_cast<int64_t>(p.B) * p.rows;
   const int64_t b0 = h * p.nb * rows_b + static_cast<int64_t>(b) * p.rows + r;  // + s * rows_b
+  pdl_wait();  // the partial sums
   const float2 none = make_float2(-INFINITY, 0.0f);
   const float2 ml_a = lane < p.na ? p.ml_a[a0 + static_cast<int64_t>(lane) * p.rows] : none;
   const float2 ml_b = lane < p.nb ? p.ml_b[b0 + lane * rows_b] : none;
