@@ -1033,28 +1033,55 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           float mx_a, mx_b;
           if (masked) {
-            // Scale first, then mask, so masked keys are exactly -inf for any scale.
-            const int va = lim_a - kbase - 2 * t0, vb = lim_b - kbase - 2 * t0;
-            const int wa = low_a - kbase - 2 * t0, wb = low_b - kbase - 2 * t0;
-            const int sk = p.sinks - kbase - 2 * t0;
-            mx_a = -INFINITY;
-            mx_b = -INFINITY;
+            if constexpr (kForm == kWindow) {
+              // Hidden scores become -inf (scale_log2 is positive), by the one
+              // bound that the tile needs where it is one: three comparisons for
+              // each score doubled a masked tile's time.
+              auto hide = [&](auto see_a, auto see_b) {
+                mx_a = -INFINITY;
+                mx_b = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < 16; ++g) {
+                for (int g = 0; g < 16; ++g) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int u = 8 * g + e;
-                bool see_a = u < va, see_b = u < vb;
-                if constexpr (kForm == kWindow) {
-                  see_a &= u >= wa || u < sk;
-                  see_b &= u >= wb || u < sk;
+                  for (int e = 0; e < 2; ++e) {
+                    if (!see_a(8 * g + e)) s[4 * g + e] = -INFINITY;
+                    if (!see_b(8 * g + e)) s[4 * g + 2 + e] = -INFINITY;
+                  }
+                  mx_a = fmax3(mx_a, s[4 * g], s[4 * g + 1]);
+                  mx_b = fmax3(mx_b, s[4 * g + 2], s[4 * g + 3]);
                 }
-                const float xa = see_a ? s[4 * g + e] * c : -INFINITY;
-                const float xb = see_b ? s[4 * g + 2 + e] * c : -INFINITY;
-                s[4 * g + e] = xa;
-                s[4 * g + 2 + e] = xb;
-                mx_a = fmaxf(mx_a, xa);
-                mx_b = fmaxf(mx_b, xb);
+                mx_a *= c;
+                mx_b *= c;
+              };
+              const int at = kbase + 2 * t0;
+              const int va = lim_a - at, vb = lim_b - at, wa = low_a - at, wb = low_b - at;
+              const int sk = p.sinks - at;
+              const bool sinks_only = kbase + kBN <= it.lo;
+              if (sinks_only || kbase >= it.top_lo) {
+                const int ua = sinks_only ? min(va, sk) : va, ub = sinks_only ? min(vb, sk) : vb;
+                hide([&](int u) { return u < ua; }, [&](int u) { return u < ub; });
+              } else if (kbase + kBN <= it.min_lim && kbase >= p.sinks) {
+                hide([&](int u) { return u >= wa; }, [&](int u) { return u >= wb; });
+              } else {
+                hide([&](int u) { return u < va && (u >= wa || u < sk); },
+                     [&](int u) { return u < vb && (u >= wb || u < sk); });
+              }
+            } else {
+              // Scale first, then mask, so masked keys are exactly -inf for any scale.
+              const int va = lim_a - kbase - 2 * t0, vb = lim_b - kbase - 2 * t0;
+              mx_a = -INFINITY;
+              mx_b = -INFINITY;
+#pragma unroll
+              for (int g = 0; g < 16; ++g) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float xa = 8 * g + e < va ? s[4 * g + e] * c : -INFINITY;
+                  const float xb = 8 * g + e < vb ? s[4 * g + 2 + e] * c : -INFINITY;
+                  s[4 * g + e] = xa;
+                  s[4 * g + 2 + e] = xb;
+                  mx_a = fmaxf(mx_a, xa);
+                  mx_b = fmaxf(mx_b, xb);
+                }
               }
             }
           } else {
@@ -1098,7 +1125,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           all_finite = __all_sync(0xffffffffu, m_a != -INFINITY && m_b != -INFINITY);
           const float nm_a = (m_a == -INFINITY) ? 0.0f : -m_a;
           const float nm_b = (m_b == -INFINITY) ? 0.0f : -m_b;
-          const float sc = masked ? 1.0f : c;  // masked scores are pre-scaled
+          // masked scores are pre-scaled (not kWindow's)
+          const float sc = masked && kForm != kWindow ? 1.0f : c;
           // P for keys 0-63 (repeats g = 0..7), then 64-127 (g = 8..15).
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
