@@ -68,7 +68,7 @@ _PROTOTYPES = {
     "attention_window_fwd_workspace": [_i, _i, _i, _i, _i, _i, _i, _i, _szp],
     "attention_window_fwd": [_t, _t, _t, _t, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
                              _sz, _vp],
-    "attention_window_bwd_workspace": [_i, _i, _i, _szp],
+    "attention_window_bwd_workspace": [_i, _i, _i, _i, _i, _i, _i, _i, _szp],
     "attention_window_bwd": [_t, _t, _t, _t, _t, _vp, _t, _t, _t, _vp, _i, _i, _i, _i, _i, _i, _i,
                              _i, _f, _vp, _sz, _vp],
     "attention_shared_prefix_workspace": [_i, _i, _i, _i, _i, _i, _i, _szp],

@@ -508,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- setup ----
   if constexpr (kForm == kPrefix) {
+    pdl_launch_dependents();  // the requests' own keys, on the SMs left over
     // Rows past a tile's box stay zero (their scores are computed, and dropped).
     for (int i = static_cast<int>(threadIdx.x); i < 2 * C::kTileBytes / 16; i += kThreads)
       reinterpret_cast<uint4*>(q_buf)[i] = make_uint4(0u, 0u, 0u, 0u);

@@ -22,7 +22,6 @@
 #include "norm_rope_kernel.cuh"
 #include "split_attention_kernel.cuh"
 #include "window_bwd_kernel.cuh"
-#include "window_bwd_tiles.cuh"
 
 #include <cublas_v2.h>
 #include <cuda_bf16.h>

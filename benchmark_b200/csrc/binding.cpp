@@ -278,7 +278,7 @@ PyObject* attention_window_bwd_(const Args& a) {
   const auto* len = static_cast<const int32_t*>(c.flat(kv_len, at::kInt, {s.B}, "kv_len"));
   const float scale = static_cast<float>(a.real(9));
   size_t n = 0;
-  check(attention_window_bwd_workspace(s.B, s.H, s.S, &n));
+  check(attention_window_bwd_workspace(s.B, s.H, t.H, s.S, t.S, s.D, window, sinks, &n));
   const at::Tensor ws = c.workspace(n);
   check(unlocked([&] {
     return attention_window_bwd(&gv, &qv, &kv, &vv, &ov, lse_p, &dqv, &dkv, &dvv, len, s.B, s.H,

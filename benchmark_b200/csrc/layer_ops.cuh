@@ -278,17 +278,22 @@ b200_status launch_split(const b200::split::Params& p, cudaStream_t stream) {
   const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * p.row_tiles * p.nsplit;
   if (grid > 0x7fffffffll) return fail(B200_EUNSUPPORTED, "attention: too many work units");
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.nsplit);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  if (p.overlaps) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+  } else {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.nsplit);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
   cfg.blockDim = dim3(b200::split::kThreads, 1, 1);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = !p.part_o && p.nsplit > 1 ? 1 : 0;
+  cfg.numAttrs = p.overlaps || (!p.part_o && p.nsplit > 1) ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   return e == cudaSuccess ? B200_OK : cuda_fail(e, "split attention launch");
 }
@@ -362,7 +367,7 @@ b200_status encode_view(CUtensorMap* map, const b200_tensor* t, int B, int H, in
 
 template <int D, int kForm>
 b200_status launch_tiles(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
-                         const CUtensorMap& om, b200::attn::Params p, long long items,
+                         const CUtensorMap& om, b200::attn::Params p, long long items, int sms,
                          cudaStream_t stream) {
   using C = b200::attn::Cfg<D>;
   static unsigned attr_done = 0;
@@ -381,7 +386,7 @@ b200_status launch_tiles(const CUtensorMap& qm, const CUtensorMap& km, const CUt
                 launch_regs, b200::attn::kLaunchRegs);
   if (items > 0x3fffffffll) return fail(B200_EUNSUPPORTED, "attention: too many work items");
   p.n_items = static_cast<int>(items);
-  const int grid = static_cast<int>(std::min<long long>(items, sm_count()));
+  const int grid = static_cast<int>(std::min<long long>(items, sms));
   kernel<<<grid, b200::attn::kThreads, C::kSmemBytes, stream>>>(qm, km, vm, om, p);
   return check_launch("attention tiles launch");
 }
@@ -428,7 +433,8 @@ b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, cons
   const double keys = std::min<double>(s.Skv, static_cast<double>(s.window) + b200::attn::kBM);
   const long long g = static_cast<long long>(64.0 * (1 << 20) / (4.0 * keys * D)) * p.group;
   p.cgroup = static_cast<int>(std::max<long long>(1, std::min<long long>(g, planes)));
-  return launch_tiles<D, b200::attn::kWindow>(qm, km, vm, om, p, planes * p.n_qtiles, stream);
+  return launch_tiles<D, b200::attn::kWindow>(qm, km, vm, om, p, planes * p.n_qtiles, sm_count(),
+                                              stream);
 }
 
 // ---- window attention's gradients ----
@@ -440,8 +446,34 @@ struct WindowGrads {
 
 int64_t padded_queries(int Sq) { return (static_cast<int64_t>(Sq) + 63) / 64 * 64; }
 
-size_t window_bwd_bytes(int B, int Hq, int Sq) {
-  return static_cast<size_t>(B) * Hq * padded_queries(Sq) * 2 * sizeof(float);
+// How the key tiles that hold sinks are divided: where one of them has more
+// steps than half of an SM's share of the launch, into parts of that size or a
+// window's, up to 8 (their fp32 sums cost 2 x 128 x D floats each).  4096
+// queries, heads 32/8 of 128, window 100, 4 sinks: 353 us undivided, 154 us.
+struct SinkPlan {
+  int tiles, parts;  // parts 0: not divided
+};
+
+SinkPlan sink_plan(const WindowShape& s) {
+  const int64_t group = s.Hq / s.Hkv, heads = static_cast<int64_t>(s.B) * s.Hkv;
+  const int64_t tiles = (std::min(s.sinks, s.Skv) + 127) / 128, all = (s.Skv + 127) / 128;
+  if (tiles == 0) return SinkPlan{0, 0};
+  const int64_t most = group * ((s.Sq + 63) / 64);
+  const int64_t window = std::min(most, group * ((static_cast<int64_t>(s.window) + 127 + 63) / 64));
+  const int64_t share = heads * (tiles * most + (all - tiles) * window) / sm_count();
+  const int64_t size = std::max(window, share / 2);
+  const int64_t parts = std::min<int64_t>(8, (most + size - 1) / std::max<int64_t>(size, 1));
+  return parts > 1 ? SinkPlan{static_cast<int>(tiles), static_cast<int>(parts)} : SinkPlan{0, 0};
+}
+
+size_t window_stat_bytes(const WindowShape& s) {
+  return static_cast<size_t>(s.B) * s.Hq * padded_queries(s.Sq) * 2 * sizeof(float);
+}
+
+size_t window_bwd_bytes(const WindowShape& s) {
+  const SinkPlan k = sink_plan(s);
+  return window_stat_bytes(s) + static_cast<size_t>(s.B) * s.Hkv * k.tiles * k.parts * 2 *
+                                    b200::bwd::kOwn * s.D * sizeof(float);
 }
 
 template <int D, bool kKeys>
@@ -453,7 +485,9 @@ b200_status launch_bwd_tiles(const CUtensorMap (&m)[4], b200::bwd::TileParams p,
   const b200_status st = ensure_smem_attr(kernel, C::kSmemBytes, &attr_done);
   if (st != B200_OK) return st;
   p.tiles = (rows + b200::bwd::kOwn - 1) / b200::bwd::kOwn;
-  const int64_t items = static_cast<int64_t>(p.B) * heads * p.tiles;
+  int64_t items = static_cast<int64_t>(p.B) * heads * p.tiles;
+  if (kKeys && p.sink_parts > 0)
+    items += static_cast<int64_t>(p.B) * heads * p.sink_tiles * (p.sink_parts - 1);
   if (items > 0x3fffffffll) return fail(B200_EUNSUPPORTED, "attention_window_bwd: too many tiles");
   p.n_items = static_cast<int>(items);
   // Key tiles differ in length (sinks): a CTA each, so that the next one starts
@@ -512,12 +546,22 @@ b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* w
   b200::bwd::stats_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
       view_of(t.dout), view_of(t.o), t.lse, stats, p.stat_plane, p.sq_pad, s.B, s.Hq, s.Sq);
   if ((st = check_launch("attention_window_bwd statistics")) != B200_OK) return st;
+  const SinkPlan sink = sink_plan(s);
+  p.sink_tiles = sink.tiles;
+  p.sink_parts = sink.parts;
+  p.sink_sums = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
+                                         window_stat_bytes(s));
   p.out1 = view_of(t.dk);
   p.out2 = view_of(t.dv);
   p.o1_b = k_b, p.o1_h = k_h, p.o2_b = v_b, p.o2_h = v_h;
   p.s1_b = q_b, p.s1_h = q_h, p.s2_b = do_b, p.s2_h = do_h;
   if ((st = launch_bwd_tiles<D, true>({k, v, q[1], dout[1]}, p, s.Hkv, s.Skv, stream)) != B200_OK)
     return st;
+  if (sink.parts > 0) {
+    const int64_t sums = static_cast<int64_t>(s.B) * s.Hkv * sink.tiles * 2 * b200::bwd::kOwn * D / 4;
+    b200::bwd::sink_sum_kernel<D><<<static_cast<unsigned>((sums + 255) / 256), 256, 0, stream>>>(p);
+    if ((st = check_launch("attention_window_bwd sinks")) != B200_OK) return st;
+  }
   p.out1 = p.out2 = view_of(t.dq);
   p.o1_b = q_b, p.o1_h = q_h, p.o2_b = do_b, p.o2_h = do_h;
   p.s1_b = k_b, p.s1_h = k_h, p.s2_b = v_b, p.s2_h = v_h;
@@ -537,7 +581,7 @@ PrefixTiles prefix_tiles(const WindowShape& own) {
 
 template <int D>
 b200_status launch_prefix_tiles(const WindowShape& own, int P, const b200_tensor* q,
-                                const b200_tensor* k, const b200_tensor* v, int nsplit,
+                                const b200_tensor* k, const b200_tensor* v, int nsplit, int sms,
                                 float* part_o, float2* part_ml, cudaStream_t stream) {
   WindowShape shared = own;
   shared.Skv = P;
@@ -566,7 +610,7 @@ b200_status launch_prefix_tiles(const WindowShape& own, int P, const b200_tensor
       (st = encode_view(&vm, v, 1, own.Hkv, P, D, kKeys, &p.v_mb, &p.v_mh)) != B200_OK)
     return st;
   return launch_tiles<D, b200::attn::kPrefix>(
-      qm, km, vm, qm, p, static_cast<long long>(own.Hkv) * t.count * nsplit, stream);
+      qm, km, vm, qm, p, static_cast<long long>(own.Hkv) * t.count * nsplit, sms, stream);
 }
 
 // A shared prefix: by 128-row tiles for the whole batch, beside the requests'
@@ -575,6 +619,7 @@ b200_status launch_prefix_tiles(const WindowShape& own, int P, const b200_tensor
 struct PrefixPlan {
   bool tiles;
   int prefix_splits;  // tiles: of the prefix
+  int prefix_sms;     // tiles: SMs that they take
   int own_splits;     // of the requests' keys (not tiles: after the prefix)
   size_t prefix_bytes, own_bytes;
 };
@@ -597,7 +642,16 @@ PrefixPlan prefix_plan(const WindowShape& own, int P, const b200_tensor* q) {
     // Least rounds x (tiles of K/V per unit + a unit's fixed cost of about 3);
     // a tile takes about 1 us.
     const int64_t items = static_cast<int64_t>(own.Hkv) * prefix_tiles(own).count;
-    const int64_t kv = (P + b200::attn::kBN - 1) / b200::attn::kBN, sms = sm_count();
+    const int64_t kv = (P + b200::attn::kBN - 1) / b200::attn::kBN;
+    // Where the requests' own keys are long (4 us at the memory's rate), they
+    // stream through three tenths of the SMs beside the tiles.  Measured (us;
+    // 0 / 20 / 44 / 74 SMs left): 64 requests, heads 64/8, P 16384, up to 1024
+    // keys: 67.9 / 68.1 / 66.3 / 66.5; P 4096: 52.7 / 52.6 / 49.7 / 45.9; 32
+    // requests, P 16384, up to 512: 40.3 / 39.8 / 34.9 / 40.5.
+    const double own_us = 4.0 * own.B * own.Hkv * static_cast<double>(own.Skv) * own.D / 6.4e6;
+    int64_t sms = sm_count();
+    if (own_us > 4.0) sms = std::max<int64_t>(1, sms * 7 / 10);
+    p.prefix_sms = static_cast<int>(sms);
     int64_t best = INT64_MAX;
     for (int ns = 1; ns <= std::min<int64_t>(kv, b200::split::kMaxSplits); ++ns) {
       const int64_t cost = (items * ns + sms - 1) / sms * ((kv + ns - 1) / ns + 3);
@@ -767,10 +821,14 @@ b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, con
   return launch_combine(c, D, cs);
 }
 
-b200_status attention_window_bwd_workspace(int B, int Hq, int Sq, size_t* bytes) {
-  if (!bytes || B < 1 || Hq < 1 || Sq < 1)
-    return fail(B200_EINVAL, "attention_window_bwd_workspace: bad argument");
-  *bytes = window_bwd_bytes(B, Hq, Sq);
+b200_status attention_window_bwd_workspace(int B, int Hq, int Hkv, int Sq, int Skv, int D,
+                                           int window, int sinks, size_t* bytes) {
+  const char* who = "attention_window_bwd_workspace";
+  if (!bytes) return fail(B200_EINVAL, "%s: null result", who);
+  WindowShape s;
+  const b200_status st = window_shape(who, B, Hq, Hkv, Sq, Skv, D, window, sinks, -1.0f, &s);
+  if (st != B200_OK) return st;
+  *bytes = window_bwd_bytes(s);
   return B200_OK;
 }
 
@@ -794,60 +852,12 @@ b200_status attention_window_bwd(const b200_tensor* dout, const b200_tensor* q,
   if ((st = check_tensor(who, "dk", dk, B, Hkv, Skv, D, true)) != B200_OK) return st;
   if ((st = check_tensor(who, "dv", dv, B, Hkv, Skv, D, true)) != B200_OK) return st;
   if (!lse) return fail(B200_EINVAL, "%s: null lse", who);
-  if ((st = check_workspace(who, workspace, workspace_bytes, window_bwd_bytes(B, Hq, Sq))) !=
-      B200_OK)
+  if ((st = check_workspace(who, workspace, workspace_bytes, window_bwd_bytes(s))) != B200_OK)
     return st;
-  if (!(std::getenv("B200_TILES") && std::getenv("B200_TILES")[0] == '0')) {
-    const WindowGrads t{dout, q, k, v, o, dq, dk, dv, lse, kv_len};
-    const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-    return D == 128 ? window_bwd_tiles<128>(s, t, workspace, cs)
-                    : window_bwd_tiles<64>(s, t, workspace, cs);
-  }
-  namespace bw = b200::bwd;
-  bw::Params p{};
-  p.dout = view_of(dout);
-  p.q = view_of(q);
-  p.k = view_of(k);
-  p.v = view_of(v);
-  p.o = view_of(o);
-  p.dq = view_of(dq);
-  p.dk = view_of(dk);
-  p.dv = view_of(dv);
-  p.lse = lse;
-  p.delta = static_cast<float*>(workspace);
-  p.kv_len = kv_len;
-  p.B = B;
-  p.Hq = Hq;
-  p.Hkv = Hkv;
-  p.group = Hq / Hkv;
-  p.Sq = Sq;
-  p.Skv = Skv;
-  p.q_tiles = (Sq + bw::kTile - 1) / bw::kTile;
-  p.k_tiles = (Skv + bw::kTile - 1) / bw::kTile;
-  p.window = s.window;
-  p.sinks = s.sinks;
-  p.scale = s.scale;
-  p.scale_log2 = s.scale * 1.4426950408889634f;
-  const int64_t g0 = (static_cast<int64_t>(B) * Hq * Sq + 7) / 8;
-  const int64_t g1 = static_cast<int64_t>(B) * Hkv * p.k_tiles;
-  const int64_t g2 = static_cast<int64_t>(B) * Hq * p.q_tiles;
-  if (std::max({g0, g1, g2}) > 0x7fffffffll)
-    return fail(B200_EUNSUPPORTED, "%s: too many work units", who);
+  const WindowGrads t{dout, q, k, v, o, dq, dk, dv, lse, kv_len};
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  auto launch = [&](auto d) -> b200_status {
-    constexpr int kD = decltype(d)::value;
-    static unsigned attr_kv = 0, attr_q = 0;
-    constexpr int bytes = bw::Cfg<kD>::kSmemBytes;
-    b200_status r = ensure_smem_attr(bw::dkdv_kernel<kD>, bytes, &attr_kv);
-    if (r != B200_OK) return r;
-    if ((r = ensure_smem_attr(bw::dq_kernel<kD>, bytes, &attr_q)) != B200_OK) return r;
-    bw::delta_kernel<kD><<<static_cast<unsigned>(g0), 256, 0, cs>>>(p);
-    bw::dkdv_kernel<kD><<<static_cast<unsigned>(g1), bw::kThreads, bytes, cs>>>(p);
-    bw::dq_kernel<kD><<<static_cast<unsigned>(g2), bw::kThreads, bytes, cs>>>(p);
-    return check_launch("attention_window_bwd launch");
-  };
-  return D == 128 ? launch(std::integral_constant<int, 128>{})
-                  : launch(std::integral_constant<int, 64>{});
+  return D == 128 ? window_bwd_tiles<128>(s, t, workspace, cs)
+                  : window_bwd_tiles<64>(s, t, workspace, cs);
 }
 
 b200_status attention_shared_prefix_workspace(int B, int Hq, int Hkv, int Sq, int P, int S, int D,
@@ -897,13 +907,14 @@ b200_status attention_shared_prefix(const b200_tensor* q, const b200_tensor* k_p
     part_pointers(workspace, static_cast<int64_t>(B) * Hkv * plan.prefix_splits * p.rows, D,
                   &part_o, &part_ml);
     st = D == 128 ? launch_prefix_tiles<128>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
-                                             part_o, part_ml, cs)
+                                             plan.prefix_sms, part_o, part_ml, cs)
                   : launch_prefix_tiles<64>(own, P, q, k_prefix, v_prefix, plan.prefix_splits,
-                                            part_o, part_ml, cs);
+                                            plan.prefix_sms, part_o, part_ml, cs);
     if (st != B200_OK) return st;
     c.part_b = part_o;
     c.ml_b = part_ml;
     c.nb = plan.prefix_splits;
+    p.overlaps = 1;
   } else if (P > 0) {
     p.kp = view_of(k_prefix);
     p.vp = view_of(v_prefix);

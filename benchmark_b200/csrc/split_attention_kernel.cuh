@@ -64,6 +64,9 @@ struct Params {
   float* part_o;    // [B * Hkv][nsplit][rows][D], or null: the nsplit CTAs are a cluster
   float2* part_ml;  // [B * Hkv][nsplit][rows] (m in log2 units, l)
   float* lse;       // [B, Hq, Sq] natural log of each row's sum, or null
+  // The launch overlaps the kernel before it (the prefix's tiles): the last CTA
+  // ends after that one, so that whatever follows this grid follows both.
+  int overlaps;
 };
 
 // The natural log of the row sum l 2^m; a row without keys has none (-inf).
@@ -321,6 +324,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   }
   if (p.part_o) {
+    if (p.overlaps && blockIdx.x + 1 == gridDim.x) pdl_wait();
     if (r >= p.rows) return;
     const int64_t part = (static_cast<int64_t>(bh) * p.nsplit + split) * p.rows + r;
     if (t8 == 0) p.part_ml[part] = make_float2(mx, l);

@@ -1,320 +1,774 @@
-// Gradients of window attention.  With S = Q K^T scale, P = exp(S - lse) over
-// the visible keys and delta_i = sum_d dO_id O_id:
+// Window attention's gradients on tcgen05 tiles.  One pipeline, two forms:
 //
-//   dV = P^T dO      dP = dO V^T      dS = P (dP - delta)
-//   dQ = dS K scale  dK = dS^T Q scale
+//   form     owns (128 rows)  streams     accumulates
+//   kKeys    K, V             Q, dO       dK += dS^T Q, dV += P^T dO
+//   queries  Q, dO            K, V        dQ += dS K
 //
-// Three kernels without atomics, so that results do not depend on any order:
-// delta; dK and dV (a CTA owns 64 keys and walks the query tiles that see
-// them, over all query heads that share the keys); dQ (a CTA owns 64 queries
-// and walks the key tiles that they see).  S and dP are computed twice, 14 D
-// flops per visible pair instead of 10 D.
+// Each step forms S = own1 str1^T and dP = own2 str2^T (fp32, TMEM, the owned
+// rows on the lanes), the elementwise warps turn them into P = exp2(S c - lse)
+// and dS = P (dP - delta) as bf16 in TMEM, and those are the A operands of the
+// accumulating products, whose B operands are the streamed tiles again (now
+// read along their rows).  Every output element has one owner that adds in a
+// fixed order: no atomics, equal bits from call to call.  (The key tiles that
+// hold sinks are seen by all later queries.  Where that would be the longest
+// chain of the launch, their steps are divided among sink_parts CTAs, whose
+// fp32 sums sink_sum_kernel adds in order.)
+//
+// TMEM (all 512 columns at D = 128): kSBufs buffers of S, one of dP, the
+// accumulators.  P and dS overwrite their S.  A step is a chain of signals of
+// about 300 cycles each (product -> barrier -> TMEM load -> barrier -> next
+// product), longer than its products: with one buffer of S and dP the chain
+// took 2,050 cycles a step where the products need 1,280 (kKeys).  So S runs
+// steps ahead, and dP alone waits for its one buffer, which is free as soon as
+// it is in the registers.  kKeys steps are 64 queries wide: two accumulators
+// of D columns leave no room for 128.
+//
+// Roles: elementwise and epilogue warps (warp w: lanes 32 (w % 4), the w / 4th
+// share of the columns), then a TMA warp, one that issues S and dP and one that
+// issues the accumulating products.  Waits are bounded as in the forward kernel.
 #pragma once
 
-#include "mma_sync.cuh"
+#include "attention_kernel.cuh"
 #include "ptx.cuh"
 #include "view.cuh"
 
 namespace b200 {
 namespace bwd {
 
-constexpr int kThreads = 128;
-constexpr int kTile = 64;  // keys or queries of a tile; 16 of the owned ones per warp
+constexpr int kOwn = 128;  // owned rows
+constexpr int kBarQuad = 1;  // named barriers 1-4: the warps of a lane quadrant
 
-template <int D>
-struct Cfg {
-  static constexpr int kRowBytes = 2 * D;
-  static constexpr int kTileBytes = kTile * kRowBytes;
-  // The owned pair of tiles, and two stages of the walked pair with the
-  // queries' lse and delta.
-  static constexpr int kStageBytes = 2 * kTileBytes + 2 * kTile * 4;
-  static constexpr int kSmemBytes = 2 * kTileBytes + 2 * kStageBytes;
+template <int D, bool kKeys>
+struct TileCfg {
+  static constexpr int kN = kKeys ? 64 : 128;  // streamed rows of a step
+  static constexpr int kGroups = 4;                 // elementwise warpgroups
+  static constexpr int kWarps = 4 * kGroups;     // elementwise warps
+  static constexpr int kCols = kN / kGroups;     // columns of a step for each
+  static constexpr int kThreads = 32 * (kWarps + 4);
+  // Epilogue: warpgroups of an accumulator, columns for each.
+  static constexpr int kAccGroups = kKeys ? kGroups / 2 : kGroups;
+  static constexpr int kAccCols = D / kAccGroups;
+  // Ring depths of the two streamed tensors.  Both of kKeys' live until the
+  // accumulating products have read them, but V only until dP has: K gets the
+  // odd stage.
+  static constexpr int kStages1 = (kKeys ? 4 : 3) * (128 / D);
+  static constexpr int kStages2 = (kKeys ? 4 : 2) * (128 / D);
+  static constexpr int kBoxes = D / 64;
+  static constexpr int kOwnBox = kOwn * 128;
+  static constexpr int kOwnBytes = kBoxes * kOwnBox;
+  static constexpr int kStrBox = kN * 128;
+  static constexpr int kStrBytes = kBoxes * kStrBox;
+  static constexpr int kStatBytes = kKeys ? 2 * kN * 4 : 0;  // -lse, -delta of the queries
+  static constexpr int kRingOff = 2 * kOwnBytes;
+  static constexpr int kRing2Off = kRingOff + kStages1 * kStrBytes;
+  static constexpr int kStatOff = kRing2Off + kStages2 * kStrBytes;
+  static constexpr int kBarOff = kStatOff + kStages2 * kStatBytes;
+  // own_full own_empty p_free[3] sd_ready dp_free p_ready[2] acc_full acc_empty drain
+  static constexpr int kNumBars = 12 + 2 * (kStages1 + kStages2);
+  static constexpr int kSlotOff = kBarOff + kNumBars * 8;
+  static constexpr int kSmemBytes = kSlotOff + 16 + 1024;  // + alignment slack
+  static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
+  static_assert(kSmemBytes > 116 * 1024, "one CTA per SM: each takes all of TMEM");
+  static constexpr int kSBufs = kKeys ? 3 : 2;
+  static constexpr uint32_t kColDp = kSBufs * kN;
+  static constexpr uint32_t kDs = kKeys ? kN / 2 : 0;  // dS in its S buffer (P at 0)
+  static constexpr uint32_t kColAcc1 = 512 - 2 * D, kColAcc2 = 512 - D;
+  static_assert(kColDp + kN <= (kKeys ? kColAcc1 : kColAcc2), "TMEM columns");
+  static constexpr uint32_t kIdescS = idesc_bf16_f32(kOwn, kN, false, false);
+  static constexpr uint32_t kIdescAcc = idesc_bf16_f32(kOwn, D, false, true);
 };
 
-struct Params {
-  View dout, q, k, v, o, dq, dk, dv;
-  const float* lse;    // [B, Hq, Sq]
-  float* delta;        // [B, Hq, Sq]
+struct TileParams {
+  View out1, out2;       // kKeys: dK, dV; queries: dQ
+  const float* stats;    // [2][B * Hq][sq_pad]: -lse in log2 units, -delta
+  int64_t stat_plane;    // B * Hq * sq_pad
+  int sq_pad;            // Sq up to a multiple of 64
   const int32_t* kv_len;
   int B, Hq, Hkv, group, Sq, Skv;
-  int q_tiles, k_tiles;
-  int window, sinks;  // at most Skv
+  int tiles;             // owned tiles of a (batch, head)
+  int n_items;
+  // kKeys: the first sink_tiles tiles are divided into sink_parts units each
+  // (0: none are), which write [B * Hkv][sink_tiles][sink_parts][dK, dV][128][D].
+  int sink_tiles, sink_parts;
+  float* sink_sums;
+  int window, sinks;
   float scale, scale_log2;
+  // Coordinate factors of broadcast axes (own1, own2, str1, str2; batch, head).
+  int o1_b, o1_h, o2_b, o2_h, s1_b, s1_h, s2_b, s2_h;
 };
 
-__device__ __forceinline__ int batch_len(const Params& p, int b) {
-  return p.kv_len ? max(0, min(p.kv_len[b], p.Skv)) : p.Skv;
-}
+enum : uint32_t {
+  kSiteBwdOwn = 0x20, kSiteBwdFull, kSiteBwdEmpty, kSiteBwdS, kSiteBwdP,
+  kSiteBwdAcc
+};
 
-// delta; one warp to a row.
+// -lse and -delta of every query row, padded with zeros.  D/8 lanes to a row
+// (16 bytes each of dO and O), four rows of each in flight.
 template <int D>
-__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Params p) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + warp_id();
-  if (row >= static_cast<int64_t>(p.B) * p.Hq * p.Sq) return;
-  const int64_t bh = row / p.Sq, s = row - bh * p.Sq, b = bh / p.Hq, h = bh - b * p.Hq;
-  const uint16_t* x = p.dout.row(b, h, s);
-  const uint16_t* y = p.o.row(b, h, s);
-  float sum = 0.0f;
+__global__ void __launch_bounds__(256)
+    stats_kernel(const View dout, const View o, const float* lse, float* stats, int64_t plane,
+                 int sq_pad, int B, int Hq, int Sq) {
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = 4;
+  pdl_launch_dependents();
+  const int lane = static_cast<int>(threadIdx.x) % kLanes;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kUnroll) +
+                       static_cast<int>(threadIdx.x) / kLanes;
+  uint4 x[kUnroll], y[kUnroll];
+  float l[kUnroll];
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const int c = i * 32 + static_cast<int>(lane_id());
-    const uint32_t a = reinterpret_cast<const uint32_t*>(x)[c];
-    const uint32_t e = reinterpret_cast<const uint32_t*>(y)[c];
-    sum = fmaf(__uint_as_float(a << 16), __uint_as_float(e << 16), sum);
-    sum = fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(e & 0xffff0000u), sum);
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t row = row0 + u * kRows;
+    x[u] = y[u] = make_uint4(0u, 0u, 0u, 0u);
+    l[u] = 0.0f;
+    const int64_t bh = row / sq_pad, s = row - bh * sq_pad, b = bh / Hq, h = bh - b * Hq;
+    if (row < plane && s < Sq) {
+      x[u] = __ldg(reinterpret_cast<const uint4*>(dout.row(b, h, s)) + lane);
+      y[u] = __ldg(reinterpret_cast<const uint4*>(o.row(b, h, s)) + lane);
+      l[u] = __ldg(lse + bh * Sq + s);
+    }
   }
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-  if (lane_id() == 0) p.delta[row] = sum;
-}
-
-// Rows [r0, r0 + 64) of one head of a tensor; rows outside [0, se) and
-// [lo, hi) are zeroed and not read.
-template <int D>
-__device__ __forceinline__ void load_tile(uint32_t dst, const View& t, int b, int h, int r0,
-                                          int se, int lo, int hi) {
-  constexpr int kChunks = D / 8;
-  const uint16_t* base = t.row(b, h, 0);
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t row = row0 + u * kRows;
+    const uint32_t a[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+    const uint32_t e[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+    float sum = 0.0f;
 #pragma unroll
-  for (int u = 0; u < kTile * kChunks / kThreads; ++u) {
-    const int idx = u * kThreads + static_cast<int>(threadIdx.x);
-    const int r = idx / kChunks, c = idx % kChunks;
-    const int row = r0 + r;
-    const bool live = row < hi && (row >= lo || row < se);
-    cp_async16(dst + swz<2 * D>(r, c), base + (live ? row : 0) * t.ss + c * 8, live);
-  }
-}
-
-// acc[t] (16 x 8 each, t = 0..3) = A (16 rows at a_row0 of tile a) x B^T
-// (32 rows at b_row0 of tile b), over D.
-template <int D>
-__device__ __forceinline__ void product_t(float (&acc)[4][4], uint32_t a, int a_row0, uint32_t b,
-                                          int b_row0) {
-  const int lane = static_cast<int>(lane_id());
-  const int ar = a_row0 + (lane & 15), ac = lane >> 4;
-  const int br = b_row0 + ((lane >> 4) << 3) + (lane & 7), bc = (lane >> 3) & 1;
+    for (int i = 0; i < 4; ++i) {
+      sum = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(e[i] << 16), sum);
+      sum = fmaf(__uint_as_float(a[i] & 0xffff0000u), __uint_as_float(e[i] & 0xffff0000u), sum);
+    }
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
-#pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) {
-    uint32_t fa[4], f0[4], f1[4];
-    ldsm4(a + swz<2 * D>(ar, 2 * kk + ac), fa);
-    ldsm4(b + swz<2 * D>(br, 2 * kk + bc), f0);
-    ldsm4(b + swz<2 * D>(br + 16, 2 * kk + bc), f1);
-    mma_bf16(acc[0], fa, f0[0], f0[1]);
-    mma_bf16(acc[1], fa, f0[2], f0[3]);
-    mma_bf16(acc[2], fa, f1[0], f1[1]);
-    mma_bf16(acc[3], fa, f1[2], f1[3]);
-  }
-}
-
-// out (16 x D) += X (16 x 32, as accumulators, rounded to bf16 for the tensor
-// cores) x B (32 rows at b_row0 of tile b).
-template <int D>
-__device__ __forceinline__ void accumulate(float (&out)[D / 8][4], const float (&x)[4][4],
-                                           uint32_t b, int b_row0) {
-  const int lane = static_cast<int>(lane_id());
-  const int br = b_row0 + (lane & 15), bc = lane >> 4;
-#pragma unroll
-  for (int kc = 0; kc < 2; ++kc) {
-    const uint32_t a[4] = {
-        pack_bf16x2(x[2 * kc][0], x[2 * kc][1]), pack_bf16x2(x[2 * kc][2], x[2 * kc][3]),
-        pack_bf16x2(x[2 * kc + 1][0], x[2 * kc + 1][1]),
-        pack_bf16x2(x[2 * kc + 1][2], x[2 * kc + 1][3])};
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      uint32_t f[4];
-      ldsm4_trans(b + swz<2 * D>(br + 16 * kc, 2 * d + bc), f);
-      mma_bf16(out[2 * d], a, f[0], f[1]);
-      mma_bf16(out[2 * d + 1], a, f[2], f[3]);
+    for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    if (lane == 0 && row < plane) {
+      stats[row] = l[u] == -INFINITY ? 0.0f : l[u] * -1.4426950408889634f;
+      stats[plane + row] = -sum;
     }
   }
 }
 
-template <int D>
-__device__ __forceinline__ void store_rows(const View& t, int b, int h, int r0, int rows,
-                                           const float (&x)[D / 8][4], float scale) {
-  const int lane = static_cast<int>(lane_id());
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = r0 + (lane >> 2) + 8 * half;
-    if (r >= rows) continue;
-    uint16_t* dst = t.row(b, h, r) + 2 * (lane & 3);
-#pragma unroll
-    for (int d = 0; d < D / 8; ++d)
-      *reinterpret_cast<uint32_t*>(dst + 8 * d) =
-          pack_bf16x2(x[d][2 * half] * scale, x[d][2 * half + 1] * scale);
-  }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
 
-// dK, dV of 64 keys.
-template <int D>
-__global__ void __launch_bounds__(kThreads) dkdv_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<D>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t ks = smem_u32(smem), vs = ks + C::kTileBytes, ring = vs + C::kTileBytes;
-  // The first key tiles (sinks) are seen by the most queries: they start first.
-  const int kt = static_cast<int>(blockIdx.x / (p.B * p.Hkv));
-  const int bh = static_cast<int>(blockIdx.x % (p.B * p.Hkv));
-  const int b = bh / p.Hkv, h = bh - b * p.Hkv;
-  const int n = batch_len(p, b), off = n - p.Sq;
-  const int k0 = kt * kTile, k1 = min(k0 + kTile, n);
-  // Queries [i0, i1) see some of keys [k0, k1).
-  const int i0 = max(0, k0 - off);
-  const int i1 = k1 <= k0 ? 0 : k0 < p.sinks ? p.Sq : min(p.Sq, k1 - 1 + p.window - off);
-  const int t0 = i0 / kTile;
-  const int nt = i1 > i0 ? (i1 + kTile - 1) / kTile - t0 : 0;
-  const int steps = nt * p.group;
-  const int warp = static_cast<int>(warp_id()), lane = static_cast<int>(lane_id());
+// TMEM loads and stores of a thread's columns.
+__device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t (&r)[16]) {
+  tmem_st16(taddr, r);
+}
+__device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t (&r)[8]) {
+  tmem_st8(taddr, r);
+}
+__device__ __forceinline__ void written_here(uint32_t (&r)[32]) { reg_written_here(r); }
+__device__ __forceinline__ void written_here(uint32_t (&r)[16]) { reg_written_here16(r); }
 
-  float dk[D / 8][4], dv[D / 8][4];
+// Transposes 16-byte pieces among groups of kShare lanes: afterwards piece e of
+// lane q is what piece q of lane e was.
+template <int kShare>
+__device__ __forceinline__ void exchange(uint32_t (&x)[4 * kShare], int lane) {
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i)
+  for (int m = 1; m < kShare; m <<= 1) {
+    const bool up = lane & m;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dk[i][e] = dv[i][e] = 0.0f;
-
-  // Step i: query head h * group + i / nt, query tile t0 + i % nt.
-  auto load_step = [&](int i) {
-    if (i < steps) {
-      const int hq = h * p.group + i / nt, r0 = (t0 + i % nt) * kTile;
-      const uint32_t dst = ring + (i & 1) * C::kStageBytes;
-      const int live0 = max(0, -off);  // earlier rows see nothing
-      load_tile<D>(dst, p.q, b, hq, r0, 0, live0, p.Sq);
-      load_tile<D>(dst + C::kTileBytes, p.dout, b, hq, r0, 0, live0, p.Sq);
-      float* st = reinterpret_cast<float*>(smem + 2 * C::kTileBytes + (i & 1) * C::kStageBytes +
-                                           2 * C::kTileBytes);
-      if (threadIdx.x < kTile) {
-        const int r = r0 + static_cast<int>(threadIdx.x);
-        const int64_t at = (static_cast<int64_t>(b) * p.Hq + hq) * p.Sq + r;
-        const float lse = r < p.Sq ? p.lse[at] : -INFINITY;
-        st[threadIdx.x] = lse == -INFINITY ? 0.0f : lse * 1.4426950408889634f;
-        st[kTile + threadIdx.x] = r < p.Sq ? p.delta[at] : 0.0f;
+    for (int e = 0; e < kShare; ++e) {
+      if (e & m) continue;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t& a = x[4 * e + u];
+        uint32_t& b = x[4 * (e | m) + u];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? a : b, m);
+        if (up)
+          a = got;
+        else
+          b = got;
       }
     }
-    cp_async_commit();
-  };
-  if (steps > 0) {
-    load_tile<D>(ks, p.k, b, h, k0, 0, 0, n);
-    load_tile<D>(vs, p.v, b, h, k0, 0, 0, n);
   }
-  load_step(0);
-  for (int i = 0; i < steps; ++i) {
-    load_step(i + 1);
-    cp_async_wait<1>();
-    __syncthreads();
-    const uint32_t qs = ring + (i & 1) * C::kStageBytes, os = qs + C::kTileBytes;
-    const float* st = reinterpret_cast<const float*>(
-        smem + 2 * C::kTileBytes + (i & 1) * C::kStageBytes + 2 * C::kTileBytes);
-    const int r0 = (t0 + i % nt) * kTile;
-#pragma unroll 1
-    for (int c0 = 0; c0 < kTile; c0 += 32) {
-      float s[4][4], dp[4][4];
-      product_t<D>(s, ks, warp * 16, qs, c0);
-      product_t<D>(dp, vs, warp * 16, os, c0);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int qi = c0 + 8 * t + 2 * (lane & 3) + (e & 1);
-          const int j = k0 + warp * 16 + (lane >> 2) + 8 * (e >> 1);
-          const int pos = off + r0 + qi;
-          const bool seen = r0 + qi < p.Sq && j <= pos && (pos - j < p.window || j < p.sinks);
-          s[t][e] = seen ? ex2_approx(fmaf(s[t][e], p.scale_log2, -st[qi])) : 0.0f;
-          dp[t][e] = seen ? s[t][e] * (dp[t][e] - st[kTile + qi]) : 0.0f;
-        }
-      accumulate<D>(dv, s, os, c0);
-      accumulate<D>(dk, dp, qs, c0);
-    }
-    __syncthreads();  // the stage is free
-  }
-  cp_async_wait<0>();
-  store_rows<D>(p.dk, b, h, k0 + warp * 16, p.Skv, dk, p.scale);
-  store_rows<D>(p.dv, b, h, k0 + warp * 16, p.Skv, dv, 1.0f);
 }
 
-// dQ of 64 queries.
-template <int D>
-__global__ void __launch_bounds__(kThreads) dq_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<D>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t qs = smem_u32(smem), os = qs + C::kTileBytes, ring = os + C::kTileBytes;
-  const int qt = p.q_tiles - 1 - static_cast<int>(blockIdx.x / (p.B * p.Hq));
-  const int bh = static_cast<int>(blockIdx.x % (p.B * p.Hq));
-  const int b = bh / p.Hq, hq = bh - b * p.Hq, h = hq / p.group;
-  const int n = batch_len(p, b), off = n - p.Sq;
-  const int r0 = qt * kTile, r_last = min(r0 + kTile, p.Sq) - 1;
-  // Keys [0, se) and [lo, hi) are seen by some of the tile's queries.
-  const int hi = max(0, off + r_last + 1);
-  int lo = max(0, off + r0 - p.window + 1);
-  if (p.sinks >= lo || hi == 0) lo = 0;
-  const int se = lo > 0 ? p.sinks : 0;
-  const int ns = min((se + kTile - 1) / kTile, lo / kTile);  // sink tiles before the window's
-  const int t0 = lo / kTile;
-  const int steps = ns + (hi + kTile - 1) / kTile - t0;
+// One owned tile: where it lies and what it streams.
+template <bool kKeys>
+struct TileItem {
+  int b, h;         // h: kv head (kKeys) or query head
+  int r0;           // first owned row
+  int n, off;       // keys of the request; position of query row 0
+  int steps;
+  int per_head, t0;             // kKeys: steps of a query head, first 64-query tile
+  int first, part;              // kKeys: first step; the part of a divided tile, or -1
+  int se, lo, hi, n_sink, skip;  // queries: as in the forward kernel
+};
+
+template <bool kKeys>
+__device__ __forceinline__ TileItem<kKeys> tile_item(const TileParams& p, int k) {
+  TileItem<kKeys> it;
+  const int heads = kKeys ? p.Hkv : p.Hq;
+  // All (batch, head) of one tile index are adjacent: for keys the first tiles
+  // (sinks, seen by most queries) start first, for queries the last ones.
+  it.part = -1;
+  if (kKeys && p.sink_parts > 0) {
+    const int divided = p.B * heads * p.sink_tiles * p.sink_parts;
+    if (k < divided) {
+      it.part = k % p.sink_parts;
+      k /= p.sink_parts;
+    } else {
+      k -= divided - p.B * heads * p.sink_tiles;
+    }
+  }
+  int tile = k / (p.B * heads);
+  const int bh = k - tile * (p.B * heads);
+  if (!kKeys) tile = p.tiles - 1 - tile;
+  it.b = bh / heads;
+  it.h = bh - it.b * heads;
+  it.r0 = tile * kOwn;
+  it.n = p.kv_len ? max(0, min(__ldg(p.kv_len + it.b), p.Skv)) : p.Skv;
+  it.off = it.n - p.Sq;
+  if constexpr (kKeys) {
+    const int k1 = min(it.r0 + kOwn, it.n);  // queries [i0, i1) see some of keys [r0, k1)
+    const int i0 = max(0, it.r0 - it.off);
+    const int i1 = k1 <= it.r0 ? 0
+                   : it.r0 < p.sinks ? p.Sq
+                                     : min(p.Sq, k1 - 1 + p.window - it.off);
+    it.t0 = i0 / 64;
+    it.per_head = i1 > i0 ? (i1 + 63) / 64 - it.t0 : 0;
+    it.first = 0;
+    it.steps = it.per_head * p.group;
+    if (it.part >= 0) {
+      const int64_t all = it.steps;
+      it.first = static_cast<int>(all * it.part / p.sink_parts);
+      it.steps = static_cast<int>(all * (it.part + 1) / p.sink_parts) - it.first;
+    }
+  } else {
+    const int last = it.off + min(it.r0 + kOwn, p.Sq) - 1;
+    it.hi = max(0, last + 1);
+    it.lo = max(0, it.off + it.r0 - p.window + 1);
+    if (p.sinks >= it.lo || it.hi == 0) it.lo = 0;
+    it.se = it.lo > 0 ? p.sinks : 0;
+    const int w0 = it.lo / 128;
+    it.per_head = -1;
+    it.n_sink = min((it.se + 127) / 128, w0);
+    it.skip = w0 - it.n_sink;
+    it.steps = it.n_sink + (it.hi + 127) / 128 - w0;
+  }
+  return it;
+}
+
+// P and dS of kCols columns of this thread's row, as bf16 pairs.  kKeys: -lse and
+// -delta of the columns at st_l and st_l + n; else the row's own.
+template <bool kKeys, bool kMasked, int kCols>
+__device__ __forceinline__ void elementwise(const uint32_t (&s)[kCols], const uint32_t (&d)[kCols],
+                                            uint64_t c2, const float* st_l, int n, float nlse,
+                                            float ndelta, int col0, int va, int vb, int vs,
+                                            uint32_t (&pk)[kCols / 2],
+                                            uint32_t (&dk)[kCols / 2]) {
+#pragma unroll
+  for (int e = 0; e < kCols / 2; ++e) {
+    uint64_t nl2, nd2;
+    if constexpr (kKeys) {
+      nl2 = *reinterpret_cast<const uint64_t*>(st_l + 2 * e);
+      nd2 = *reinterpret_cast<const uint64_t*>(st_l + n + 2 * e);
+    } else {
+      nl2 = f2_pack(nlse, nlse);
+      nd2 = f2_pack(ndelta, ndelta);
+    }
+    const uint64_t x2 =
+        f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, nl2);
+    float x0, x1;
+    f2_unpack(x2, x0, x1);
+    float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+    const uint64_t g2 =
+        f2_mul(f2_pack(p0, p1),
+               f2_add(f2_pack(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1])), nd2));
+    float g0, g1;
+    f2_unpack(g2, g0, g1);
+    if constexpr (kMasked) {
+      const int u = col0 + 2 * e;
+      bool see0 = u >= va && u < vb, see1 = u + 1 >= va && u + 1 < vb;
+      if constexpr (!kKeys) {
+        see0 |= u < vs;
+        see1 |= u + 1 < vs;
+      }
+      p0 = see0 ? p0 : 0.0f;
+      p1 = see1 ? p1 : 0.0f;
+      g0 = see0 ? g0 : 0.0f;
+      g1 = see1 ? g1 : 0.0f;
+    }
+    if constexpr (kKeys) pk[e] = pack_bf16x2(p0, p1);
+    dk[e] = pack_bf16x2(g0, g1);
+  }
+}
+
+template <int D, bool kKeys>
+__global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
+    bwd_tile_kernel(const __grid_constant__ CUtensorMap own1_map,
+                    const __grid_constant__ CUtensorMap own2_map,
+                    const __grid_constant__ CUtensorMap str1_map,
+                    const __grid_constant__ CUtensorMap str2_map,
+                    const __grid_constant__ TileParams p) {
+  using C = TileCfg<D, kKeys>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* own = smem;
+  uint8_t* ring1 = smem + C::kRingOff;
+  uint8_t* ring2 = smem + C::kRing2Off;
+  float* stat = reinterpret_cast<float*>(smem + C::kStatOff);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t *own_full = bars, *own_empty = bars + 1, *p_free = bars + 2, *sd_ready = bars + 5,
+           *dp_free = bars + 6, *p_ready = bars + 7, *acc_full = bars + 9,
+           *acc_empty = bars + 10, *drain = bars + 11, *full1 = bars + 12,
+           *empty1 = full1 + C::kStages1, *full2 = empty1 + C::kStages1,
+           *empty2 = full2 + C::kStages2;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kSlotOff);
   const int warp = static_cast<int>(warp_id()), lane = static_cast<int>(lane_id());
 
-  float dq[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) dq[i][e] = 0.0f;
-  auto tile_of = [&](int i) { return i < ns ? i : t0 + i - ns; };
-  auto load_step = [&](int i) {
-    if (i < steps) {
-      const int k0 = tile_of(i) * kTile;
-      const uint32_t dst = ring + (i & 1) * C::kStageBytes;
-      load_tile<D>(dst, p.k, b, h, k0, se, lo, hi);
-      load_tile<D>(dst + C::kTileBytes, p.v, b, h, k0, se, lo, hi);
+  if (threadIdx.x == 0) {
+    mbar_init(own_full, 1);
+    mbar_init(own_empty, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&p_free[i], 1);
+    mbar_init(sd_ready, 1);
+    mbar_init(dp_free, C::kWarps);
+    // Two: a warp may be a step ahead of another, but not two (dP's buffer).
+    mbar_init(&p_ready[0], C::kWarps);
+    mbar_init(&p_ready[1], C::kWarps);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, C::kWarps);
+    mbar_init(drain, 2);
+    for (int i = 0; i < 2 * (C::kStages1 + C::kStages2); ++i) mbar_init(&full1[i], 1);
+    fence_mbar_init();
+  }
+  if (warp == C::kWarps) {
+    tmem_alloc(slot, 512);
+    tmem_relinquish();
+    if (lane == 0) {
+      tma_prefetch_desc(&own1_map);
+      tma_prefetch_desc(&own2_map);
+      tma_prefetch_desc(&str1_map);
+      tma_prefetch_desc(&str2_map);
     }
-    cp_async_commit();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  pdl_wait();  // the row statistics
+
+  // First streamed row of a query head's step i.
+  auto str_row = [&](const TileItem<kKeys>& it, int i) {
+    if constexpr (kKeys)
+      return (it.t0 + i) * 64;
+    else
+      return (i < it.n_sink ? i : i + it.skip) * 128;
   };
-  if (steps > 0) {
-    load_tile<D>(qs, p.q, b, hq, r0, 0, max(0, -off), p.Sq);
-    load_tile<D>(os, p.dout, b, hq, r0, 0, max(0, -off), p.Sq);
-  }
-  load_step(0);
-  float lse[2], delta[2];
-  int pos[2];
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = min(r0 + warp * 16 + (lane >> 2) + 8 * half, p.Sq - 1);
-    const int64_t at = (static_cast<int64_t>(b) * p.Hq + hq) * p.Sq + r;
-    const float x = p.lse[at];
-    lse[half] = x == -INFINITY ? 0.0f : x * 1.4426950408889634f;
-    delta[half] = p.delta[at];
-    pos[half] = off + r;
-  }
-  for (int i = 0; i < steps; ++i) {
-    load_step(i + 1);
-    cp_async_wait<1>();
-    __syncthreads();
-    const uint32_t ks = ring + (i & 1) * C::kStageBytes, vs = ks + C::kTileBytes;
-    const int k0 = tile_of(i) * kTile;
-#pragma unroll 1
-    for (int c0 = 0; c0 < kTile; c0 += 32) {
-      float s[4][4], dp[4][4];
-      product_t<D>(s, qs, warp * 16, ks, c0);
-      product_t<D>(dp, os, warp * 16, vs, c0);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int half = e >> 1;
-          const int j = k0 + c0 + 8 * t + 2 * (lane & 3) + (e & 1);
-          const bool seen =
-              j <= pos[half] && (pos[half] - j < p.window || j < p.sinks);
-          const float w =
-              seen ? ex2_approx(fmaf(s[t][e], p.scale_log2, -lse[half])) : 0.0f;
-          dp[t][e] = seen ? w * (dp[t][e] - delta[half]) : 0.0f;
+
+  if (warp == C::kWarps) {
+    // ================= TMA producer =================
+    if (lane == 0) {
+      const uint64_t pol_own = l2_policy_evict_first(), pol_str = l2_policy_evict_last();
+      int t = 0, li = 0, n1 = 0, n2 = 0;  // steps; copies issued
+      bool ok = true;
+      for (int k = static_cast<int>(blockIdx.x); k < p.n_items && ok; k += gridDim.x) {
+        const TileItem<kKeys> it = tile_item<kKeys>(p, k);
+        if (it.steps == 0) continue;
+        ok = mbar_wait(own_empty, (static_cast<uint32_t>(li) & 1u) ^ 1u, kSiteBwdOwn,
+                       kDefaultWaitLimitNs, 20000u);
+        if (!ok) break;
+        mbar_arrive_expect_tx(own_full, 2 * C::kOwnBytes);
+        for (int x = 0; x < C::kBoxes; ++x) {
+          tma_load_4d(own + x * C::kOwnBox, &own1_map, own_full, x * 64, it.r0, it.h * p.o1_h,
+                      it.b * p.o1_b, pol_own);
+          tma_load_4d(own + C::kOwnBytes + x * C::kOwnBox, &own2_map, own_full, x * 64, it.r0,
+                      it.h * p.o2_h, it.b * p.o2_b, pol_own);
         }
-      accumulate<D>(dq, dp, ks, c0);
+        ++li;
+        // Step of a query head; the head.
+        int hi = kKeys && it.steps > 0 ? it.first % it.per_head : 0;
+        int hq = kKeys ? it.h * p.group + it.first / max(it.per_head, 1) : it.h;
+        for (int i = 0; i < it.steps; ++i, ++t) {
+          const int st1 = t % C::kStages1, st2 = t % C::kStages2;
+          const int row = str_row(it, hi);
+          const int h = kKeys ? hq : it.h / p.group;
+          ok = mbar_wait(&empty1[st1], (static_cast<uint32_t>(t / C::kStages1) & 1u) ^ 1u,
+                         kSiteBwdEmpty, kDefaultWaitLimitNs, 20000u);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full1[st1], C::kStrBytes);
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_4d(ring1 + st1 * C::kStrBytes + x * C::kStrBox, &str1_map, &full1[st1],
+                        x * 64, row, h * p.s1_h, it.b * p.s1_b, pol_str);
+          n1 = t + 1;
+          ok = mbar_wait(&empty2[st2], (static_cast<uint32_t>(t / C::kStages2) & 1u) ^ 1u,
+                         kSiteBwdEmpty, kDefaultWaitLimitNs, 20000u);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full2[st2], C::kStrBytes + C::kStatBytes);
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_4d(ring2 + st2 * C::kStrBytes + x * C::kStrBox, &str2_map, &full2[st2],
+                        x * 64, row, h * p.s2_h, it.b * p.s2_b, pol_str);
+          if constexpr (kKeys) {
+            const float* src =
+                p.stats + (static_cast<int64_t>(it.b) * p.Hq + hq) * p.sq_pad + row;
+            float* sdst = stat + st2 * 2 * C::kN;
+            bulk_load(sdst, src, C::kN * 4, &full2[st2]);
+            bulk_load(sdst + C::kN, src + p.stat_plane, C::kN * 4, &full2[st2]);
+          }
+          n2 = t + 1;
+          ++hi;
+          if (kKeys && hi == it.per_head) {
+            hi = 0;
+            ++hq;
+          }
+        }
+      }
+      if (!ok) {
+        // Unwinding: let every copy already issued land before the CTA exits.
+        if (li > 0) attn::drain_wait(own_full, static_cast<uint32_t>(li - 1) & 1u);
+        for (int i = max(0, n1 - C::kStages1); i < n1; ++i)
+          attn::drain_wait(&full1[i % C::kStages1], static_cast<uint32_t>(i / C::kStages1) & 1u);
+        for (int i = max(0, n2 - C::kStages2); i < n2; ++i)
+          attn::drain_wait(&full2[i % C::kStages2], static_cast<uint32_t>(i / C::kStages2) & 1u);
+      }
     }
-    __syncthreads();
+    __syncwarp();
+  } else if (warp == C::kWarps + 1 || warp == C::kWarps + 2) {
+    // ================= MMA issuers =================
+    const bool acc = warp == C::kWarps + 2;
+    const uint32_t own_addr = smem_u32(own);
+    const uint64_t d_own1 = sdesc_sw128(own_addr, 16, 1024);
+    const uint64_t d_own2 = sdesc_sw128(own_addr + C::kOwnBytes, 16, 1024);
+    // Streamed tiles with their rows as N (S, dP) and as K (accumulation).
+    const uint64_t d_n1 = sdesc_sw128(smem_u32(ring1), 16, 1024);
+    const uint64_t d_n2 = sdesc_sw128(smem_u32(ring2), 16, 1024);
+    const uint64_t d_k1 = sdesc_sw128(smem_u32(ring1), C::kStrBox, 1024);
+    const uint64_t d_k2 = sdesc_sw128(smem_u32(ring2), C::kStrBox, 1024);
+    constexpr uint32_t kStr16 = C::kStrBytes >> 4;
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
+      const bool ok = attn::warp_wait(bar, parity, site);
+      tc_fence_after();
+      return ok;
+    };
+    int t = 0, li = 0;
+    bool ok = true;
+    for (int k = static_cast<int>(blockIdx.x); k < p.n_items && ok; k += gridDim.x) {
+      const int steps = tile_item<kKeys>(p, k).steps;
+      if (steps == 0) continue;
+      if (!acc) {
+        ok = warp_wait(own_full, static_cast<uint32_t>(li) & 1u, kSiteBwdOwn);
+      } else {
+        // The epilogue of the item before has read the accumulators.
+        ok = warp_wait(acc_empty, (static_cast<uint32_t>(li) & 1u) ^ 1u, kSiteBwdAcc);
+      }
+      ++li;
+      for (int i = 0; i < steps && ok; ++i, ++t) {
+        const int st1 = t % C::kStages1, st2 = t % C::kStages2;
+        const uint32_t par1 = static_cast<uint32_t>(t / C::kStages1) & 1u;
+        const uint32_t par2 = static_cast<uint32_t>(t / C::kStages2) & 1u;
+        const int sb = t % C::kSBufs;  // S buffer
+        const uint32_t t_s = tmem + static_cast<uint32_t>(sb * C::kN);
+        if (!acc) {
+          // S(t), once the products of step t - kSBufs have read P and dS there.
+          {
+            const uint32_t f = smem_u32(&full1[st1]);
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait3(f, par1, smem_u32(&p_free[sb]),
+                                       (static_cast<uint32_t>(t / C::kSBufs) & 1u) ^ 1u, f, par1,
+                                       kSiteBwdFull));
+          }
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss_warp(t_s, d_own1 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
+                        d_n1 + st1 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
+                        C::kIdescS, kk > 0 ? 1u : 0u);
+          // dP(t), once dP(t - 1) is in the registers.
+          {
+            const uint32_t f = smem_u32(&full2[st2]);
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait3(f, par2, smem_u32(dp_free),
+                                       (static_cast<uint32_t>(t) & 1u) ^ 1u, f, par2,
+                                       kSiteBwdFull));
+          }
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss_warp(tmem + C::kColDp, d_own2 + (kk >> 2) * (C::kOwnBox >> 4) + (kk & 3) * 2,
+                        d_n2 + st2 * kStr16 + (kk >> 2) * (C::kStrBox >> 4) + (kk & 3) * 2,
+                        C::kIdescS, kk > 0 ? 1u : 0u);
+          if constexpr (!kKeys) mma_commit_warp(&empty2[st2]);
+          mma_commit_warp(sd_ready);
+          if (i + 1 == steps) mma_commit_warp(own_empty);
+        } else {
+          ok = warp_wait(&p_ready[t & 1], static_cast<uint32_t>(t >> 1) & 1u, kSiteBwdP);
+          if (!ok) break;
+          if constexpr (kKeys) {
+#pragma unroll
+            for (int kk = 0; kk < C::kN / 16; ++kk)
+              mma_ts_warp(tmem + C::kColAcc2, t_s + kk * 8,
+                          d_k2 + st2 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
+                          (i > 0 || kk > 0) ? 1u : 0u);
+          }
+#pragma unroll
+          for (int kk = 0; kk < C::kN / 16; ++kk)
+            mma_ts_warp(tmem + (kKeys ? C::kColAcc1 : C::kColAcc2), t_s + C::kDs + kk * 8,
+                        d_k1 + st1 * kStr16 + kk * (2048 >> 4), C::kIdescAcc,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit_warp(&empty1[st1]);
+          if constexpr (kKeys) mma_commit_warp(&empty2[st2]);
+          mma_commit_warp(&p_free[sb]);
+          if (i + 1 == steps) mma_commit_warp(acc_full);
+        }
+      }
+    }
+    mma_commit_warp(drain);
+    attn::drain_wait(drain, 0);
+    __syncwarp();
+  } else if (warp < C::kWarps) {
+    // ================= elementwise and epilogue =================
+    const int quad = warp & 3, wg = warp >> 2;
+    const int col0 = wg * C::kCols;
+    const int row = quad * 32 + lane;
+    const uint32_t tlane = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const float c = p.scale_log2;
+    const uint64_t c2 = f2_pack(c, c);
+    const uint32_t sd_bar = smem_u32(sd_ready), full2_bar = smem_u32(full2);
+    // Epilogue: this warpgroup's columns of dQ, or of dK or dV (`second`).
+    const bool second = kKeys && wg >= C::kAccGroups;
+    const View& out = second ? p.out2 : p.out1;
+    const float out_scale = second ? 1.0f : p.scale;
+    const int c0 = wg % C::kAccGroups * C::kAccCols;
+    const uint32_t tacc = tlane + (kKeys && !second ? C::kColAcc1 : C::kColAcc2) + c0;
+    int t = 0, sb = 0, li = 0;  // steps, t % kSBufs, items with steps
+    bool ok = true;
+    TileItem<kKeys> it{};
+    float nlse = 0.0f, ndelta = 0.0f;
+    auto open_item = [&](int k) {
+      it = tile_item<kKeys>(p, k);
+      if (!kKeys && it.r0 + row < p.Sq) {
+        const float* src =
+            p.stats + (static_cast<int64_t>(it.b) * p.Hq + it.h) * p.sq_pad + it.r0 + row;
+        nlse = __ldg(src);
+        ndelta = __ldg(src + p.stat_plane);
+      }
+    };
+    if (static_cast<int>(blockIdx.x) < p.n_items) open_item(static_cast<int>(blockIdx.x));
+    for (int k = static_cast<int>(blockIdx.x); k < p.n_items && ok; k += gridDim.x) {
+      const int my = it.r0 + row;  // this thread's key or query
+      // Steps whose pairs are all visible: those with str0 in [clear0, clear1],
+      // or (queries) below clear1 and within the sinks.
+      int clear0, clear1;
+      // The streamed positions [va, vb) that this row meets; queries also
+      // those below vs (sinks).
+      int va, vb, vs = 0;
+      // Live streamed rows: [0, se) and [lo, hi).  The others may hold anything.
+      int se, lo, hi;
+      if constexpr (kKeys) {
+        const bool sinks_only = it.r0 + kOwn <= p.sinks;
+        clear0 = it.r0 + kOwn - 1 - it.off;
+        clear1 = min(p.Sq - 64, sinks_only ? p.Sq : p.window - 64 + it.r0 - it.off);
+        va = my - it.off;
+        vb = min(p.Sq, my < p.sinks ? p.Sq : my + p.window - it.off);
+        se = 0;
+        lo = max(0, -it.off);
+        hi = 0x7fffffff;
+      } else {
+        const int first = it.off + it.r0, pos = it.off + my;
+        clear0 = first + kOwn - p.window;
+        clear1 = it.r0 + kOwn <= p.Sq ? first - 127 : -1;
+        va = pos - p.window + 1;
+        vb = pos + 1;
+        vs = min(p.sinks, pos + 1);
+        if (my >= p.Sq) va = vb = vs = 0;
+        se = it.se;
+        lo = it.lo;
+        hi = it.hi;
+      }
+      int head_i = kKeys && it.steps > 0 ? it.first % it.per_head : 0;  // step of a head
+      int str0 = str_row(it, head_i);
+      for (int i = 0; i < it.steps; ++i, ++t) {
+        const bool masked =
+            str0 > clear1 || (str0 < clear0 && (kKeys || str0 + 128 > p.sinks));
+        // S and dP; kKeys: the columns' statistics, which came with dO.
+        {
+          const uint32_t par = static_cast<uint32_t>(t) & 1u;
+          const uint32_t f_bar = kKeys ? full2_bar + 8u * (t % C::kStages2) : sd_bar;
+          const uint32_t f_par = kKeys ? static_cast<uint32_t>(t / C::kStages2) & 1u : par;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait3(sd_bar, par, f_bar, f_par, sd_bar, par, kSiteBwdS));
+        }
+        if (!ok) {
+          // Another warp of the quadrant may have seen the barrier: it must not
+          // wait for this one.  (It gets no further: dP stays taken.)
+          named_bar_arrive(kBarQuad + quad, 32 * C::kGroups);
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[C::kCols], d[C::kCols];
+        const uint32_t t_s = tlane + static_cast<uint32_t>(sb * C::kN);
+        if (++sb == C::kSBufs) sb = 0;
+        ld_cols(t_s + col0, s);
+        ld_cols(tlane + C::kColDp + col0, d);
+        tmem_wait_ld();
+        written_here(s);
+        written_here(d);
+        // The next step's dP may overwrite this one's, and, once the warps of
+        // this quadrant have all loaded S, P and dS may overwrite that.
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_warp(dp_free);
+        named_bar_sync(kBarQuad + quad, 32 * C::kGroups);
+        tc_fence_after();
+        uint32_t pk[C::kCols / 2], dk[C::kCols / 2];
+        const float* st_l = stat + t % C::kStages2 * 2 * C::kN + col0;
+        if (masked)
+          elementwise<kKeys, true>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, va - str0, vb - str0,
+                                   vs - str0, pk, dk);
+        else
+          elementwise<kKeys, false>(s, d, c2, st_l, C::kN, nlse, ndelta, col0, 0, 0, 0, pk, dk);
+        if constexpr (kKeys) st_cols(t_s + (col0 >> 1), pk);
+        st_cols(t_s + C::kDs + (col0 >> 1), dk);
+        // Streamed rows that nothing sees: zeroed before the accumulating
+        // products read them (0 * NaN is NaN).
+        if (str0 + C::kN > hi || (str0 < lo && str0 + C::kN > se)) {
+          const int st1 = t % C::kStages1, st2 = t % C::kStages2;
+          ok = attn::warp_wait(&full1[st1], static_cast<uint32_t>(t / C::kStages1) & 1u,
+                               kSiteBwdFull);
+          if (!ok) break;
+          for (int r = static_cast<int>(threadIdx.x); r < (kKeys ? 2 : 1) * C::kBoxes * C::kN;
+               r += 32 * C::kWarps) {
+            const int sr = str0 + r % C::kN;
+            if (sr >= hi || (sr < lo && sr >= se)) {
+              const int x = r / C::kN;  // boxes of the first tensor, then of the second
+              uint8_t* box = x < C::kBoxes
+                                 ? ring1 + st1 * C::kStrBytes + x * C::kStrBox
+                                 : ring2 + st2 * C::kStrBytes + (x - C::kBoxes) * C::kStrBox;
+              const uint32_t at = smem_u32(box) + static_cast<uint32_t>(r % C::kN) * 128u;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) st_shared_v4(at + e * 16, 0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_warp(&p_ready[t & 1]);
+        if constexpr (kKeys) {
+          str0 += 64;
+          if (++head_i == it.per_head) {
+            head_i = 0;
+            str0 = str_row(it, 0);
+          }
+        } else {
+          str0 = i + 1 == it.n_sink ? str_row(it, i + 1) : str0 + 128;
+        }
+      }
+      if (!ok) break;
+      const bool any = it.steps > 0;
+      const int b = it.b, h = it.h, r0 = it.r0, part = it.part;
+      // The next item's request length and statistics, under this one's end.
+      if (k + static_cast<int>(gridDim.x) < p.n_items) open_item(k + gridDim.x);
+      if (any) {
+        ok = attn::warp_wait(acc_full, static_cast<uint32_t>(li) & 1u, kSiteBwdAcc);
+        if (!ok) break;
+        ++li;
+        tc_fence_after();
+      }
+      float* sums = nullptr;  // a divided tile's row
+      if (kKeys && part >= 0)
+        sums = p.sink_sums + ((((static_cast<int64_t>(b) * p.Hkv + h) * p.sink_tiles + r0 / kOwn) *
+                                   p.sink_parts + part) * 2 + second) * (kOwn * D) + row * D + c0;
+      uint32_t w[C::kAccCols / 2];
+#pragma unroll
+      for (int cc = 0; cc < C::kAccCols; cc += 16) {
+        uint32_t v[16];
+        if (any) {
+          tmem_ld16(tacc + cc, v);
+          tmem_wait_ld();
+          written_here(v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = 0u;
+        }
+        if (kKeys && sums) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            reinterpret_cast<uint4*>(sums + cc)[e] =
+                make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[cc / 2 + e] = pack_bf16x2(__uint_as_float(v[2 * e]) * out_scale,
+                                      __uint_as_float(v[2 * e + 1]) * out_scale);
+      }
+      if (any) {
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_warp(acc_empty);
+      }
+      if (kKeys && sums) continue;
+      // A thread holds kAccCols columns of its row; kShare threads exchange
+      // 16-byte pieces so that together they store 64 bytes of a row at a time.
+      constexpr int kShare = C::kAccCols >= 32 ? 4 : 2;
+      const int rows = kKeys ? p.Skv : p.Sq;
+#pragma unroll
+      for (int cc = 0; cc < C::kAccCols / 2; cc += 4 * kShare) {
+        uint32_t(&x)[4 * kShare] = *reinterpret_cast<uint32_t(*)[4 * kShare]>(&w[cc]);
+        exchange<kShare>(x, lane);
+        // Now piece e of x is piece lane % kShare of row e of the kShare rows.
+#pragma unroll
+        for (int e = 0; e < kShare; ++e) {
+          const int r = r0 + quad * 32 + (lane & ~(kShare - 1)) + e;
+          if (r < rows)
+            *reinterpret_cast<uint4*>(out.row(b, h, r) + c0 + 2 * cc +
+                                      8 * (lane & (kShare - 1))) =
+                make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        }
+      }
+    }
   }
-  cp_async_wait<0>();
-  store_rows<D>(p.dq, b, hq, r0 + warp * 16, p.Sq, dq, p.scale);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::kWarps) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// dK and dV of the divided tiles: the parts' sums, in part order.  Four columns
+// to a thread.
+template <int D>
+__global__ void __launch_bounds__(256) sink_sum_kernel(const __grid_constant__ TileParams p) {
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int c = static_cast<int>(i % (D / 4)) * 4;
+  i /= D / 4;
+  const int row = static_cast<int>(i % kOwn);
+  i /= kOwn;
+  const int which = static_cast<int>(i % 2);
+  i /= 2;
+  const int tile = static_cast<int>(i % p.sink_tiles);
+  const int64_t bh = i / p.sink_tiles;
+  const int key = tile * kOwn + row;
+  if (bh >= static_cast<int64_t>(p.B) * p.Hkv || key >= p.Skv) return;
+  const float* src = p.sink_sums +
+                     (((bh * p.sink_tiles + tile) * p.sink_parts) * 2 + which) * (kOwn * D) +
+                     row * D + c;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int part = 0; part < p.sink_parts; ++part) {
+    const float4 x = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(part) * 2 * kOwn * D);
+    sum.x += x.x;
+    sum.y += x.y;
+    sum.z += x.z;
+    sum.w += x.w;
+  }
+  const float scale = which ? 1.0f : p.scale;
+  const View& out = which ? p.out2 : p.out1;
+  *reinterpret_cast<uint2*>(out.row(bh / p.Hkv, bh % p.Hkv, key) + c) =
+      make_uint2(pack_bf16x2(sum.x * scale, sum.y * scale), pack_bf16x2(sum.z * scale, sum.w * scale));
 }
 
 }  // namespace bwd

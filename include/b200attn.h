@@ -210,7 +210,8 @@ b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, con
  * sum over the query heads that share a key and are written whole (zeros for
  * keys that no query sees).  No atomics: equal calls give equal bits.
  */
-b200_status attention_window_bwd_workspace(int B, int Hq, int Sq, size_t* bytes);
+b200_status attention_window_bwd_workspace(int B, int Hq, int Hkv, int Sq, int Skv, int D,
+                                           int window, int sinks, size_t* bytes);
 b200_status attention_window_bwd(const b200_tensor* dout, const b200_tensor* q,
                                  const b200_tensor* k, const b200_tensor* v, const b200_tensor* o,
                                  const float* lse, const b200_tensor* dq, const b200_tensor* dk,

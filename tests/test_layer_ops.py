@@ -73,6 +73,20 @@ def test_window_bwd_refuses(bad, status, word):
     assert word in _lib.last_error()
 
 
+def test_window_bwd_workspace():
+    L, n = _lib.lib(), ctypes.c_size_t()
+
+    def need(Sq, W, sinks):
+        assert L.attention_window_bwd_workspace(1, 8, 2, Sq, Sq, 128, W, sinks,
+                                                ctypes.byref(n)) == 0
+        return n.value
+    # Two floats for each query, padded to 64; sums of the sinks' parts where they are divided.
+    assert need(100, 100, 0) == need(128, 128, 0) == 2 * 4 * 8 * 128
+    assert need(4096, 64, 4) > need(4096, 64, 0) == 2 * 4 * 8 * 4096
+    assert L.attention_window_bwd_workspace(1, 8, 2, 0, 1, 128, 1, 0, ctypes.byref(n)) == 1
+    assert L.attention_window_bwd_workspace(1, 8, 2, 1, 1, 128, 1, 0, None) == 1
+
+
 def rope(q=None, k=None, qo=None, ko=None, wq=256, wk=256, freq=256, R=128, pos=256, pos_sb=0,
          eps=1e-6, B=2, S=16, Hq=8, Hkv=2, D=128):
     t = [T() if x is None else x for x in (q, k, qo, ko)]

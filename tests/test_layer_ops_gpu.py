@@ -160,6 +160,9 @@ WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks, lens
     (1, 32, 8, 1024, 4096, 128, 2000, 1000, None),
     (16, 32, 8, 64, 700, 128, 300, 5, [700] * 8 + [65, 64, 63, 0, 1, 128, 300, 699]),
     (1, 8, 1, 2048, 2048, 128, 256, 130, None),
+    # sinks that many queries see (backward divides their tiles)
+    (1, 4, 2, 1500, 1500, 128, 64, 4, None),
+    (3, 4, 1, 1000, 1300, 64, 32, 140, [1300, 1000, 30]),
 ]
 
 
