@@ -200,10 +200,13 @@ b200_status window_shape(const char* who, int B, int Hq, int Hkv, int Sq, int Sk
 // go through a workspace and a second kernel, which pays from twice as many
 // on.  Measured (us, second kernel / cluster of 8): 32 splits, B 1, 8 kv heads,
 // 8192 keys: 12.7 / 17.6; 9 splits, B 4, 32768 keys: 87.8 / 81.7; 8 splits, B 4,
-// 8192 keys: 27.1 / 26.1.
+// 8192 keys: 27.1 / 26.1.  Units of few keys go one to a warp, without a merge
+// (us, CTA / warp; D 128): 160 units of 16 keys 4.8 / 3.9, of 64: 5.5 / 6.0; 600 of
+// 256: 20.2 / 18.9, of 512: 36.0 / 36.7; 4800 of 16: 58.9 / 16.3, of 128: 92 / 59.
 struct SplitPlan {
   int nsplit;
   bool cluster;
+  int units;  // not 0: this many units, one to a warp
 };
 
 SplitPlan split_plan(int64_t units, int64_t keys, bool partial) {
@@ -212,8 +215,11 @@ SplitPlan split_plan(int64_t units, int64_t keys, bool partial) {
   const int64_t most = keys / (2 * sp::kWarps * sp::kKeys);
   const int n =
       static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, sp::kMaxSplits})));
-  if (partial || n >= 2 * sp::kMaxCluster) return SplitPlan{n, false};
-  return SplitPlan{std::min(n, sp::kMaxCluster), true};
+  if (partial || n >= 2 * sp::kMaxCluster) return SplitPlan{n, false, 0};
+  const bool many = units >= 4 * static_cast<int64_t>(sm_count());
+  if (n == 1 && units < (1 << 30) && keys <= (many ? 256 : 2 * sp::kKeys))
+    return SplitPlan{1, true, static_cast<int>(units)};
+  return SplitPlan{std::min(n, sp::kMaxCluster), true, 0};
 }
 
 int row_tiles_of(int64_t rows) {
@@ -253,6 +259,7 @@ struct WindowPlan {
   bool tiles;   // 128-row tiles (tcgen05); else 16-row tiles that split the keys
   int nsplit;
   size_t bytes;  // of the splits' partial sums; 0: a cluster merges them
+  int units;     // as SplitPlan
 };
 
 size_t split_bytes(int64_t rows, const SplitPlan& p, int D) {
@@ -260,12 +267,12 @@ size_t split_bytes(int64_t rows, const SplitPlan& p, int D) {
 }
 
 WindowPlan window_plan(const WindowShape& s) {
-  if (window_by_tiles(s)) return WindowPlan{true, 1, 0};
+  if (window_by_tiles(s)) return WindowPlan{true, 1, 0, 0};
   const int64_t rows = static_cast<int64_t>(s.Hq / s.Hkv) * s.Sq;
   const int64_t heads = static_cast<int64_t>(s.B) * s.Hkv;
   const int64_t keys = std::min<int64_t>(s.Skv, static_cast<int64_t>(s.window) + s.sinks);
   const SplitPlan p = split_plan(heads * row_tiles_of(rows), keys, false);
-  return WindowPlan{false, p.nsplit, split_bytes(heads * rows, p, s.D)};
+  return WindowPlan{false, p.nsplit, split_bytes(heads * rows, p, s.D), p.units};
 }
 
 template <int D>
@@ -275,7 +282,9 @@ b200_status launch_split(const b200::split::Params& p, cudaStream_t stream) {
   auto kernel = b200::split::split_attention_kernel<D>;
   const b200_status st = ensure_smem_attr(kernel, C::kSmemBytes, &attr_done);
   if (st != B200_OK) return st;
-  const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * p.row_tiles * p.nsplit;
+  const int64_t grid =
+      p.units ? (p.units + b200::split::kWarps - 1) / b200::split::kWarps
+              : static_cast<int64_t>(p.B) * p.Hkv * p.row_tiles * p.nsplit;
   if (grid > 0x7fffffffll) return fail(B200_EUNSUPPORTED, "attention: too many work units");
   cudaLaunchAttribute attr[1];
   if (p.overlaps) {
@@ -309,8 +318,9 @@ b200_status launch_combine(const b200::split::CombineParams& p, int D, cudaStrea
 
 b200::split::Params split_params(const WindowShape& s, const b200_tensor* q, const b200_tensor* k,
                                  const b200_tensor* v, const b200_tensor* o,
-                                 const int32_t* kv_len, int nsplit) {
+                                 const int32_t* kv_len, int nsplit, int units) {
   b200::split::Params p{};
+  p.units = units;
   p.q = view_of(q);
   p.k = view_of(k);
   p.v = view_of(v);
@@ -502,7 +512,7 @@ b200_status launch_bwd_tiles(const CUtensorMap (&m)[4], b200::bwd::TileParams p,
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = kKeys ? 1 : 0;  // the keys' launch follows the row statistics'
+  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], p);
   return e == cudaSuccess ? B200_OK : cuda_fail(e, "attention_window_bwd launch");
 }
@@ -557,15 +567,17 @@ b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* w
   p.s1_b = q_b, p.s1_h = q_h, p.s2_b = do_b, p.s2_h = do_h;
   if ((st = launch_bwd_tiles<D, true>({k, v, q[1], dout[1]}, p, s.Hkv, s.Skv, stream)) != B200_OK)
     return st;
-  if (sink.parts > 0) {
-    const int64_t sums = static_cast<int64_t>(s.B) * s.Hkv * sink.tiles * 2 * b200::bwd::kOwn * D / 4;
-    b200::bwd::sink_sum_kernel<D><<<static_cast<unsigned>((sums + 255) / 256), 256, 0, stream>>>(p);
-    if ((st = check_launch("attention_window_bwd sinks")) != B200_OK) return st;
-  }
   p.out1 = p.out2 = view_of(t.dq);
   p.o1_b = q_b, p.o1_h = q_h, p.o2_b = do_b, p.o2_h = do_h;
   p.s1_b = k_b, p.s1_h = k_h, p.s2_b = v_b, p.s2_h = v_h;
-  return launch_bwd_tiles<D, false>({q[0], dout[0], k, v}, p, s.Hq, s.Sq, stream);
+  if ((st = launch_bwd_tiles<D, false>({q[0], dout[0], k, v}, p, s.Hq, s.Sq, stream)) != B200_OK)
+    return st;
+  if (sink.parts == 0) return B200_OK;
+  p.out1 = view_of(t.dk);
+  p.out2 = view_of(t.dv);
+  const int64_t sums = static_cast<int64_t>(s.B) * s.Hkv * sink.tiles * 2 * b200::bwd::kOwn * D / 4;
+  b200::bwd::sink_sum_kernel<D><<<static_cast<unsigned>((sums + 255) / 256), 256, 0, stream>>>(p);
+  return check_launch("attention_window_bwd sinks");
 }
 
 // Tiles of the prefix form: whole batches, up to 128 rows.
@@ -621,6 +633,7 @@ struct PrefixPlan {
   int prefix_splits;  // tiles: of the prefix
   int prefix_sms;     // tiles: SMs that they take
   int own_splits;     // of the requests' keys (not tiles: after the prefix)
+  int own_units;      // as SplitPlan
   size_t prefix_bytes, own_bytes;
 };
 
@@ -672,6 +685,7 @@ PrefixPlan prefix_plan(const WindowShape& own, int P, const b200_tensor* q) {
   } else {
     const SplitPlan o = split_plan(units, static_cast<int64_t>(P) + own.Skv, false);
     p.own_splits = o.nsplit;
+    p.own_units = o.units;
     p.own_bytes = split_bytes(heads * rows, o, own.D);
     p.prefix_bytes = 0;
   }
@@ -801,7 +815,7 @@ b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, con
   if (plan.tiles)
     return D == 128 ? launch_window_tiles<128>(s, q, k, v, o, lse, kv_len, cs)
                     : launch_window_tiles<64>(s, q, k, v, o, lse, kv_len, cs);
-  b200::split::Params p = split_params(s, q, k, v, o, kv_len, plan.nsplit);
+  b200::split::Params p = split_params(s, q, k, v, o, kv_len, plan.nsplit, plan.units);
   p.lse = lse;
   const int64_t rows = static_cast<int64_t>(B) * Hkv * plan.nsplit * p.rows;
   if (plan.bytes > 0) part_pointers(workspace, rows, D, &p.part_o, &p.part_ml);
@@ -893,7 +907,7 @@ b200_status attention_shared_prefix(const b200_tensor* q, const b200_tensor* k_p
                             plan.prefix_bytes + plan.own_bytes)) != B200_OK)
     return st;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  b200::split::Params p = split_params(own, q, k, v, o, kv_len, plan.own_splits);
+  b200::split::Params p = split_params(own, q, k, v, o, kv_len, plan.own_splits, plan.own_units);
   b200::split::CombineParams c{};
   c.B = B;
   c.Hkv = Hkv;

@@ -60,6 +60,9 @@ struct Params {
   int row_tiles;  // ceil(rows / 16)
   int nsplit;
   int window, sinks;  // at most Skv
+  // Many short units: each warp takes one whole (nsplit is 1), `units` in all.
+  // 0: a CTA takes a unit.
+  int units;
   float scale_log2;
   float* part_o;    // [B * Hkv][nsplit][rows][D], or null: the nsplit CTAs are a cluster
   float2* part_ml;  // [B * Hkv][nsplit][rows] (m in log2 units, l)
@@ -89,7 +92,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   pdl_launch_dependents();
   const int lane = static_cast<int>(lane_id());
   const int warp = static_cast<int>(warp_id());
+  const int stride = p.units ? 1 : kWarps;      // of a warp's blocks
+  const int first = p.units ? 0 : warp;
   int unit = static_cast<int>(blockIdx.x);
+  if (p.units) {
+    unit = unit * kWarps + warp;
+    if (unit >= p.units) return;
+  }
   const int split = unit % p.nsplit;
   unit /= p.nsplit;
   const int rt = unit % p.row_tiles;
@@ -150,9 +159,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     cp_async_commit();
   };
-  int next = b0 + warp;
+  int next = b0 + first;
 #pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s, next += kWarps) load_block(next, s);
+  for (int s = 0; s < C::kStages - 1; ++s, next += stride) load_block(next, s);
 
   // Q as the A operand: lane holds rows lane/4 and lane/4 + 8, columns
   // 2 (lane % 4) + {0, 1, 8, 9} of every 16.
@@ -183,12 +192,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int vrow = (((lane >> 3) & 1) << 3) + (lane & 7), vpar = lane >> 4;
 
   int stage = 0;
-  for (int i = b0 + warp; i < b1; i += kWarps) {
+  for (int i = b0 + first; i < b1; i += stride) {
     cp_async_wait<C::kStages - 2>();
     __syncwarp();
     // The stage consumed in the previous step takes the next block.
     load_block(next, stage == 0 ? C::kStages - 1 : stage - 1);
-    next += kWarps;
+    next += stride;
     const uint32_t kt = ring + stage * C::kStageBytes;
     const uint32_t vt = kt + C::kTileBytes;
     stage = stage + 1 == C::kStages ? 0 : stage + 1;
@@ -270,6 +279,26 @@ __global__ void __launch_bounds__(kThreads, 2)
   l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
   l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
   l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
+
+  if (p.units) {
+    // The warp's own rows.
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = half ? rb : ra;
+      if (r >= p.rows) continue;
+      const float m = half ? m_b : m_a, l = half ? l_b : l_a;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int head = h * p.group + r % p.group, tok = r / p.group;
+      if (p.lse && (lane & 3) == 0)
+        p.lse[(static_cast<int64_t>(b) * p.Hkv * p.group + head) * p.Sq + tok] = row_lse(m, l);
+      uint16_t* dst = p.o.row(b, head, tok) + ca;
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d)
+        *reinterpret_cast<uint32_t*>(dst + 8 * d) =
+            pack_bf16x2(o[d][2 * half] * inv, o[d][2 * half + 1] * inv);
+    }
+    return;
+  }
 
   // Merge the warps through shared memory (the rings are free by then).
   cp_async_wait<0>();

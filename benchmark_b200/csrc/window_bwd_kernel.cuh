@@ -356,7 +356,12 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot;
-  pdl_wait();  // the row statistics
+  if constexpr (kKeys) {
+    // The row statistics; then the queries' kernel may start where this one's
+    // last CTAs leave SMs free (they are complete for it too).
+    pdl_wait();
+    pdl_launch_dependents();
+  }
 
   // First streamed row of a query head's step i.
   auto str_row = [&](const TileItem<kKeys>& it, int i) {
@@ -737,6 +742,8 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  // The queries' grid ends after the keys', so that what follows it follows both.
+  if (!kKeys && blockIdx.x + 1 == gridDim.x) pdl_wait();
 }
 
 // dK and dV of the divided tiles: the parts' sums, in part order.  Four columns

@@ -160,6 +160,10 @@ WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks, lens
     (1, 32, 8, 1024, 4096, 128, 2000, 1000, None),
     (16, 32, 8, 64, 700, 128, 300, 5, [700] * 8 + [65, 64, 63, 0, 1, 128, 300, 699]),
     (1, 8, 1, 2048, 2048, 128, 256, 130, None),
+    # many short units: one to a warp
+    (40, 32, 16, 3, 200, 64, 150, 4, [(37 * i) % 201 for i in range(40)]),
+    (75, 16, 8, 1, 90, 128, 1 << 40, 0, [(17 * i) % 91 for i in range(75)]),
+    (3, 6, 3, 20, 30, 128, 9, 2, [30, 20, 0]),
     # sinks that many queries see (backward divides their tiles)
     (1, 4, 2, 1500, 1500, 128, 64, 4, None),
     (3, 4, 1, 1000, 1300, 64, 32, 140, [1300, 1000, 30]),
@@ -312,6 +316,7 @@ PREFIX = [  # B, Hq, Hkv, Sq, P, S, D, lens
     (70, 8, 2, 1, 3001, 5, 128, None),
     (2, 48, 16, 2, 127, 9, 64, [9, 2]),
     (40, 16, 16, 1, 5003, 20, 64, None),
+    (70, 36, 12, 7, 33, 20, 128, None),
     (25, 40, 8, 3, 3000, 30, 128, None),
     (3, 64, 1, 2, 9000, 10, 128, None),
     (2, 192, 2, 2, 9000, 10, 128, [1, 10]),  # more rows of a request than a tile has
