@@ -508,7 +508,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- setup ----
   if constexpr (kForm == kPrefix) {
-    pdl_launch_dependents();  // the requests' own keys, on the SMs left over
     // Rows past a tile's box stay zero (their scores are computed, and dropped).
     for (int i = static_cast<int>(threadIdx.x); i < 2 * C::kTileBytes / 16; i += kThreads)
       reinterpret_cast<uint4*>(q_buf)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -568,6 +567,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (kForm != kDense) {
+    pdl_wait();  // nothing was read before this
+    // Only now: what follows kPrefix (the requests' own keys, on the SMs left
+    // over) does not wait for this grid, and reads what this one waited for.
+    pdl_launch_dependents();
+  }
   const bool trace_cta = kTrace && static_cast<int>(blockIdx.x) == p.trace_cta;
   // Each warpgroup moves its register budget first, inside its own branch,
   // so the compiler sizes each role's code to that role's budget.

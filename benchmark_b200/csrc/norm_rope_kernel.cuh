@@ -244,6 +244,8 @@ __device__ __forceinline__ void store_chunks(uint16_t* row, const Lane& x,
 template <int D, bool kInterleaved, bool kPerRow>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) norm_rope_kernel(const __grid_constant__ Params p) {
   using Sh = Shape<D, kPerRow>;
+  pdl_wait();
+  pdl_launch_dependents();
   const Lane x = lane_of<Sh::kLanes>(p.rot);
   const uint32_t item = blockIdx.x * kWarps + warp_id();
   const uint32_t tg = p.slices == 1 ? item : item / static_cast<uint32_t>(p.slices);
@@ -303,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, kGradCtasPerSm)
     norm_rope_bwd_kernel(const __grid_constant__ Params p) {
   using Sh = Shape<D, kPerRow>;
   __shared__ float dw_sh[kWarps][D];
+  pdl_wait();
   pdl_launch_dependents();
   const Lane x = lane_of<Sh::kLanes>(p.rot);
   const bool is_q = static_cast<int>(blockIdx.x) < p.ctas_q;

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     split_attention_kernel(const __grid_constant__ Params p) {
   using C = Cfg<D>;
   extern __shared__ __align__(128) uint8_t smem[];
+  if (!p.overlaps) pdl_wait();
   pdl_launch_dependents();
   const int lane = static_cast<int>(lane_id());
   const int warp = static_cast<int>(warp_id());
