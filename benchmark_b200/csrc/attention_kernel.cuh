@@ -211,8 +211,8 @@ struct Cfg {
   static constexpr int kFlagOff = kLOff + 128 * 8;  // abort flag and merge flag (epilogue)
   static constexpr int kBarOff = kFlagOff + 16;
   // q_full[2] q_empty[2] k_full[K] k_empty[K] v_full[V] v_empty[V]
-  // s_ready[3] p_ready[3] p_free[3] pv_done o_full o_empty l_ready[2] drain done o_free
-  static constexpr int kNumBars = 4 + 2 * kKStages + 2 * kVStages + 3 * kSBufs + 1 + 4 + 3;
+  // s_ready[3] p_ready[3] p_free[3] pv_done[2] o_full o_empty l_ready[2] drain done o_free
+  static constexpr int kNumBars = 4 + 2 * kKStages + 2 * kVStages + 3 * kSBufs + 2 + 4 + 3;
   static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kTmemSlotOff + 16 + 1024;  // + 1 KiB alignment slack
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
@@ -466,8 +466,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_ready = v_empty + C::kVStages;
   uint64_t* p_ready = s_ready + kSBufs;
   uint64_t* p_free = p_ready + kSBufs;  // PV(t) done: S buffer t % kSBufs reusable
+  // PV(t) done, by the parity of t: a softmax warp at tile t may run ahead of
+  // PV(t - 2), so one barrier's parity could not tell PV(t - 1) from PV(t - 3).
   uint64_t* pv_done = p_free + kSBufs;
-  uint64_t* o_full = pv_done + 1;
+  uint64_t* o_full = pv_done + 2;
   uint64_t* o_empty = o_full + 1;
   uint64_t* l_ready = o_empty + 1;
   uint64_t* drain = l_ready + 2;
@@ -535,7 +537,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
-    mbar_init(pv_done, 1);
+    mbar_init(&pv_done[0], 1);
+    mbar_init(&pv_done[1], 1);
     mbar_init(drain, 2);  // one commit from each MMA issuer
     mbar_init(done, 1);
     mbar_arrive(done);
@@ -841,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               commit_both(&v_empty[t % C::kVStages]);
               commit_lead(&p_free[sb]);
-              commit_both(pv_done);
+              commit_both(&pv_done[t & 1]);
             }
             if (!ok) break;
             commit_both(o_full);
@@ -953,7 +956,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Rescale the O rows whose maximum jumped, once PV(tt-1) has
         // completed (PV(tt) waits for this tile's P barrier); rare.
         auto rescale_o = [&]() {
-          if (!warp_wait(pv_done, static_cast<uint32_t>(tt - 1) & 1u, kSitePvDone)) {
+          if (!warp_wait(&pv_done[(tt - 1) & 1], static_cast<uint32_t>((tt - 1) >> 1) & 1u,
+                         kSitePvDone)) {
             ok = false;
             return;
           }
