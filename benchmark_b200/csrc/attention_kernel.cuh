@@ -1156,7 +1156,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           // two threads to a row, before this warp's P is published.
           if (ok && (kbase + kBN > it.hi || (kbase < it.lo && kbase + kBN > it.se))) {
             const int vs = tt % C::kVStages;
-            ok = warp_wait(&v_full[vs], static_cast<uint32_t>(tt / C::kVStages) & 1u, kSiteVFull);
+            // With fewer V stages than S buffers the stage may still hold
+            // V(tt - kVStages), and its barrier's parity could not tell.
+            if (C::kVStages < kSBufs && tt >= C::kVStages)
+              ok = warp_wait(&pv_done[(tt - C::kVStages) & 1],
+                             static_cast<uint32_t>((tt - C::kVStages) >> 1) & 1u, kSitePvDone);
+            ok = ok && warp_wait(&v_full[vs], static_cast<uint32_t>(tt / C::kVStages) & 1u,
+                                 kSiteVFull);
             const int row = static_cast<int>(threadIdx.x >> 1), key = kbase + row;
             if (ok && (key >= it.hi || (key < it.lo && key >= it.se))) {
               const uint32_t at = smem_u32(v_buf + vs * C::kVTileBytes) +

@@ -49,3 +49,13 @@ def test_rescales_wait_for_the_previous_product(B, H, S, D, causal):
     k, v = inputs(30, B, H, S, D)
     want, bound = form(k, v, 1, S if causal else None)
     check(lambda: ops.attention_fwd(k, k, v, causal=causal), want, bound)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_zeroed_values_wait_for_the_products_before(D):
+    """Rows of V that no query of a tile may see are zeroed in the tile's stage, once the
+    products that read the stage before have completed."""
+    B, H, S, window, sinks = 32, 4, 1100, 200, 3
+    k, v = inputs(31, B, H, S, D)
+    want, bound = form(k, v, 1, window, sinks)
+    check(lambda: ops.attention_window_fwd(k, k, v, window, sinks), want, bound)
