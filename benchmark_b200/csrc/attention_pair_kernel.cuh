@@ -60,9 +60,9 @@ constexpr int kLOff = kVOff + kVStages * kTileBytes;  // (m, l) [pipe][128]
 constexpr int kFlagOff = kLOff + 2 * 128 * 8;          // abort flag (epilogue)
 constexpr int kBarOff = kFlagOff + 16;
 // q_full[2][2] q_empty[2][2] k_full[K] k_empty[K] v_full[V] v_empty[V]
-// s_ready[3] p_ready[3] p_free[3] pv_done[2] o_full[2] o_empty[2] l_ready[2]
+// s_ready[2][3] p_ready[3] p_free[3] o_full[2] o_empty[2] l_ready[2]
 // drain done
-constexpr int kNumBars = 8 + 2 * kKStages + 2 * kVStages + 3 * kSBufs + 8 + 2;
+constexpr int kNumBars = 8 + 2 * kKStages + 2 * kVStages + 4 * kSBufs + 6 + 2;
 constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
 constexpr int kSmemBytes = kTmemSlotOff + 16 + 1024;  // + 1 KiB alignment slack
 static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
@@ -171,10 +171,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_full = k_empty + kKStages;
   uint64_t* v_empty = v_full + kVStages;
   uint64_t* s_ready = v_empty + kVStages;
-  uint64_t* p_ready = s_ready + kSBufs;
+  // [pipe][its tile % kSBufs]: a pipe sees every phase of its own (the B pipe
+  // sits out a unit with one Q tile, and a barrier shared with the A pipe could
+  // be any number of phases behind or ahead when it comes back).
+  uint64_t* p_ready = s_ready + 2 * kSBufs;
   uint64_t* p_free = p_ready + kSBufs;
-  uint64_t* pv_done = p_free + kSBufs;  // [pipe]
-  uint64_t* o_full = pv_done + 2;       // [pipe]
+  uint64_t* o_full = p_free + kSBufs;   // [pipe]
   uint64_t* o_empty = o_full + 2;       // [pipe]
   uint64_t* l_ready = o_empty + 2;      // [pipe]
   uint64_t* drain = l_ready + 2;
@@ -202,11 +204,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kSBufs; ++i) {
       mbar_init(&s_ready[i], 1);
+      mbar_init(&s_ready[kSBufs + i], 1);
       mbar_init(&p_ready[i], 4);  // the pipe's four softmax warps
       mbar_init(&p_free[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_empty[i], 4);  // the four epilogue warps
       mbar_init(&l_ready[i], 4);  // the pipe's four softmax warps
@@ -327,6 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       int u = 0, t = 0, lq[2] = {0, 0};
+      int ts_pipe[2] = {0, 0};  // S tiles issued for each pipe
       bool ok = true;
       for (int r = 0; r < rounds && ok; ++r) {
         const int k = unit_index(r);
@@ -352,7 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int kk = 0; kk < D / 16; ++kk)
                 mma_ss_warp(ts, dq + kk * 2, dk + kk * 2, kIdescS, kk > 0 ? 1u : 0u);
-              mma_commit_warp(&s_ready[sb]);
+              mma_commit_warp(&s_ready[pp * kSBufs + ts_pipe[pp] % kSBufs]);
+              ++ts_pipe[pp];
             }
             if (ok) mma_commit_warp(&k_empty[ks]);
           }
@@ -377,7 +381,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mma_ts_warp(to, tp + kk * 8, dv + kk * (2048 >> 4), kIdescO,
                             (j > 0 || kk > 0) ? 1u : 0u);
               mma_commit_warp(&p_free[sb]);
-              mma_commit_warp(&pv_done[pp]);
             }
             if (ok) mma_commit_warp(&v_empty[vs]);
           }
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tO = tmem_base + lane_addr + kColO + static_cast<uint32_t>(pp * D);
     const float c = p.scale_log2;
     Tracer<kTrace> tr(p, 2 + pp, trace_cta && quad == 0 && lane == 0);
-    int u = 0, tp = 0, lq = 0;
+    int u = 0, tp = 0, lq = 0;  // S tiles of the CTA, tiles of this pipe, its units
     bool ok = true;
 #pragma unroll 1
     for (int r = 0; r < rounds && ok; ++r) {
@@ -421,7 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int sb = uu % kSBufs;
         const uint32_t tS = tmem_base + lane_addr + static_cast<uint32_t>(sb * 128);
         tr(kEvSmWait, pp, uu);
-        ok = warp_wait(&s_ready[sb], static_cast<uint32_t>(uu / kSBufs) & 1u, kSiteSReady);
+        ok = warp_wait(&s_ready[pp * kSBufs + tp % kSBufs], static_cast<uint32_t>(tp / kSBufs) & 1u,
+                       kSiteSReady);
         if (!ok) break;
         tc_fence_after();
         tr(kEvSmReady, pp, uu);
@@ -497,9 +501,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tr(kEvSmPComputed, pp, uu);
         // O holds this pipe's tiles before j in the old max: rescale it once
-        // PV(j-1) has completed (rare; the tile's PV waits for this P).
+        // PV(j-1) has completed (rare; the tile's PV waits for this P).  Its
+        // S buffer's barrier says so: PV(j-2) may not have completed yet, so
+        // one barrier for all of the pipe's tiles could not by its parity.
         if (resc && j > 0) {
-          ok = warp_wait(&pv_done[pp], static_cast<uint32_t>(tp - 1) & 1u, kSitePvDone);
+          const int prev = uu - un.nq;  // the pipe's tile j - 1 in the S sequence
+          ok = warp_wait(&p_free[prev % kSBufs], static_cast<uint32_t>(prev / kSBufs) & 1u,
+                         kSitePvDone);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1

@@ -59,3 +59,13 @@ def test_zeroed_values_wait_for_the_products_before(D):
     k, v = inputs(31, B, H, S, D)
     want, bound = form(k, v, 1, window, sinks)
     check(lambda: ops.attention_window_fwd(k, k, v, window, sinks), want, bound)
+
+
+@pytest.mark.parametrize("B,H,S", [(64, 2, 600), (64, 2, 640), (64, 2, 768), (200, 1, 130),
+                                   (300, 2, 128), (64, 4, 384)])
+def test_pairs_of_query_tiles_with_one_left_over(B, H, S):
+    """head_dim 64, not causal: with an odd number of query tiles one of the two softmax
+    pipes sits out every unit that has only one."""
+    k, v = inputs(32, B, H, S, 64)
+    want, bound = form(k, v, B)
+    check(lambda: ops.attention_fwd(k, k, v), want, bound)
