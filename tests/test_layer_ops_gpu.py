@@ -493,3 +493,49 @@ def test_python_refusals():
         ops.qk_norm_rope(q, k, w, w.bfloat16(), f, i32([0] * 8))
     with pytest.raises(ValueError, match="v_prefix"):
         ops.attention_shared_prefix(q, k[0], k[0, :, :5], k, k)
+
+
+def test_calls_follow_what_was_queued_before_them():
+    """Each call reads what the stream's earlier work writes, however early its kernels
+    start: inputs filled just before, outputs overwritten just after."""
+    g = gen(30)
+    B, Hq, Hkv, P, S, D = 64, 16, 2, 6000, 600, 128
+    q0, k0, v0 = randn(g, B, Hq, 1, D), randn(g, B, Hkv, S, D), randn(g, B, Hkv, S, D)
+    kp0, vp0 = randn(g, Hkv, P, D), randn(g, Hkv, P, D)
+    w, f, pos = torch.ones(D, device="cuda"), torch.rand(64, device="cuda"), i32([5])
+    bufs = [torch.zeros_like(t) for t in (q0, k0, v0, kp0, vp0)]
+    q, k, v, kp, vp = bufs
+
+    def fill():
+        for t, s in zip(bufs, (q0, k0, v0, kp0, vp0)):
+            t.copy_(s)
+
+    def wipe():
+        for t in bufs:
+            t.fill_(NAN)
+
+    calls = {
+        "prefix": lambda: ops.attention_shared_prefix(q, kp, vp, k, v),
+        "decode": lambda: ops.attention_window_fwd(q, k, v, 500, 4),
+        "tiles": lambda: ops.attention_window_fwd(k, k, v, 300, 4),
+        "rope": lambda: ops.qk_norm_rope(q, q, w, w, f, pos)[0],
+    }
+    fill()
+    want = {n: c() for n, c in calls.items()}
+    qr, _ = ops.qk_norm_rope(q, q, w, w, f, pos)
+    chained = ops.attention_shared_prefix(qr, kp, vp, k, v)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for n, c in calls.items():
+            fill()
+            got = c()
+            wipe()
+            assert torch.equal(got, want[n]), n
+        fill()  # the kernels of one call behind those of another
+        qr.fill_(NAN)
+        ops.qk_norm_rope(q, q, w, w, f, pos, q_out=qr, k_out=torch.empty_like(q))
+        got = ops.attention_shared_prefix(qr, kp, vp, k, v)
+        qr.fill_(NAN)
+        wipe()
+        assert torch.equal(got, chained)
+    ops.check()
