@@ -370,7 +370,9 @@ __global__ void __launch_bounds__(kThreads, kGradCtasPerSm)
         nx = load_chunks(then.in, x, then.live && row < H);
         ng = load_chunks(then.gin, x, then.live && row < H);
       }
-      const float rn = row_norm<D>(v, p.eps);
+      const bool live = now.live && h < H;
+      // (Without eps the zeros of a row that is not there would give NaN.)
+      const float norm = row_norm<D>(v, p.eps), rn = live ? norm : 0.0f;
       const uint64_t rn2 = f2_pack(rn, rn);
       rotate16<kInterleaved, true>(g, turn);
       uint64_t dot2 = 0ull;
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, kGradCtasPerSm)
       const uint64_t d2 = f2_pack(dot, dot);
 #pragma unroll
       for (int i = 0; i < 8; ++i) g[i] = f2_mul(rn2, f2_fma(v[i], d2, g[i]));
-      if (now.live && h < H) store_chunks(now.out, x, g);
+      if (live) store_chunks(now.out, x, g);
       now.out += out_step;
     }
     now = then;

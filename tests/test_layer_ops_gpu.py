@@ -116,6 +116,22 @@ def test_norm_rope_zero_and_tiny_rows():
     U.check_close(qo, *U.norm_rope(q, wq, angles, 1e-6, False), "q")
 
 
+@pytest.mark.parametrize("Hq,Hkv,S", [(3, 1, 5), (5, 9, 130), (1, 1, 7)])
+def test_norm_rope_without_eps(Hq, Hkv, S):
+    """eps 0, with heads or tokens that do not fill a warp: its other rows add nothing."""
+    q, k, wq, wk, freq, pos = rope_inputs(1, S, Hq, Hkv, 128, 64, True, seed=7)
+    g = gen(8)
+    gq, gk = randn(g, 1, Hq, S, 128), randn(g, 1, Hkv, S, 128)
+    angles = U.rope_angles(pos, freq, 1)
+    got = ops.qk_norm_rope_bwd(gq, gk, q, k, wq, wk, freq, pos, eps=0.0)
+    y = ops.qk_norm_rope(q, k, wq, wk, freq, pos, eps=0.0)
+    for i, (x, w, gy) in enumerate(((q, wq, gq), (k, wk, gk))):
+        U.check_close(y[i], *U.norm_rope(x, w, angles, 0.0, False), "y")
+        ref = U.norm_rope_bwd(gy, x, w, angles, 0.0, False)
+        U.check_close(got[i], *ref[:2], "dx")
+        U.check_close(got[2 + i], *ref[2:], "dw")
+
+
 def test_norm_rope_gradient_is_the_difference_of_its_plain_form():
     q, k, wq, wk, freq, pos = rope_inputs(2, 9, 3, 2, 64, 32, True, seed=5)
     g = gen(6)
