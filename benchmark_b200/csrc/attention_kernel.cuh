@@ -277,7 +277,7 @@ __device__ __forceinline__ FormItem decode_window_item(const Params& p, int k) {
   it.hq = bh - it.b * p.Hq;
   it.hkv = it.hq / p.group;
   it.row0 = qt * kBM;
-  it.kv_len = p.kv_len ? max(0, min(__ldg(p.kv_len + it.b), p.Skv)) : p.Skv;
+  it.kv_len = p.kv_len ? max(0, min(ld_global(p.kv_len + it.b), p.Skv)) : p.Skv;
   it.off = it.kv_len - p.Sq;
   const int last = it.off + min(it.row0 + kBM, p.Sq) - 1;  // the last row's position
   it.hi = max(0, last + 1);
@@ -843,8 +843,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                               (j > 0 || kk > 0) ? 1u : 0u);
               }
               commit_both(&v_empty[t % C::kVStages]);
-              commit_lead(&p_free[sb]);
+              // Before p_free: a softmax warp that sees S(t + 3), which that one
+              // admits, relies on this phase having passed.
               commit_both(&pv_done[t & 1]);
+              commit_lead(&p_free[sb]);
             }
             if (!ok) break;
             commit_both(o_full);

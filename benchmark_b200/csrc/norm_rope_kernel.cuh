@@ -16,7 +16,7 @@
 // keep their angles and weights in registers; it has the next rows in flight
 // while it works on its own, and nothing synchronises the warps.  (A first
 // form kept both in shared memory for a block of tokens: its reads kept the
-// load/store unit 80 % busy, 77 us against KFWD for 16384 tokens of 32 + 8
+// load/store unit 80 % busy, 77 us against 63 for 16384 tokens of 32 + 8
 // heads of 128.)  With few heads a warp's lanes would stay empty: then each
 // of its rows walks a token of its own (kPerRow).
 #pragma once
@@ -105,14 +105,15 @@ __device__ __forceinline__ void load_weights(const void* w, int w_f32, const Lan
   for (int h = 0; h < 2; ++h) {
     const int c = h ? x.c1 : x.c0;
     if (w_f32) {
-      const float4* src = static_cast<const float4*>(w) + 2 * c;
-      const float4 a = __ldg(src), b = __ldg(src + 1);
-      out[4 * h] = f2_pack(a.x, a.y);
-      out[4 * h + 1] = f2_pack(a.z, a.w);
-      out[4 * h + 2] = f2_pack(b.x, b.y);
-      out[4 * h + 3] = f2_pack(b.z, b.w);
+      const uint4* src = static_cast<const uint4*>(w) + 2 * c;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 a = ld_global(src + e);
+        out[4 * h + 2 * e] = f2_pack(__uint_as_float(a.x), __uint_as_float(a.y));
+        out[4 * h + 2 * e + 1] = f2_pack(__uint_as_float(a.z), __uint_as_float(a.w));
+      }
     } else {
-      unpack8(__ldg(static_cast<const uint4*>(w) + c), out + 4 * h);
+      unpack8(ld_global(static_cast<const uint4*>(w) + c), out + 4 * h);
     }
   }
 }
@@ -147,7 +148,7 @@ __device__ __forceinline__ Angles lane_angles(const float* inv_freq, int pos, co
     oc[i] = 1.0f;
     os[i] = 0.0f;
     if (x.rotated)
-      angle(pos, __ldg(inv_freq + pair((kPerRow ? 0 : x.row * kOwn) + i)), &oc[i], &os[i]);
+      angle(pos, ld_global(inv_freq + pair((kPerRow ? 0 : x.row * kOwn) + i)), &oc[i], &os[i]);
   }
   Angles a;
 #pragma unroll
@@ -228,8 +229,8 @@ struct Chunks {
 __device__ __forceinline__ Chunks load_chunks(const uint16_t* row, const Lane& x, bool live) {
   Chunks r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
   if (live) {
-    r.a = __ldcs(reinterpret_cast<const uint4*>(row) + x.c0);
-    r.b = __ldcs(reinterpret_cast<const uint4*>(row) + x.c1);
+    r.a = ld_global_stream(reinterpret_cast<const uint4*>(row) + x.c0);
+    r.b = ld_global_stream(reinterpret_cast<const uint4*>(row) + x.c1);
   }
   return r;
 }
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) norm_rope_kernel(const _
   const int groups = groups_q + (p.Hkv + Sh::kHeads - 1) / Sh::kHeads;
   const int row = kPerRow ? 0 : x.row;
   const int g0 = slice * p.slice_groups, g1 = min(groups, g0 + p.slice_groups);
-  const int pos = p.rot > 0 && live_t ? __ldg(p.pos + b * p.pos_sb + s) : 0;
+  const int pos = p.rot > 0 && live_t ? ld_global(p.pos + b * p.pos_sb + s) : 0;
   Angles turn;
   uint64_t w[8];
   bool first = true;
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, kGradCtasPerSm)
     r.live = t < p.tokens;
     const uint32_t b = r.live ? t / static_cast<uint32_t>(p.S) : 0u;
     const uint32_t s = r.live ? t - b * static_cast<uint32_t>(p.S) : 0u;
-    r.pos = p.rot > 0 && r.live ? __ldg(p.pos + b * p.pos_sb + s) : 0;
+    r.pos = p.rot > 0 && r.live ? ld_global(p.pos + b * p.pos_sb + s) : 0;
     r.in = in.row(b, row, s);
     r.gin = gin.row(b, row, s);
     r.out = out.row(b, row, s);

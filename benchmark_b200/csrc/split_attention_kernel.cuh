@@ -106,8 +106,25 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int bh = unit / p.row_tiles;
   const int b = bh / p.Hkv, h = bh - b * p.Hkv;
 
+  const int len = p.kv_len ? ld_global_l2(p.kv_len + b) : p.Skv;
+  // Q as the A operand: lane holds rows lane/4 and lane/4 + 8, columns
+  // 2 (lane % 4) + {0, 1, 8, 9} of every 16.
+  uint32_t qa[D / 16][4];
+  const int ra = rt * kRows + (lane >> 2), rb = ra + 8;
+  const int ca = 2 * (lane & 3);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = min(half ? rb : ra, p.rows - 1);
+    const uint16_t* src = p.q.row(b, h * p.group + r % p.group, r / p.group) + ca;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      qa[kk][half] = ld_global_l2(reinterpret_cast<const uint32_t*>(src + kk * 16));
+      qa[kk][2 + half] = ld_global_l2(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8));
+    }
+  }
+
   // The tile's rows and the keys that some of them see.
-  const int n = p.kv_len ? max(0, min(p.kv_len[b], p.Skv)) : p.Skv;
+  const int n = max(0, min(len, p.Skv));
   const int r_last = min(rt * kRows + kRows - 1, p.rows - 1);
   auto position = [&](int r) { return n - p.Sq + r / p.group; };
   const int p_first = position(rt * kRows), p_last = position(r_last);
@@ -164,21 +181,6 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
   for (int s = 0; s < C::kStages - 1; ++s, next += stride) load_block(next, s);
 
-  // Q as the A operand: lane holds rows lane/4 and lane/4 + 8, columns
-  // 2 (lane % 4) + {0, 1, 8, 9} of every 16.
-  uint32_t qa[D / 16][4];
-  const int ra = rt * kRows + (lane >> 2), rb = ra + 8;
-  const int ca = 2 * (lane & 3);
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = min(half ? rb : ra, p.rows - 1);
-    const uint16_t* src = p.q.row(b, h * p.group + r % p.group, r / p.group) + ca;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      qa[kk][half] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
-      qa[kk][2 + half] = *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
-    }
-  }
   const int pos_a = position(min(ra, p.rows - 1)), pos_b = position(min(rb, p.rows - 1));
 
   float o[D / 8][4];

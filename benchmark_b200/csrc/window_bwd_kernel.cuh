@@ -226,7 +226,7 @@ __device__ __forceinline__ TileItem<kKeys> tile_item(const TileParams& p, int k)
   it.b = bh / heads;
   it.h = bh - it.b * heads;
   it.r0 = tile * kOwn;
-  it.n = p.kv_len ? max(0, min(__ldg(p.kv_len + it.b), p.Skv)) : p.Skv;
+  it.n = p.kv_len ? max(0, min(ld_global_l2(p.kv_len + it.b), p.Skv)) : p.Skv;
   it.off = it.n - p.Sq;
   if constexpr (kKeys) {
     const int k1 = min(it.r0 + kOwn, it.n);  // queries [i0, i1) see some of keys [r0, k1)
@@ -556,8 +556,8 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
       if (!kKeys && it.r0 + row < p.Sq) {
         const float* src =
             p.stats + (static_cast<int64_t>(it.b) * p.Hq + it.h) * p.sq_pad + it.r0 + row;
-        nlse = __ldg(src);
-        ndelta = __ldg(src + p.stat_plane);
+        nlse = ld_global_l2(src);
+        ndelta = ld_global_l2(src + p.stat_plane);
       }
     };
     if (static_cast<int>(blockIdx.x) < p.n_items) open_item(static_cast<int>(blockIdx.x));

@@ -555,3 +555,41 @@ def test_calls_follow_what_was_queued_before_them():
         wipe()
         assert torch.equal(got, chained)
     ops.check()
+
+
+def test_calls_read_the_small_inputs_that_were_written_before_them():
+    """Positions, frequencies, weights, lengths and statistics, changed between calls."""
+    g = gen(31)
+    B, Hq, Hkv, S, D = 6, 8, 2, 700, 128
+    q, k, v, gy = (randn(g, B, h, S, D) for h in (Hq, Hkv, Hkv, Hq))
+    sets = []
+    for _ in range(2):
+        sets.append([torch.randint(0, 9000, (B, S), generator=g, device="cuda", dtype=torch.int32),
+                     torch.rand(D // 2, generator=g, device="cuda"),
+                     torch.randn(D, generator=g, device="cuda"),
+                     torch.randint(1, S + 1, (B,), generator=g, device="cuda", dtype=torch.int32)])
+    pos, freq, w, lens = (t.clone() for t in sets[0])
+
+    def step():
+        qr, kr = ops.qk_norm_rope(q, k, w, w, freq, pos)
+        lse = torch.empty(B, Hq, S, device="cuda")
+        o = ops.attention_window_fwd(qr, kr, v, 150, 4, kv_len=lens, lse=lse)
+        dq, dk, dv = ops.attention_window_bwd(gy, qr, kr, v, o, lse, 150, 4, kv_len=lens)
+        one = ops.attention_window_fwd(qr[:, :, -1:], kr, v, 150, 4, kv_len=lens)
+        own = ops.attention_shared_prefix(qr[:, :, -1:], kr[0], v[0], kr, v, kv_len=lens)
+        return (o, dv, one, own, *ops.qk_norm_rope_bwd(dq, dk, q, k, w, w, freq, pos))
+
+    def fill(values):
+        for t, x in zip((pos, freq, w, lens), values):
+            t.copy_(x)
+    want = []
+    for s in sets:
+        fill(s)
+        torch.cuda.synchronize()
+        want.append(step())
+        torch.cuda.synchronize()
+    for i in range(20):
+        fill(sets[i % 2])
+        got = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2]))
+    ops.check()
