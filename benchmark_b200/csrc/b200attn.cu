@@ -76,13 +76,9 @@ struct MapKey {
   const void* base;
   uint64_t d0, d1, d2;
   uint32_t box0, box1, rank;
-  // 4-D maps only: the last extent, the strides and the outer box sizes.
-  uint64_t d3 = 0, s0 = 0, s1 = 0, s2 = 0;
-  uint32_t box2 = 0, box3 = 0;
   bool operator==(const MapKey& o) const {
     return base == o.base && d0 == o.d0 && d1 == o.d1 && d2 == o.d2 && box0 == o.box0 &&
-           box1 == o.box1 && rank == o.rank && d3 == o.d3 && s0 == o.s0 && s1 == o.s1 &&
-           s2 == o.s2 && box2 == o.box2 && box3 == o.box3;
+           box1 == o.box1 && rank == o.rank;
   }
 };
 
@@ -113,8 +109,7 @@ class MapCache {
   static size_t index(const MapKey& k) {
     uint64_t h = reinterpret_cast<uintptr_t>(k.base) * 0x9E3779B97F4A7C15ull;
     for (uint64_t v : {k.d0, k.d1, k.d2, static_cast<uint64_t>(k.box0) << 32 | k.box1,
-                       static_cast<uint64_t>(k.rank), k.d3, k.s0, k.s1, k.s2,
-                       static_cast<uint64_t>(k.box2) << 32 | k.box3})
+                       static_cast<uint64_t>(k.rank)})
       h = (h ^ v) * 0x100000001B3ull;
     return static_cast<size_t>(h >> 32) % kSlots;
   }
@@ -195,14 +190,6 @@ b200_status encode_bf16_2d_uncached(CUtensorMap* map, const void* base, uint64_t
 // 1 to 3), 128-byte swizzled boxes.
 b200_status encode_bf16_4d(CUtensorMap* map, const void* base, const cuuint64_t (&d)[4],
                            const cuuint64_t (&s)[3], const cuuint32_t (&box)[4]) {
-  MapKey key{base, d[0], d[1], d[2], box[0], box[1], 4};
-  key.d3 = d[3];
-  key.s0 = s[0];
-  key.s1 = s[1];
-  key.s2 = s[2];
-  key.box2 = box[2];
-  key.box3 = box[3];
-  if (map_cache().find(key, map)) return B200_OK;
   EncodeTiledFn enc = encode_fn();
   if (!enc) return fail(B200_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
   const cuuint32_t estr[4] = {1, 1, 1, 1};
@@ -214,7 +201,6 @@ b200_status encode_bf16_4d(CUtensorMap* map, const void* base, const cuuint64_t 
                 static_cast<int>(r), static_cast<unsigned long long>(d[0]),
                 static_cast<unsigned long long>(d[1]), static_cast<unsigned long long>(d[2]),
                 static_cast<unsigned long long>(d[3]));
-  map_cache().put(key, *map);
   return B200_OK;
 }
 

@@ -430,8 +430,8 @@ b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, cons
     return st;
   p.n_qtiles = (s.Sq + b200::attn::kBM - 1) / b200::attn::kBM;
   p.causal = 1;  // the order of the items, as causal attention's
-  // Hidden scores are -inf before the scale: a scale of 0 becomes one that no
-  // finite score notices.
+  // Hidden scores are -inf before the scale: a scale of 0 becomes one that
+  // changes no weight of scores below 1e30.
   if (p.scale_log2 == 0.0f) p.scale_log2 = 1e-37f;
   p.window = s.window;
   p.sinks = s.sinks;
