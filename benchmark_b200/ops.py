@@ -123,6 +123,9 @@ def _call(name: str, stream: torch.cuda.Stream | None, *args):
     fn = getattr(_binding or binding(), name)
     if stream is None:
         return fn(*args)
+    device = getattr(args[0], "device", None)
+    if device != stream.device:
+        raise ValueError(f"{name}: the stream is on {stream.device}, the tensors on {device}")
     with torch.cuda.stream(stream):  # what the call allocates belongs to that stream
         return fn(*args)
 

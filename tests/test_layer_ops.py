@@ -149,6 +149,14 @@ def test_python_refuses_cpu_tensors():
         ops.qk_norm_rope(q, q, q[0, 0, 0], q[0, 0, 0], torch.ones(8), torch.zeros(4))
 
 
+def test_python_refuses_a_stream_of_another_device():
+    class Stream:
+        device = torch.device("cuda", 1)
+    q = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        ops.attention_window_fwd(q, q, q, 4, stream=Stream())
+
+
 def directional(f, inputs, grads, seed=0, h=1e-5):
     """The gradients' inner product with a direction, and f's difference along it."""
     g = torch.Generator().manual_seed(seed)
