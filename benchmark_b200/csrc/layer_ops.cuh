@@ -92,7 +92,7 @@ b200_status rope_args(const char* who, const b200_tensor* q, const b200_tensor* 
                       const void* q_weight, const void* k_weight, int weight_f32,
                       const float* inv_freq, int rotary_dim, int interleaved,
                       const int32_t* positions, int64_t position_stride_b, float eps, int B,
-                      int S, int Hq, int Hkv, int D, RopeArgs* out) {
+                      int S, int Hq, int Hkv, int D, bool backward, RopeArgs* out) {
   if (B < 1 || S < 1 || Hq < 1 || Hkv < 1)
     return fail(B200_EINVAL, "%s: invalid shape B=%d S=%d Hq=%d Hkv=%d", who, B, S, Hq, Hkv);
   if (D != 64 && D != 128)
@@ -131,11 +131,21 @@ b200_status rope_args(const char* who, const b200_tensor* q, const b200_tensor* 
   p.Hkv = Hkv;
   p.rot = rotary_dim;
   p.eps = eps;
-  // Rows of a warp hold heads of one token unless half of them or more would
-  // stay empty.
+  // Rows of a warp hold heads of one token, or a token each (per_row).  The
+  // second leaves none empty, but each row forms its own angles and few tokens
+  // fill few warps.  Measured (us, first / second form; tokens, heads x D),
+  // forward: 2048, 1+1 x 128 4.3 / 3.7; 8192, 4+2 x 128 9.3 / 8.0; 4096, 4+2 x
+  // 128 5.6 / 6.3; 16384, 8+8 x 128 25.3 / 25.0, 16+4 x 128 29.8 / 30.9, 16+16 x
+  // 64 25.3 / 27.1.  Backward: 2048, 1+1 x 128 7.1 / 5.8; 4096, 16+4 x 128 17.7 /
+  // 15.7; 2048, 4+2 x 128 7.3 / 7.0; 666, 10+5 x 64 5.6 / 8.4; 16384, 16+16 x 64
+  // 38.2 / 40.8; 8192, 32+8 x 128 47.3 / 53.1.
   const int rows = 512 / D;
   RopeArgs a{p, false, (Hq + rows - 1) / rows, (Hkv + rows - 1) / rows, p.tokens};
-  a.per_row = 2ll * (Hq + Hkv) <= static_cast<long long>(a.groups_q + a.groups_k) * rows;
+  const bool half_empty =
+      2ll * (Hq + Hkv) <= static_cast<long long>(a.groups_q + a.groups_k) * rows;
+  a.per_row = half_empty ? p.tokens >= 2048
+                         : Hq + Hkv <= (backward ? 24 : 16) &&
+                               p.tokens >= (backward ? 4096u : 8192u);
   if (a.per_row) {
     a.groups_q = Hq;
     a.groups_k = Hkv;
@@ -706,7 +716,8 @@ b200_status qk_norm_rope(const b200_tensor* q, const b200_tensor* k, const void*
   const char* who = "qk_norm_rope";
   RopeArgs a;
   b200_status st = rope_args(who, q, k, q_weight, k_weight, weight_f32, inv_freq, rotary_dim,
-                             interleaved, positions, position_stride_b, eps, B, S, Hq, Hkv, D, &a);
+                             interleaved, positions, position_stride_b, eps, B, S, Hq, Hkv, D, false,
+                             &a);
   if (st != B200_OK) return st;
   if ((st = check_tensor(who, "q_out", q_out, B, Hq, S, D, true)) != B200_OK) return st;
   if ((st = check_tensor(who, "k_out", k_out, B, Hkv, S, D, true)) != B200_OK) return st;
@@ -746,7 +757,8 @@ b200_status qk_norm_rope_bwd(const b200_tensor* dq_out, const b200_tensor* dk_ou
   const char* who = "qk_norm_rope_bwd";
   RopeArgs a;
   b200_status st = rope_args(who, q, k, q_weight, k_weight, weight_f32, inv_freq, rotary_dim,
-                             interleaved, positions, position_stride_b, eps, B, S, Hq, Hkv, D, &a);
+                             interleaved, positions, position_stride_b, eps, B, S, Hq, Hkv, D, true,
+                             &a);
   if (st != B200_OK) return st;
   if ((st = check_tensor(who, "dq_out", dq_out, B, Hq, S, D, false)) != B200_OK) return st;
   if ((st = check_tensor(who, "dk_out", dk_out, B, Hkv, S, D, false)) != B200_OK) return st;

@@ -13,14 +13,17 @@
 // D/16 lanes, 16 values each as two 16-byte chunks placed so that a rotated
 // pair never crosses lanes: the row statistics take log2(D/16) shuffles and
 // the rotation none.  A warp walks the heads of one token, so that its lanes
-// keep their angles and weights in registers; it has the next rows in flight
-// while it works on its own, and nothing synchronises the warps.  (A first
-// form kept both in shared memory for a block of tokens: its reads kept the
-// load/store unit 80 % busy, 77 us against 63 for 16384 tokens of 32 + 8
-// heads of 128.)  With few heads a warp's lanes would stay empty: then each
-// of its rows walks a token of its own (kPerRow).
+// keep their angles and weights in registers; the next rows are on their way
+// through a ring in shared memory, of which each lane copies and reads its own
+// slots: nothing synchronises the warps.  16384 tokens of 32 + 8 heads of 128:
+// forward 54.6 us (6.1 TB/s), backward 88.4 us (5.7 TB/s).  (With the next rows
+// in registers instead, one row group ahead: 63.5 and 107 us.  With angles and
+// weights in shared memory for a block of tokens, their reads kept the
+// load/store unit 80 % busy: 77 us forward.)  With few heads a warp's lanes
+// would stay empty: then each of its rows walks a token of its own (kPerRow).
 #pragma once
 
+#include "mma_sync.cuh"
 #include "ptx.cuh"
 #include "view.cuh"
 
@@ -29,11 +32,13 @@ namespace rope {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-// Resident CTAs, by registers: forward measured 66 / 63 / 68 / 75 us with 6 / 7
-// / 8 / 9 (16384 tokens, 32 + 8 heads of 128), backward 114 / 109 / 142 us with
-// 3 / 4 / 5.
+// Resident CTAs, by registers, and row groups of a warp's ring.  Measured (us;
+// 16384 tokens, 32 + 8 heads of 128): forward with 6 / 7 / 8 / 10 CTAs 55.2 /
+// 54.6 / 55.6 / 86, with 2 / 3 / 4 groups 59.3 / 54.6 / 55.2; backward with 3 /
+// 4 / 5 CTAs 95 / 88.4 / 146, with 2 / 3 / 4 groups 94.5 / 88.4 / 94.7.
 constexpr int kCtasPerSm = 7;
 constexpr int kGradCtasPerSm = 4;
+constexpr int kStages = 3, kGradStages = 3;
 
 struct Params {
   View q, k;            // x
@@ -221,18 +226,19 @@ __device__ __forceinline__ float row_norm(const uint64_t (&v)[8], float eps) {
   return rsqrtf(row_sum<D / 16>(f2_add(e, o)) * (1.0f / D) + eps);
 }
 
-// The two chunks of a lane; streamed, since nothing reads them again.
-struct Chunks {
-  uint4 a, b;
-};
+// A lane's two chunks of a row on their way through its own slots of a ring in
+// shared memory (nothing but its own copies and reads meet there: no barrier).
+using Slots = uint4[2][kThreads];
 
-__device__ __forceinline__ Chunks load_chunks(const uint16_t* row, const Lane& x, bool live) {
-  Chunks r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-  if (live) {
-    r.a = ld_global_stream(reinterpret_cast<const uint4*>(row) + x.c0);
-    r.b = ld_global_stream(reinterpret_cast<const uint4*>(row) + x.c1);
-  }
-  return r;
+__device__ __forceinline__ void copy_chunks(Slots& to, const uint16_t* row, const Lane& x,
+                                            bool live) {
+  cp_async16(smem_u32(&to[0][threadIdx.x]), row + 8 * x.c0, live);
+  cp_async16(smem_u32(&to[1][threadIdx.x]), row + 8 * x.c1, live);
+}
+
+__device__ __forceinline__ void read_chunks(const Slots& from, uint64_t (&v)[8]) {
+  unpack8(from[0][threadIdx.x], v);
+  unpack8(from[1][threadIdx.x], v + 4);
 }
 
 __device__ __forceinline__ void store_chunks(uint16_t* row, const Lane& x,
@@ -245,6 +251,7 @@ __device__ __forceinline__ void store_chunks(uint16_t* row, const Lane& x,
 template <int D, bool kInterleaved, bool kPerRow>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) norm_rope_kernel(const __grid_constant__ Params p) {
   using Sh = Shape<D, kPerRow>;
+  __shared__ Slots ring[kStages];
   pdl_wait();
   pdl_launch_dependents();
   const Lane x = lane_of<Sh::kLanes>(p.rot);
@@ -261,40 +268,39 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) norm_rope_kernel(const _
   const int row = kPerRow ? 0 : x.row;
   const int g0 = slice * p.slice_groups, g1 = min(groups, g0 + p.slice_groups);
   const int pos = p.rot > 0 && live_t ? ld_global(p.pos + b * p.pos_sb + s) : 0;
-  Angles turn;
-  uint64_t w[8];
-  bool first = true;
-  // Row groups [g, end) of one tensor, the next one's rows in flight.
-  auto walk = [&](const View& from, const View& to, const void* weight, int H, int g, int end) {
-    if (g >= end) return;
-    int h = g * Sh::kHeads + row;
-    const int64_t step = Sh::kHeads * from.sh, out_step = Sh::kHeads * to.sh;
-    const uint16_t* in = from.row(b, h, s);
-    uint16_t* out = to.row(b, h, s);
-    const int H_live = live_t ? H : 0;
-    Chunks next = load_chunks(in, x, h < H_live);
-    if (first) turn = lane_angles<D, kInterleaved, kPerRow>(p.inv_freq, pos, x);
-    first = false;
-    load_weights(weight, p.w_f32, x, w);
-    for (int i = end - g; i > 0; --i) {
-      uint64_t v[8];
-      unpack8(next.a, v);
-      unpack8(next.b, v + 4);
-      const bool live = h < H_live;
-      h += Sh::kHeads;
-      in += step;
-      next = load_chunks(in, x, h < H_live);
-      const float rn = row_norm<D>(v, p.eps);
-      const uint64_t rn2 = f2_pack(rn, rn);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = f2_mul(v[e], f2_mul(w[e], rn2));
-      rotate16<kInterleaved, false>(v, turn);
-      if (live) store_chunks(out, x, v);
-      out += out_step;
+  // Row groups g0 to g1, the queries' before the keys'; kStages - 1 on their way.
+  auto copy = [&](int g, int stage) {
+    if (g < g1) {
+      const bool is_q = g < groups_q;
+      const View& from = is_q ? p.q : p.k;
+      const int h = (is_q ? g : g - groups_q) * Sh::kHeads + row;
+      const bool live = live_t && h < (is_q ? p.Hq : p.Hkv);
+      copy_chunks(ring[stage], from.row(b, live ? h : 0, s), x, live);
     }
+    cp_async_commit();
   };
-  walk(p.q, p.qy, p.wq, p.Hq, g0, min(g1, groups_q));
-  walk(p.k, p.ky, p.wk, p.Hkv, max(g0 - groups_q, 0), g1 - groups_q);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) copy(g0 + i, i);
+  const Angles turn = lane_angles<D, kInterleaved, kPerRow>(p.inv_freq, pos, x);
+  uint64_t w[8];
+  int stage = 0;
+  for (int g = g0; g < g1; ++g) {
+    const bool is_q = g < groups_q;
+    if (g == g0 || g == groups_q) load_weights(is_q ? p.wq : p.wk, p.w_f32, x, w);
+    cp_async_wait<kStages - 2>();
+    uint64_t v[8];
+    read_chunks(ring[stage], v);
+    copy(g + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    const float rn = row_norm<D>(v, p.eps);
+    const uint64_t rn2 = f2_pack(rn, rn);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f2_mul(v[e], f2_mul(w[e], rn2));
+    rotate16<kInterleaved, false>(v, turn);
+    const int h = (is_q ? g : g - groups_q) * Sh::kHeads + row;
+    if (live_t && h < (is_q ? p.Hq : p.Hkv))
+      store_chunks((is_q ? p.qy : p.ky).row(b, h, s), x, v);
+  }
 }
 
 // Backward: the first ctas_q CTAs take the queries, the others the keys.
@@ -306,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, kGradCtasPerSm)
     norm_rope_bwd_kernel(const __grid_constant__ Params p) {
   using Sh = Shape<D, kPerRow>;
   __shared__ float dw_sh[kWarps][D];
+  __shared__ Slots ring[kGradStages][2];
   pdl_wait();
   pdl_launch_dependents();
   const Lane x = lane_of<Sh::kLanes>(p.rot);
@@ -327,50 +334,60 @@ __global__ void __launch_bounds__(kThreads, kGradCtasPerSm)
   struct Place {
     bool live;
     int pos;
-    const uint16_t *in, *gin;
-    uint16_t* out;
+    int64_t b, s;
   };
   auto place = [&](uint32_t tg) {
     Place r;
     const uint32_t t = tg * Sh::kTokens + (kPerRow ? x.row : 0);
     r.live = t < p.tokens;
     const uint32_t b = r.live ? t / static_cast<uint32_t>(p.S) : 0u;
-    const uint32_t s = r.live ? t - b * static_cast<uint32_t>(p.S) : 0u;
-    r.pos = p.rot > 0 && r.live ? ld_global(p.pos + b * p.pos_sb + s) : 0;
-    r.in = in.row(b, row, s);
-    r.gin = gin.row(b, row, s);
-    r.out = out.row(b, row, s);
+    r.b = b;
+    r.s = r.live ? t - b * static_cast<uint32_t>(p.S) : 0u;
+    r.pos = p.rot > 0 && r.live ? ld_global(p.pos + r.b * p.pos_sb + r.s) : 0;
     return r;
   };
-  const int64_t in_step = Sh::kHeads * in.sh, gin_step = Sh::kHeads * gin.sh,
-                out_step = Sh::kHeads * out.sh;
-  Chunks nx, ng;
-  uint32_t tg = static_cast<uint32_t>(cta) * kWarps + warp_id();
-  Place now{}, then{};
-  if (tg < token_groups) {
-    now = place(tg);
-    nx = load_chunks(now.in, x, now.live && row < H);
-    ng = load_chunks(now.gin, x, now.live && row < H);
-  }
+  // The copies run kStages - 1 row groups ahead, through the warp's tokens.
+  uint32_t tg = static_cast<uint32_t>(cta) * kWarps + warp_id(), ctg = tg;
+  int ch = row;  // head of the next copy
+  const uint16_t *c_in = nullptr, *c_gin = nullptr;
+  bool c_live = false;
+  auto open = [&]() {
+    if (ctg >= token_groups) return;
+    const Place r = place(ctg);
+    c_live = r.live;
+    c_in = in.row(r.b, 0, r.s);
+    c_gin = gin.row(r.b, 0, r.s);
+  };
+  auto copy = [&](int stage) {
+    if (ctg < token_groups) {
+      const bool live = c_live && ch < H;
+      const int64_t h = live ? ch : 0;
+      copy_chunks(ring[stage][0], c_in + h * in.sh, x, live);
+      copy_chunks(ring[stage][1], c_gin + h * gin.sh, x, live);
+      ch += Sh::kHeads;
+      if (ch - row >= H) {
+        ch = row;
+        ctg += stride;
+        open();
+      }
+    }
+    cp_async_commit();
+  };
+  open();
+#pragma unroll
+  for (int i = 0; i < kGradStages - 1; ++i) copy(i);
+  int stage = 0;
+  Place now = place(tg);
   for (; tg < token_groups; tg += stride) {
-    const bool more = tg + stride < token_groups;
-    if (more) then = place(tg + stride);
+    const Place then = place(min(tg + stride, token_groups - 1));
     const Angles turn = lane_angles<D, kInterleaved, kPerRow>(p.inv_freq, now.pos, x);
     for (int h = row; h - row < H; h += Sh::kHeads) {
       uint64_t v[8], g[8];
-      unpack8(nx.a, v);
-      unpack8(nx.b, v + 4);
-      unpack8(ng.a, g);
-      unpack8(ng.b, g + 4);
-      if (h - row + Sh::kHeads < H) {
-        now.in += in_step;
-        now.gin += gin_step;
-        nx = load_chunks(now.in, x, now.live && h + Sh::kHeads < H);
-        ng = load_chunks(now.gin, x, now.live && h + Sh::kHeads < H);
-      } else if (more) {
-        nx = load_chunks(then.in, x, then.live && row < H);
-        ng = load_chunks(then.gin, x, then.live && row < H);
-      }
+      cp_async_wait<kGradStages - 2>();
+      read_chunks(ring[stage][0], v);
+      read_chunks(ring[stage][1], g);
+      copy(stage == 0 ? kGradStages - 1 : stage - 1);
+      stage = stage + 1 == kGradStages ? 0 : stage + 1;
       const bool live = now.live && h < H;
       // (Without eps the zeros of a row that is not there would give NaN.)
       const float norm = row_norm<D>(v, p.eps), rn = live ? norm : 0.0f;
@@ -388,8 +405,7 @@ __global__ void __launch_bounds__(kThreads, kGradCtasPerSm)
       const uint64_t d2 = f2_pack(dot, dot);
 #pragma unroll
       for (int i = 0; i < 8; ++i) g[i] = f2_mul(rn2, f2_fma(v[i], d2, g[i]));
-      if (live) store_chunks(now.out, x, g);
-      now.out += out_step;
+      if (live) store_chunks(out.row(now.b, h, now.s), x, g);
     }
     now = then;
   }

@@ -231,14 +231,6 @@ __device__ __forceinline__ uint4 ld_global(const uint4* p) {
                : "l"(p));
   return v;
 }
-// As these, of data that is read once.
-__device__ __forceinline__ uint4 ld_global_stream(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 // From L2, for a kernel that does not wait: what it reads was complete before
 // its predecessor let it start, but L1 may hold older lines.
 __device__ __forceinline__ int ld_global_l2(const int* p) {

@@ -52,6 +52,8 @@ ROPE = [  # B, S, Hq, Hkv, D, R, interleaved, w32
     (3, 77, 2, 1, 128, 128, False, True),   # few heads: a token to each row of a warp
     (2, 1301, 2, 2, 64, 64, True, False),
     (1, 3, 1, 1, 64, 32, False, False),
+    (1, 2300, 2, 1, 128, 128, False, True),
+    (3, 1399, 17, 6, 128, 64, False, False),  # backward only: a token to each row
 ]
 
 
