@@ -9,20 +9,23 @@
  *
  * Conventions
  *   - All tensor pointers are device pointers owned by the caller, 16-byte
- *     aligned, contiguous.
+ *     aligned, contiguous unless passed as a b200_tensor (by its strides).
  *   - attention_fwd splits the K/V range of short problems (too few 128-row
  *     Q tiles to fill the GPU, K/V ranges of 48 or more 128-key tiles) among
  *     several CTAs that merge through a workspace.  The workspace belongs to
  *     the library, one per (device, stream); the first such call on a
  *     (device, stream) allocates it (cudaMalloc, which synchronises the
  *     device) and later calls reuse it, growing it when a larger problem
- *     needs more.  Nothing else allocates.
+ *     needs more.  Nothing else allocates: the attention layer's operators
+ *     take their workspaces from the caller, who may reuse one as soon as the
+ *     call's work on the stream is done.
  *   - bf16 tensors are passed as raw 16-bit words (uint16_t storage).
  *   - Calls are asynchronous on `stream` (NULL = legacy default stream) and
  *     use the calling thread's current CUDA device.
- *   - TMA tensor maps are encoded on the first call for a (pointer, shape)
- *     and kept in a fixed-size table, so repeated calls on the same buffers
- *     skip the driver encode.
+ *   - The dense entry points' TMA tensor maps are encoded on the first call
+ *     for a (pointer, shape) and kept in a fixed-size table, so repeated calls
+ *     on the same buffers skip the driver encode.  Those of b200_tensor
+ *     arguments are encoded at each call.
  *   - Errors are returned as b200_status, never by exit(); a message for the
  *     most recent failure on the calling thread is in b200_last_error().
  *   - Device-side waits are bounded.  A kernel whose pipeline wait runs out
@@ -224,7 +227,7 @@ b200_status attention_window_bwd(const b200_tensor* dout, const b200_tensor* q,
  * Attention of a batch whose requests share a prefix: query i of request b
  * sees all P prefix keys, and of its own keys those at j <= kv_len[b] - Sq + i
  * (kv_len as above, of at most S).  The prefix is read for the whole batch at
- * once, not for each request.
+ * once, or, where that is little work, for each request through L2.
  *   q, o: [B, Hq, Sq, D]   k_prefix, v_prefix: [1, Hkv, P, D] (P = 0: ignored)
  *   k, v: [B, Hkv, S, D]   D in {64, 128}
  */
