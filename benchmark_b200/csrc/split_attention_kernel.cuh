@@ -107,21 +107,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int b = bh / p.Hkv, h = bh - b * p.Hkv;
 
   const int len = p.kv_len ? ld_global_l2(p.kv_len + b) : p.Skv;
-  // Q as the A operand: lane holds rows lane/4 and lane/4 + 8, columns
-  // 2 (lane % 4) + {0, 1, 8, 9} of every 16.
-  uint32_t qa[D / 16][4];
-  const int ra = rt * kRows + (lane >> 2), rb = ra + 8;
-  const int ca = 2 * (lane & 3);
+  // The tile's Q rows, through the ring's last stage, which no block takes
+  // before the loop.
+  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStageBytes;
+  const uint32_t q_at = ring + (C::kStages - 1) * C::kStageBytes;
+  {
+    // Two lanes to a row; those past the last are zeroed, not read.
+    const int i = lane >> 1;
+    const bool live = rt * kRows + i < p.rows;
+    const int r = live ? rt * kRows + i : 0;
+    const uint16_t* src = p.q.row(b, h * p.group + r % p.group, r / p.group);
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = min(half ? rb : ra, p.rows - 1);
-    const uint16_t* src = p.q.row(b, h * p.group + r % p.group, r / p.group) + ca;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      qa[kk][half] = ld_global_l2(reinterpret_cast<const uint32_t*>(src + kk * 16));
-      qa[kk][2 + half] = ld_global_l2(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8));
-    }
+    for (int c = lane & 1; c < D / 8; c += 2)
+      cp_async16(q_at + swz<C::kRowBytes>(i, c), src + c * 8, live);
   }
+  cp_async_commit();
 
   // The tile's rows and the keys that some of them see.
   const int n = max(0, min(len, p.Skv));
@@ -138,7 +138,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int b0 = static_cast<int>(static_cast<int64_t>(nb) * split / p.nsplit);
   const int b1 = static_cast<int>(static_cast<int64_t>(nb) * (split + 1) / p.nsplit);
 
-  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStageBytes;
   // Keys [j0, j1) of block i, of the prefix or of the request.
   auto block_keys = [&](int i, int* j0, int* j1) {
     if (i < nb_p) {
@@ -181,6 +180,16 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
   for (int s = 0; s < C::kStages - 1; ++s, next += stride) load_block(next, s);
 
+  // Q as the A operand: lane holds rows lane/4 and lane/4 + 8, columns
+  // 2 (lane % 4) + {0, 1, 8, 9} of every 16.
+  cp_async_wait<C::kStages - 1>();
+  __syncwarp();
+  uint32_t qa[D / 16][4];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    ldsm4(q_at + swz<C::kRowBytes>(lane & 15, 2 * kk + (lane >> 4)), qa[kk]);
+  const int ra = rt * kRows + (lane >> 2), rb = ra + 8;
+  const int ca = 2 * (lane & 3);
   const int pos_a = position(min(ra, p.rows - 1)), pos_b = position(min(rb, p.rows - 1));
 
   float o[D / 8][4];
