@@ -63,11 +63,14 @@
 // stores O and resets the counter.  No second launch is needed.
 //
 // Two more forms of the same pipeline (kForm), on strided tensors (4-D maps):
-//   kWindow: sliding window and sinks, a key count per batch row.  An item
-//     visits the tiles of [0, sinks), then the window's; masked tiles test
-//     both ends.  V rows that no row of the item sees are zeroed in shared
-//     memory before the PV product reads them, since they may hold anything
-//     (0 * NaN is NaN); K's need not be: their scores are replaced.
+//   kWindow: sliding window and sinks, a key count per batch row.  The 128 rows
+//     are a box of (tokens, heads of one kv head) of Q, so that they reach few
+//     keys beyond the window.  An item's tiles start at its first key, not at a
+//     multiple of 128; up to kFold sinks lie in the first one's first rows,
+//     more have tiles of their own.  Masked tiles test both ends.  V rows that
+//     no row of the item sees are zeroed in shared memory before the PV product
+//     reads them, since they may hold anything (0 * NaN is NaN); K's need not
+//     be: their scores are replaced.
 //   kPrefix: the queries of a whole batch against one shared K/V.  A tile's
 //     128 rows are a box of (batches, tokens, heads of one kv head) of Q; every
 //     unit takes a share of the keys and leaves unnormalised O and (m, l) in a
@@ -139,6 +142,7 @@ struct Params {
   // in its map: its coordinate is multiplied by 0 (q, k, v; batch and head).
   int q_mb, q_mh, k_mb, k_mh, v_mb, v_mh;
   int window, sinks;      // kWindow
+  int tile_heads, tile_tokens;  // kWindow: of a tile; heads divide group, heads x tokens <= 128
   const int32_t* kv_len;  // kWindow: [B] or null (Skv)
   float* lse;             // kWindow: [B, Hq, Sq] or null
   int tile_batches;       // kPrefix: batches of a tile
@@ -148,6 +152,16 @@ struct Params {
 
 // Forms of the kernel.
 constexpr int kDense = 0, kWindow = 1, kPrefix = 2;
+
+// kWindow: the rows that sinks take in an item's first tile, and the maps of
+// its two parts, kFold and kBN - kFold rows.
+constexpr int kFold = 8;
+struct FoldMaps {
+  CUtensorMap k_sinks, k_rest, v_sinks, v_rest;
+};
+struct NoFold {};  // the other forms'
+template <int kForm>
+using FoldOf = std::conditional_t<kForm == kWindow, FoldMaps, NoFold>;
 
 // Clock-trace events (kTrace); names in benchmark_b200/trace.py.
 enum : uint32_t {
@@ -257,37 +271,40 @@ struct Item {
 struct FormItem : Item {
   int b, hq, hkv;
   int split;       // kPrefix
-  // kWindow: rows of the item see keys of [0, se) and [lo, hi) only; tile j is
-  // j for the n_sink tiles before the window's and j + skip after them; row r
-  // is at position off + row0 + r; keys below top_lo (and past the sinks) are
-  // hidden from the last row.
-  int se, lo, hi, n_sink, skip, off, top_lo, kv_len;
+  // kWindow: rows of the item see keys of [0, se) and [lo, hi) only.  Row r is
+  // at position off + row0 + r / tile_heads; keys below top_lo (and past the
+  // sinks) are hidden from the last row.  Tile j starts at key 128 j for the
+  // n_sink tiles of sinks and at base + 128 (j - n_sink) after them; with fold,
+  // the first kFold rows of the first tile are keys [0, kFold).
+  int se, lo, hi, base, n_sink, off, top_lo, kv_len;
+  bool fold;
 };
 
 __device__ __forceinline__ FormItem decode_window_item(const Params& p, int k) {
-  const int bhs = p.B * p.Hq;
+  const int planes_b = p.Hq / p.tile_heads;  // of a batch row
+  const int planes = p.B * planes_b;
   const int per_group = p.cgroup * p.n_qtiles;
   const int g = k / per_group;
   const int kl = k - g * per_group;
-  const int gs = min(p.cgroup, bhs - g * p.cgroup);
+  const int gs = min(p.cgroup, planes - g * p.cgroup);
   const int qt = p.n_qtiles - 1 - kl / gs;
-  const int bh = g * p.cgroup + (kl - (kl / gs) * gs);
+  const int plane = g * p.cgroup + (kl - (kl / gs) * gs);
   FormItem it;
-  it.b = bh / p.Hq;
-  it.hq = bh - it.b * p.Hq;
+  it.b = plane / planes_b;
+  it.hq = (plane - it.b * planes_b) * p.tile_heads;
   it.hkv = it.hq / p.group;
-  it.row0 = qt * kBM;
+  it.row0 = qt * p.tile_tokens;
   it.kv_len = p.kv_len ? max(0, min(ld_global(p.kv_len + it.b), p.Skv)) : p.Skv;
   it.off = it.kv_len - p.Sq;
-  const int last = it.off + min(it.row0 + kBM, p.Sq) - 1;  // the last row's position
+  const int last = it.off + min(it.row0 + p.tile_tokens, p.Sq) - 1;  // the last row's position
   it.hi = max(0, last + 1);
   it.lo = max(0, it.off + it.row0 - p.window + 1);
   if (p.sinks >= it.lo || it.hi == 0) it.lo = 0;
   it.se = it.lo > 0 ? p.sinks : 0;
-  const int w0 = it.lo / kBN;
-  it.n_sink = min((it.se + kBN - 1) / kBN, w0);
-  it.skip = w0 - it.n_sink;
-  it.n = it.n_sink + (it.hi + kBN - 1) / kBN - w0;
+  it.fold = it.se > 0 && it.se <= kFold;
+  it.n_sink = it.fold ? 0 : (it.se + kBN - 1) / kBN;
+  it.base = it.fold ? it.lo - kFold : it.lo;
+  it.n = it.n_sink + (it.hi - it.base + kBN - 1) / kBN;
   it.j0 = 0;
   it.top_lo = last - p.window + 1;
   it.min_lim = min(it.kv_len, it.off + it.row0 + 1);
@@ -307,8 +324,6 @@ __device__ __forceinline__ FormItem decode_prefix_item(const Params& p, int k) {
   const int n_all = (p.Skv + kBN - 1) / kBN;
   it.j0 = static_cast<int>(static_cast<int64_t>(n_all) * it.split / p.nsplit);
   it.n = static_cast<int>(static_cast<int64_t>(n_all) * (it.split + 1) / p.nsplit) - it.j0;
-  it.n_sink = it.n;  // tile j is j0 + j
-  it.skip = 0;
   it.min_lim = p.Skv;
   return it;
 }
@@ -446,7 +461,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap q_map,
                          const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map,
-                         const __grid_constant__ CUtensorMap o_map, const Params p) {
+                         const __grid_constant__ CUtensorMap o_map, const Params p,
+                         const __grid_constant__ FoldOf<kForm> fold) {
   using C = Cfg<D, kPair>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -498,18 +514,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     else
       return kPair ? decode_pair_item(p, k) : decode_item(p, k);
   };
-  // Index of an item's K/V tile j.
-  auto kv_tile = [](const auto& it, int j) {
-    if constexpr (kForm == kDense)
-      return it.j0 + j;
+  // First key of an item's K/V tile j.
+  auto kv_key = [](const auto& it, int j) {
+    if constexpr (kForm == kWindow)
+      return j < it.n_sink ? j * kBN : it.base + (j - it.n_sink) * kBN;
     else
-      return it.j0 + (j < it.n_sink ? j : j + it.skip);
+      return (it.j0 + j) * kBN;
+  };
+  // kWindow: the two parts of a tile that holds sinks, box h.
+  auto load_fold = [](uint8_t* dst, const CUtensorMap& sinks, const CUtensorMap& rest,
+                      uint64_t* bar, int h, int lo, int head, int b, uint64_t pol) {
+    tma_load_4d(dst + h * C::kBoxBytes, &sinks, bar, h * 64, 0, head, b, pol);
+    tma_load_4d(dst + h * C::kBoxBytes + kFold * 128, &rest, bar, h * 64, lo, head, b, pol);
   };
   // The leader's copy of a barrier of this CTA's layout (shared::cluster).
   auto lead_bar = [&](uint64_t* b_) { return mapa_shared(smem_u32(b_), 0u); };
 
   // ---- setup ----
-  if constexpr (kForm == kPrefix) {
+  if constexpr (kForm != kDense) {
     // Rows past a tile's box stay zero (their scores are computed, and dropped).
     for (int i = static_cast<int>(threadIdx.x); i < 2 * C::kTileBytes / 16; i += kThreads)
       reinterpret_cast<uint4*>(q_buf)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -611,10 +633,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_load_3d_pair(q_buf + qb * C::kTileBytes + h * C::kBoxBytes, &q_map,
                                  lead_bar(&q_full[qb]), h * 64, it.row0, it.zq, pol_q);
             } else if constexpr (kForm == kWindow) {
-              mbar_arrive_expect_tx(&q_full[qb], C::kTileBytes);
+              // A box of (64 columns, heads, tokens).
+              mbar_arrive_expect_tx(&q_full[qb], static_cast<uint32_t>(C::kBoxes * 128 *
+                                                                       p.tile_heads *
+                                                                       p.tile_tokens));
               for (int h = 0; h < C::kBoxes; ++h)
                 tma_load_4d(q_buf + qb * C::kTileBytes + h * C::kBoxBytes, &q_map, &q_full[qb],
-                            h * 64, it.row0, it.hq * p.q_mh, it.b * p.q_mb, pol_q);
+                            h * 64, it.hq * p.q_mh, it.row0, it.b * p.q_mb, pol_q);
             } else if constexpr (kForm == kPrefix) {
               // A box of (64 columns, heads of the kv head, tokens, batches).
               mbar_arrive_expect_tx(&q_full[qb],
@@ -648,10 +673,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    it.zkv, pol_kv);
               } else if constexpr (kForm != kDense) {
                 mbar_arrive_expect_tx(&k_full[ks], C::kTileBytes);
-                for (int h = 0; h < C::kBoxes; ++h)
-                  tma_load_4d(k_buf + ks * C::kTileBytes + h * C::kBoxBytes, &k_map, &k_full[ks],
-                              h * 64, kv_tile(it, j) * kBN, it.hkv * p.k_mh, it.b * p.k_mb,
-                              pol_kv);
+                bool folded = false;
+                if constexpr (kForm == kWindow) folded = it.fold && j == 0;
+                for (int h = 0; h < C::kBoxes; ++h) {
+                  uint8_t* dst = k_buf + ks * C::kTileBytes;
+                  const int head = it.hkv * p.k_mh, b = it.b * p.k_mb;
+                  if (!folded)
+                    tma_load_4d(dst + h * C::kBoxBytes, &k_map, &k_full[ks], h * 64,
+                                kv_key(it, j), head, b, pol_kv);
+                  if constexpr (kForm == kWindow) {
+                    if (folded)
+                      load_fold(dst, fold.k_sinks, fold.k_rest, &k_full[ks], h, it.lo, head, b,
+                                pol_kv);
+                  }
+                }
               } else {
                 mbar_arrive_expect_tx(&k_full[ks], C::kTileBytes);
                 for (int h = 0; h < C::kBoxes; ++h)
@@ -674,10 +709,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    (it.j0 + j) * kBN, it.zkv, pol_kv);
               } else if constexpr (kForm != kDense) {
                 mbar_arrive_expect_tx(&v_full[vs], C::kTileBytes);
-                for (int h = 0; h < C::kBoxes; ++h)
-                  tma_load_4d(v_buf + vs * C::kTileBytes + h * C::kBoxBytes, &v_map, &v_full[vs],
-                              h * 64, kv_tile(it, j) * kBN, it.hkv * p.v_mh, it.b * p.v_mb,
-                              pol_kv);
+                bool folded = false;
+                if constexpr (kForm == kWindow) folded = it.fold && j == 0;
+                for (int h = 0; h < C::kBoxes; ++h) {
+                  uint8_t* dst = v_buf + vs * C::kTileBytes;
+                  const int head = it.hkv * p.v_mh, b = it.b * p.v_mb;
+                  if (!folded)
+                    tma_load_4d(dst + h * C::kBoxBytes, &v_map, &v_full[vs], h * 64,
+                                kv_key(it, j), head, b, pol_kv);
+                  if constexpr (kForm == kWindow) {
+                    if (folded)
+                      load_fold(dst, fold.v_sinks, fold.v_rest, &v_full[vs], h, it.lo, head, b,
+                                pol_kv);
+                  }
+                }
               } else {
                 mbar_arrive_expect_tx(&v_full[vs], C::kTileBytes);
                 for (int h = 0; h < C::kBoxes; ++h)
@@ -874,6 +919,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t0 = static_cast<int>(lane & 3u);
     const int ra = rbase + static_cast<int>(lane >> 2);  // rows of this thread
     const int rb = ra + 8;
+    // kWindow: their tokens.
+    const int token_a = kForm == kWindow ? ra / p.tile_heads : 0;
+    const int token_b = kForm == kWindow ? rb / p.tile_heads : 0;
     const uint32_t lane_addr = static_cast<uint32_t>(rbase) << 16;
     const float c = p.scale_log2;
     Tracer<kTrace> tr(p, 2 + static_cast<int>(warp >> 2), trace_cta && quad == 0 && lane == 0);
@@ -912,10 +960,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int lim_a, lim_b;        // keys below these are visible to rows a and b,
       int low_a = 0, low_b = 0;  // kWindow: from these on (or before the sinks' end)
       if constexpr (kForm == kWindow) {
-        lim_a = min(it.kv_len, it.off + it.row0 + ra + 1);
-        lim_b = min(it.kv_len, it.off + it.row0 + rb + 1);
-        low_a = it.off + it.row0 + ra - p.window + 1;
-        low_b = it.off + it.row0 + rb - p.window + 1;
+        lim_a = min(it.kv_len, it.off + it.row0 + token_a + 1);
+        lim_b = min(it.kv_len, it.off + it.row0 + token_b + 1);
+        low_a = it.off + it.row0 + token_a - p.window + 1;
+        low_b = it.off + it.row0 + token_b - p.window + 1;
       } else {
         lim_a = p.causal ? min(p.Skv, it.row0 + ra + p.causal_off + 1) : p.Skv;
         lim_b = p.causal ? min(p.Skv, it.row0 + rb + p.causal_off + 1) : p.Skv;
@@ -943,7 +991,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         have_s = false;
         tr(kEvSmLdDone, warp >> 2, tt);
         float* s = reinterpret_cast<float*>(sr);
-        const int kbase = kv_tile(it, j) * kBN;
+        const int kbase = kv_key(it, j);
         bool masked = kbase + kBN > it.min_lim;  // uniform across the tile
         if constexpr (kForm == kWindow)
           masked |= kbase < it.top_lo && kbase + kBN > p.sinks;
@@ -1067,13 +1115,17 @@ __global__ void __launch_bounds__(kThreads, 1)
               };
               const int at = kbase + 2 * t0;
               const int va = lim_a - at, vb = lim_b - at, wa = low_a - at, wb = low_b - at;
-              const int sk = p.sinks - at;
-              const bool sinks_only = kbase + kBN <= it.lo;
+              // Sinks among the tile's keys: below sk (of a tile that holds them
+              // in its first rows, by column).
+              const bool sinks_only = j < it.n_sink, folded = it.fold && j == 0;
+              const int sk = p.sinks - (folded ? 2 * t0 : at);
               if (sinks_only || kbase >= it.top_lo) {
                 const int ua = sinks_only ? min(va, sk) : va, ub = sinks_only ? min(vb, sk) : vb;
                 hide([&](int u) { return u < ua; }, [&](int u) { return u < ub; });
-              } else if (kbase + kBN <= it.min_lim && kbase >= p.sinks) {
-                hide([&](int u) { return u >= wa; }, [&](int u) { return u >= wb; });
+              } else if (kbase + kBN <= it.min_lim && (folded || kbase >= p.sinks)) {
+                const int fs = folded ? sk : 0;  // (2 t0 + u < kFold: only u < kFold)
+                hide([&](int u) { return u >= wa || (u < kFold && u < fs); },
+                     [&](int u) { return u >= wb || (u < kFold && u < fs); });
               } else {
                 hide([&](int u) { return u < va && (u >= wa || u < sk); },
                      [&](int u) { return u < vb && (u >= wb || u < sk); });
@@ -1156,7 +1208,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (kForm == kWindow) {
           // Zero the V rows of keys that no row of the item sees: eight warps,
           // two threads to a row, before this warp's P is published.
-          if (ok && (kbase + kBN > it.hi || (kbase < it.lo && kbase + kBN > it.se))) {
+          const bool folded = it.fold && j == 0;
+          const int end = j < it.n_sink ? it.se : it.hi;  // of the tile's live keys
+          if (ok && (kbase + kBN > end || (folded && it.se < kFold))) {
             const int vs = tt % C::kVStages;
             // With fewer V stages than S buffers the stage may still hold
             // V(tt - kVStages), and its barrier's parity could not tell.
@@ -1166,7 +1220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = ok && warp_wait(&v_full[vs], static_cast<uint32_t>(tt / C::kVStages) & 1u,
                                  kSiteVFull);
             const int row = static_cast<int>(threadIdx.x >> 1), key = kbase + row;
-            if (ok && (key >= it.hi || (key < it.lo && key >= it.se))) {
+            if (ok && (folded && row < kFold ? row >= it.se : key >= end)) {
               const uint32_t at = smem_u32(v_buf + vs * C::kVTileBytes) +
                                   static_cast<uint32_t>(row * 128 + (threadIdx.x & 1) * 64);
 #pragma unroll
@@ -1292,8 +1346,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       bool store = true;  // this unit stores the O tile
       if constexpr (kForm == kWindow) {
-        if (p.lse && it.row0 + row < p.Sq)
-          p.lse[(static_cast<int64_t>(it.b) * p.Hq + it.hq) * p.Sq + it.row0 + row] =
+        const int token = row / p.tile_heads, head = it.hq + row - token * p.tile_heads;
+        if (p.lse && token < p.tile_tokens && it.row0 + token < p.Sq)
+          p.lse[(static_cast<int64_t>(it.b) * p.Hq + head) * p.Sq + it.row0 + token] =
               have_o && ml.y > 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : -INFINITY;
       }
       if constexpr (kForm == kPrefix) {
@@ -1458,7 +1513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (store && it.row0 < p.Sq) {
           for (int b = 0; b < C::kBoxes; ++b) {
             if constexpr (kForm == kWindow)
-              tma_store_4d_hint(&o_map, obuf + b * C::kBoxBytes, b * 64, it.row0, it.hq, it.b,
+              tma_store_4d_hint(&o_map, obuf + b * C::kBoxBytes, b * 64, it.hq, it.row0, it.b,
                                 pol_o);
             else
               tma_store_3d_hint(&o_map, obuf + b * C::kBoxBytes, b * 64, it.row0, it.zq, pol_o);

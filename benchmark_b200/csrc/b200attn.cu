@@ -451,7 +451,7 @@ b200_status launch_cpair(const CUtensorMap& qm, const CUtensorMap& km, const CUt
   p.n_items = static_cast<int>(units);
   p.nsplit = 1;
   return launch_cluster2(kernel, C::kSmemBytes, units, stream, "attention_fwd launch (CTA pairs)",
-                         qm, km, vm, om, p);
+                         qm, km, vm, om, p, b200::attn::NoFold{});
 }
 
 template <int D, int EMU, bool TRACE = false>
@@ -563,7 +563,7 @@ b200_status launch_attention(const void* q, const void* k, const void* v, void* 
   }
   // Persistent: one CTA per SM (shared memory admits one), or fewer items.
   const int grid = static_cast<int>(std::min<long long>(items, sm_count()));
-  kernel<<<grid, b200::attn::kThreads, C::kSmemBytes, stream>>>(qm, km, vm, om, p);
+  kernel<<<grid, b200::attn::kThreads, C::kSmemBytes, stream>>>(qm, km, vm, om, p, b200::attn::NoFold{});
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "attention_fwd launch");
   return B200_OK;

@@ -239,28 +239,54 @@ int row_tiles_of(int64_t rows) {
   return static_cast<int>((rows + b200::split::kRows - 1) / b200::split::kRows);
 }
 
-// Work of the 16-row kernel, in us at the rate it was measured at with the GPU
-// full (keys x units per us; a unit is a 16-row tile of one kv head).
-double split_us(int64_t units, int64_t keys, int D) {
-  return static_cast<double>(units) * static_cast<double>(keys) / (D == 128 ? 23400.0 : 36400.0);
+// A 128-row tile of a window call: heads of one kv head x tokens.
+struct WindowTile {
+  int heads, tokens;
+  int64_t key_tiles, items;  // tiles of 128 keys of an item, at most; items
+};
+
+// Of the group's divisors the one with the least work: few tokens reach few keys
+// beyond the window, but heads x tokens may fall short of 128.  A map cannot
+// hold several heads of a broadcast axis (q null: it is none).
+WindowTile window_tile(const WindowShape& s, const b200_tensor* q) {
+  const int group = s.Hq / s.Hkv;
+  const int most = q && s.Hq > 1 && q->stride_h == 0 ? 1 : std::min(group, b200::attn::kBM);
+  const bool folded = s.sinks <= b200::attn::kFold;
+  WindowTile best{};
+  for (int heads = 1; heads <= most; ++heads) {
+    if (group % heads != 0) continue;
+    WindowTile t{heads, b200::attn::kBM / heads, 0, 0};
+    const int64_t reach = static_cast<int64_t>(s.window) + std::min(t.tokens, s.Sq) - 1 +
+                          (s.sinks > 0 && folded ? b200::attn::kFold : 0);
+    t.key_tiles = (std::min<int64_t>(s.Skv, reach) + 127) / 128 +
+                  (folded || reach >= s.Skv ? 0 : (s.sinks + 127) / 128);
+    t.items = static_cast<int64_t>(s.B) * (s.Hq / heads) * ((s.Sq + t.tokens - 1) / t.tokens);
+    if (best.heads == 0 || t.key_tiles * t.items < best.key_tiles * best.items) best = t;
+  }
+  return best;
 }
 
 // Whether a window call goes by 128-row tiles: by the time of each kernel's
-// work, since both start alike (about 7 us).  A 128-row tile spends about 1 us
-// on 128 keys, whatever its rows; the 16-row kernel splits the keys, so that
-// few rows fill the GPU.  Measured (us, 16-row / 128-row): B 1, heads 32/8,
-// window 1024, Sq 64: 15.5 / 18.9, Sq 128: 19.6 / 18.8; B 8, 8192 keys, Sq 16:
-// 107 / 124, Sq 32: 210 / 125; D 64, B 8, window 1024, Sq 32: 24.5 / 32.3,
-// Sq 64: 44.0 / 32.3.
+// work, neither below its bytes'.  The 16-row kernel does 16,500 (D 64: 21,500)
+// keys x units a us with the GPU full; it splits the keys, so that few rows fill
+// the GPU.  A 128-row tile spends about 0.87 us on 128 keys, whatever its rows,
+// and starts 1.5 us later.  Measured (us, 16-row / 128-row; heads 32/8 of 128):
+// B 1, window 1024, Sq 32: 12.5 / 15.5, 64: 16.7 / 15.7, 128: 22.8 / 15.9; B 8,
+// 8192 keys, Sq 4: 46.3 / 62.4, 8: 70.5 / 62.7, 16: 128 / 62.7; B 1, 32768 keys,
+// Sq 32: 131 / 221, 64: 251 / 223; B 16, window 128, Sq 8: 8.4 / 10.5, 16: 14.9 /
+// 10.5; D 64, B 8, window 1024, Sq 8: 13.1 / 14.7, 16: 16.7 / 15.0; B 64, heads
+// 64/8, window 4096, Sq 2: 158 / 177, 4: 267 / 178.
 bool window_by_tiles(const WindowShape& s) {
   const int64_t rows = static_cast<int64_t>(s.Hq / s.Hkv) * s.Sq;
-  const int64_t reach = static_cast<int64_t>(s.window) + s.sinks;
-  const int64_t units = static_cast<int64_t>(s.B) * s.Hkv * row_tiles_of(rows);
-  const int64_t items = static_cast<int64_t>(s.B) * s.Hq * ((s.Sq + 127) / 128);
-  const int64_t sms = sm_count(), rounds = (items + sms - 1) / sms;
-  const double tiles_us =
-      static_cast<double>(rounds * (std::min<int64_t>(s.Skv, reach + 127) / 128 + 1));
-  return split_us(units, std::min<int64_t>(s.Skv, reach), s.D) > tiles_us;
+  const double keys = static_cast<double>(
+      std::min<int64_t>(s.Skv, static_cast<int64_t>(s.window) + s.sinks));
+  const double heads = static_cast<double>(s.B) * s.Hkv;
+  const double bytes_us = 4.0 * heads * keys * s.D / 6.4e6;
+  const double split_us = heads * row_tiles_of(rows) * keys / (s.D == 128 ? 16500.0 : 21500.0);
+  const WindowTile t = window_tile(s, nullptr);
+  const int64_t sms = sm_count(), rounds = (t.items + sms - 1) / sms;
+  const double tiles_us = 0.87 * static_cast<double>(rounds * t.key_tiles) + 1.5;
+  return std::max(split_us, bytes_us) > std::max(tiles_us, bytes_us);
 }
 
 size_t part_bytes(int64_t rows, int D) {
@@ -385,10 +411,28 @@ b200_status encode_view(CUtensorMap* map, const b200_tensor* t, int B, int H, in
   return encode_bf16_4d(map, t->data, d, s, box);
 }
 
+// Map of the queries' tensor with boxes of heads x tokens rows, heads innermost.
+// An axis that is broadcast as in encode_view; heads is 1 where that one is.
+b200_status encode_rows(CUtensorMap* map, const b200_tensor* t, int B, int H, int S, int D,
+                        int heads, int tokens, int* mul_b, int* mul_h) {
+  const bool wide_b = B > 1 && t->stride_b != 0, wide_h = H > 1 && t->stride_h != 0;
+  *mul_b = wide_b;
+  *mul_h = wide_h;
+  const cuuint64_t any = static_cast<cuuint64_t>(D) * 2;  // stride of an axis of extent 1
+  const cuuint64_t d[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(wide_h ? H : 1),
+                           static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(wide_b ? B : 1)};
+  const cuuint64_t s[3] = {wide_h ? static_cast<cuuint64_t>(t->stride_h) * 2 : any,
+                           S > 1 ? static_cast<cuuint64_t>(t->stride_s) * 2 : any,
+                           wide_b ? static_cast<cuuint64_t>(t->stride_b) * 2 : any};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(tokens),
+                             1};
+  return encode_bf16_4d(map, t->data, d, s, box);
+}
+
 template <int D, int kForm>
 b200_status launch_tiles(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
                          const CUtensorMap& om, b200::attn::Params p, long long items, int sms,
-                         cudaStream_t stream) {
+                         cudaStream_t stream, const b200::attn::FoldOf<kForm>& fold) {
   using C = b200::attn::Cfg<D>;
   static unsigned attr_done = 0;
   auto kernel = b200::attn::attention_fwd_kernel<D, D == 128 ? kDefaultEmuD128 : kDefaultEmuD64,
@@ -408,7 +452,8 @@ b200_status launch_tiles(const CUtensorMap& qm, const CUtensorMap& km, const CUt
   p.n_items = static_cast<int>(items);
   const int grid = static_cast<int>(std::min<long long>(items, sms));
   return launch_dependent(kernel, static_cast<unsigned>(grid), b200::attn::kThreads,
-                          C::kSmemBytes, stream, "attention tiles launch", qm, km, vm, om, p);
+                          C::kSmemBytes, stream, "attention tiles launch", qm, km, vm, om, p,
+                          fold);
 }
 
 b200::attn::Params tile_params(const WindowShape& s) {
@@ -432,13 +477,28 @@ b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, cons
   CUtensorMap qm, km, vm, om;
   int one;
   b200_status st;
-  constexpr uint32_t kRows = b200::attn::kBM, kKeys = b200::attn::kBN;
-  if ((st = encode_view(&qm, q, s.B, s.Hq, s.Sq, D, kRows, &p.q_mb, &p.q_mh)) != B200_OK ||
+  const WindowTile t = window_tile(s, q);
+  p.tile_heads = t.heads;
+  p.tile_tokens = t.tokens;
+  b200::attn::FoldMaps fold;
+  constexpr uint32_t kKeys = b200::attn::kBN, kFold = b200::attn::kFold;
+  if ((st = encode_rows(&qm, q, s.B, s.Hq, s.Sq, D, t.heads, t.tokens, &p.q_mb, &p.q_mh)) !=
+          B200_OK ||
+      (st = encode_rows(&om, o, s.B, s.Hq, s.Sq, D, t.heads, t.tokens, &one, &one)) != B200_OK ||
       (st = encode_view(&km, k, s.B, s.Hkv, s.Skv, D, kKeys, &p.k_mb, &p.k_mh)) != B200_OK ||
-      (st = encode_view(&vm, v, s.B, s.Hkv, s.Skv, D, kKeys, &p.v_mb, &p.v_mh)) != B200_OK ||
-      (st = encode_view(&om, o, s.B, s.Hq, s.Sq, D, kRows, &one, &one)) != B200_OK)
+      (st = encode_view(&vm, v, s.B, s.Hkv, s.Skv, D, kKeys, &p.v_mb, &p.v_mh)) != B200_OK)
     return st;
-  p.n_qtiles = (s.Sq + b200::attn::kBM - 1) / b200::attn::kBM;
+  fold.k_sinks = fold.k_rest = km;  // not used without sinks
+  fold.v_sinks = fold.v_rest = vm;
+  if (s.sinks > 0 && s.sinks <= static_cast<int>(kFold)) {
+    const CUtensorMap* const maps[2][2] = {{&fold.k_sinks, &fold.k_rest},
+                                           {&fold.v_sinks, &fold.v_rest}};
+    for (int i = 0; i < 4; ++i)
+      if ((st = encode_view(const_cast<CUtensorMap*>(maps[i / 2][i % 2]), i < 2 ? k : v, s.B,
+                            s.Hkv, s.Skv, D, i % 2 ? kKeys - kFold : kFold, &one, &one)) != B200_OK)
+        return st;
+  }
+  p.n_qtiles = (s.Sq + t.tokens - 1) / t.tokens;
   p.causal = 1;  // the order of the items, as causal attention's
   // Hidden scores are -inf before the scale: a scale of 0 becomes one that
   // changes no weight of scores below 1e30.
@@ -447,14 +507,15 @@ b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, cons
   p.sinks = s.sinks;
   p.kv_len = kv_len;
   p.lse = lse;
-  const long long planes = static_cast<long long>(s.B) * s.Hq;
+  const long long planes = static_cast<long long>(s.B) * (s.Hq / t.heads);
   // Planes of an ordering group: their K/V in use fit in half of the L2 (as
   // for causal attention).
   const double keys = std::min<double>(s.Skv, static_cast<double>(s.window) + b200::attn::kBM);
-  const long long g = static_cast<long long>(64.0 * (1 << 20) / (4.0 * keys * D)) * p.group;
+  const long long g =
+      static_cast<long long>(64.0 * (1 << 20) / (4.0 * keys * D)) * (p.group / t.heads);
   p.cgroup = static_cast<int>(std::max<long long>(1, std::min<long long>(g, planes)));
   return launch_tiles<D, b200::attn::kWindow>(qm, km, vm, om, p, planes * p.n_qtiles, sm_count(),
-                                              stream);
+                                              stream, fold);
 }
 
 // ---- window attention's gradients ----
@@ -580,6 +641,13 @@ b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* w
   return check_launch("attention_window_bwd sinks");
 }
 
+// Work of the 16-row kernel behind a shared prefix, in us at the rate it was
+// measured at with the GPU full (keys x units per us; a unit is a 16-row tile of
+// one kv head).
+double split_us(int64_t units, int64_t keys, int D) {
+  return static_cast<double>(units) * static_cast<double>(keys) / (D == 128 ? 23400.0 : 36400.0);
+}
+
 // Tiles of the prefix form: whole batches, up to 128 rows.
 struct PrefixTiles {
   int batches, rows, count;  // of a tile; tiles
@@ -622,7 +690,7 @@ b200_status launch_prefix_tiles(const WindowShape& own, int P, const b200_tensor
       (st = encode_view(&vm, v, 1, own.Hkv, P, D, kKeys, &p.v_mb, &p.v_mh)) != B200_OK)
     return st;
   return launch_tiles<D, b200::attn::kPrefix>(
-      qm, km, vm, qm, p, static_cast<long long>(own.Hkv) * t.count * nsplit, sms, stream);
+      qm, km, vm, qm, p, static_cast<long long>(own.Hkv) * t.count * nsplit, sms, stream, {});
 }
 
 // A shared prefix: by 128-row tiles for the whole batch, beside the requests'

@@ -201,7 +201,9 @@ struct TileItem {
   int steps;
   int per_head, t0;             // kKeys: steps of a query head, first 64-query tile
   int first, part;              // kKeys: first step; the part of a divided tile, or -1
-  int se, lo, hi, n_sink, skip;  // queries: as in the forward kernel
+  // queries: they see keys of [0, se) and [lo, hi) only; tile i of keys is i for
+  // the n_sink tiles before the window's and i + skip after them.
+  int se, lo, hi, n_sink, skip;
 };
 
 template <bool kKeys>

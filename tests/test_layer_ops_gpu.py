@@ -178,6 +178,13 @@ WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks, lens
     (1, 32, 8, 1024, 4096, 128, 2000, 1000, None),
     (16, 32, 8, 64, 700, 128, 300, 5, [700] * 8 + [65, 64, 63, 0, 1, 128, 300, 699]),
     (1, 8, 1, 2048, 2048, 128, 256, 130, None),
+    # sinks in the first tile's first rows (up to 8), heads x tokens that fall short of 128
+    (4, 12, 4, 500, 1200, 64, 200, 8, [1200, 500, 777, 300]),
+    (2, 10, 2, 700, 900, 128, 130, 1, None),
+    (2, 14, 2, 600, 2000, 128, 400, 9, [2000, 650]),
+    (2, 48, 1, 130, 1500, 64, 300, 4, None),
+    (2, 192, 1, 40, 700, 128, 100, 7, [700, 41]),
+    (8, 8, 8, 300, 300, 128, 123, 4, [300, 299, 200, 128, 129, 1, 0, 250]),
     # many short units: one to a warp
     (40, 32, 16, 3, 200, 64, 150, 4, [(37 * i) % 201 for i in range(40)]),
     (75, 16, 8, 1, 90, 128, 1 << 40, 0, [(17 * i) % 91 for i in range(75)]),
@@ -237,6 +244,21 @@ def test_window_bwd(case):
         U.check_close(a, w, bound, name)
     again = ops.attention_window_bwd(do, q, k, v, o, lse, W, sinks, kv_len=n)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_of_heads_that_share_one_query(D):
+    """Queries broadcast over the heads and the batch, by stride 0."""
+    g = gen(9)
+    B, Hq, Hkv, Sq, Skv = 8, 16, 4, 300, 900
+    q = randn(g, 1, 1, Sq, D).expand(B, Hq, Sq, D)
+    k, v = randn(g, B, Hkv, Skv, D), randn(g, B, Hkv, Skv, D)
+    seen = U.visible(i32([Skv] * B), Sq, Skv, 200, 6, "cuda")
+    want, bound, _, _ = U.attention(q, k, v, seen)
+    # (A tile holds one head of these, several of a copy: sums of another order.)
+    for x in (q, q.contiguous()):
+        U.check_close(ops.attention_window_fwd(x, k, v, 200, 6), want, bound, "o")
+    ops.check()
 
 
 @pytest.mark.parametrize("Sq", [1, 40, 300])
