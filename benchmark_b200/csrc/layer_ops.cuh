@@ -527,24 +527,46 @@ struct WindowGrads {
 
 int64_t padded_queries(int Sq) { return (static_cast<int64_t>(Sq) + 63) / 64 * 64; }
 
-// How the key tiles that hold sinks are divided: where one of them has more
-// steps than half of an SM's share of the launch, into parts of that size or a
-// window's, up to 8 (their fp32 sums cost 2 x 128 x D floats each).  4096
-// queries, heads 32/8 of 128, window 100, 4 sinks: 353 us undivided, 154 us.
-struct SinkPlan {
+// How the steps of the gradients' first key tiles are divided among CTAs (their
+// fp32 sums cost 2 x 128 x D floats each): those of the tiles that hold sinks,
+// into parts of half of an SM's share of the launch or of a window, or those of
+// all tiles, where they are few; up to 8.  What is left is the longest chain of
+// steps or an SM's share, and, if divided, about 4 steps' time for the sums'
+// kernel.  Measured (us, undivided / divided): heads 32/8 of 128, 4096 queries,
+// window 100, 4 sinks 353 / 154 (sinks); heads 8/1 of 128, causal, 128 queries
+// 26.8 / 23.9, 512: 69.8 / 24.0, 4000: 470 / 134 (all); heads 8/2 of 128, 2000
+// queries, window 256, 4 sinks: 40.2 (sinks) or 51.9 (all).
+struct PartPlan {
   int tiles, parts;  // parts 0: not divided
 };
 
-SinkPlan sink_plan(const WindowShape& s) {
+PartPlan part_plan(const WindowShape& s) {
   const int64_t group = s.Hq / s.Hkv, heads = static_cast<int64_t>(s.B) * s.Hkv;
-  const int64_t tiles = (std::min(s.sinks, s.Skv) + 127) / 128, all = (s.Skv + 127) / 128;
-  if (tiles == 0) return SinkPlan{0, 0};
-  const int64_t most = group * ((s.Sq + 63) / 64);
+  const int64_t sinks = (std::min(s.sinks, s.Skv) + 127) / 128, all = (s.Skv + 127) / 128;
+  const int64_t most = group * ((s.Sq + 63) / 64);  // steps of a tile that all queries see
   const int64_t window = std::min(most, group * ((static_cast<int64_t>(s.window) + 127 + 63) / 64));
-  const int64_t share = heads * (tiles * most + (all - tiles) * window) / sm_count();
-  const int64_t size = std::max(window, share / 2);
-  const int64_t parts = std::min<int64_t>(8, (most + size - 1) / std::max<int64_t>(size, 1));
-  return parts > 1 ? SinkPlan{static_cast<int>(tiles), static_cast<int>(parts)} : SinkPlan{0, 0};
+  const int64_t sms = sm_count();
+  const int64_t share = heads * (sinks * most + (all - sinks) * window) / sms;
+  auto cost = [&](int64_t tiles, int64_t parts) {
+    const int64_t rest = tiles < all ? window : 0, longest = tiles > 0 && sinks > 0 ? most : window;
+    const int64_t waves = tiles < all ? 1 : (heads * tiles * parts + sms - 1) / sms;
+    const int64_t chain = waves * ((longest + parts - 1) / parts + 3);  // 3: a CTA's start
+    return static_cast<double>(std::max({chain, rest, share})) + 4.0 +
+           0.04 * static_cast<double>(heads * tiles * parts);
+  };
+  PartPlan best{0, 0};
+  double least = static_cast<double>(std::max(sinks > 0 ? most : window, share));
+  auto consider = [&](int64_t tiles, int64_t parts) {
+    if (tiles == 0 || parts < 2 || cost(tiles, parts) >= least) return;
+    least = cost(tiles, parts);
+    best = PartPlan{static_cast<int>(tiles), static_cast<int>(parts)};
+  };
+  const int64_t size = std::max<int64_t>(std::max(window, share / 2), 1);
+  consider(sinks, std::min<int64_t>(8, (most + size - 1) / size));
+  for (int64_t waves = 1; waves <= 2; ++waves)
+    consider(all, std::min<int64_t>({8, waves * sms / (heads * all),
+                                     (sinks > 0 ? most : window) / 6}));
+  return best;
 }
 
 size_t window_stat_bytes(const WindowShape& s) {
@@ -552,7 +574,7 @@ size_t window_stat_bytes(const WindowShape& s) {
 }
 
 size_t window_bwd_bytes(const WindowShape& s) {
-  const SinkPlan k = sink_plan(s);
+  const PartPlan k = part_plan(s);
   return window_stat_bytes(s) + static_cast<size_t>(s.B) * s.Hkv * k.tiles * k.parts * 2 *
                                     b200::bwd::kOwn * s.D * sizeof(float);
 }
@@ -567,8 +589,8 @@ b200_status launch_bwd_tiles(const CUtensorMap (&m)[4], b200::bwd::TileParams p,
   if (st != B200_OK) return st;
   p.tiles = (rows + b200::bwd::kOwn - 1) / b200::bwd::kOwn;
   int64_t items = static_cast<int64_t>(p.B) * heads * p.tiles;
-  if (kKeys && p.sink_parts > 0)
-    items += static_cast<int64_t>(p.B) * heads * p.sink_tiles * (p.sink_parts - 1);
+  if (kKeys && p.parts > 0)
+    items += static_cast<int64_t>(p.B) * heads * p.part_tiles * (p.parts - 1);
   if (items > 0x3fffffffll) return fail(B200_EUNSUPPORTED, "attention_window_bwd: too many tiles");
   p.n_items = static_cast<int>(items);
   // Key tiles differ in length (sinks): a CTA each, so that the next one starts
@@ -610,17 +632,16 @@ b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* w
   if ((st = encode_view(&k, t.k, s.B, s.Hkv, s.Skv, D, 128, &k_b, &k_h)) != B200_OK ||
       (st = encode_view(&v, t.v, s.B, s.Hkv, s.Skv, D, 128, &v_b, &v_h)) != B200_OK)
     return st;
-  constexpr int kRowsPerBlock = 4 * 256 / (D / 8);
-  const int64_t blocks = (p.stat_plane + kRowsPerBlock - 1) / kRowsPerBlock;
+  const int64_t blocks = p.stat_plane / b200::bwd::kStatRows;
   if (blocks > 0x7fffffffll)
     return fail(B200_EUNSUPPORTED, "attention_window_bwd: too many query rows");
   b200::bwd::stats_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
       view_of(t.dout), view_of(t.o), t.lse, stats, p.stat_plane, p.sq_pad, s.B, s.Hq, s.Sq);
   if ((st = check_launch("attention_window_bwd statistics")) != B200_OK) return st;
-  const SinkPlan sink = sink_plan(s);
-  p.sink_tiles = sink.tiles;
-  p.sink_parts = sink.parts;
-  p.sink_sums = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
+  const PartPlan plan = part_plan(s);
+  p.part_tiles = plan.tiles;
+  p.parts = plan.parts;
+  p.part_sums = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
                                          window_stat_bytes(s));
   p.out1 = view_of(t.dk);
   p.out2 = view_of(t.dv);
@@ -633,12 +654,12 @@ b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* w
   p.s1_b = k_b, p.s1_h = k_h, p.s2_b = v_b, p.s2_h = v_h;
   if ((st = launch_bwd_tiles<D, false>({q[0], dout[0], k, v}, p, s.Hq, s.Sq, stream)) != B200_OK)
     return st;
-  if (sink.parts == 0) return B200_OK;
+  if (plan.parts == 0) return B200_OK;
   p.out1 = view_of(t.dk);
   p.out2 = view_of(t.dv);
-  const int64_t sums = static_cast<int64_t>(s.B) * s.Hkv * sink.tiles * 2 * b200::bwd::kOwn * D / 4;
-  b200::bwd::sink_sum_kernel<D><<<static_cast<unsigned>((sums + 255) / 256), 256, 0, stream>>>(p);
-  return check_launch("attention_window_bwd sinks");
+  const int64_t sums = static_cast<int64_t>(s.B) * s.Hkv * plan.tiles * 2 * b200::bwd::kOwn * D / 4;
+  b200::bwd::part_sum_kernel<D><<<static_cast<unsigned>((sums + 255) / 256), 256, 0, stream>>>(p);
+  return check_launch("attention_window_bwd sums");
 }
 
 // Work of the 16-row kernel behind a shared prefix, in us at the rate it was

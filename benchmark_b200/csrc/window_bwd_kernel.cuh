@@ -9,10 +9,10 @@
 // and dS = P (dP - delta) as bf16 in TMEM, and those are the A operands of the
 // accumulating products, whose B operands are the streamed tiles again (now
 // read along their rows).  Every output element has one owner that adds in a
-// fixed order: no atomics, equal bits from call to call.  (The key tiles that
-// hold sinks are seen by all later queries.  Where that would be the longest
-// chain of the launch, their steps are divided among sink_parts CTAs, whose
-// fp32 sums sink_sum_kernel adds in order.)
+// fixed order: no atomics, equal bits from call to call.  (Where a key tile's
+// steps would be the longest chain of the launch -- sinks are seen by all later
+// queries, or there are few tiles -- they are divided among `parts` CTAs, whose
+// fp32 sums part_sum_kernel adds in order.)
 //
 // TMEM (all 512 columns at D = 128): kSBufs buffers of S, one of dP, the
 // accumulators.  P and dS overwrite their S.  A step is a chain of signals of
@@ -87,10 +87,10 @@ struct TileParams {
   int B, Hq, Hkv, group, Sq, Skv;
   int tiles;             // owned tiles of a (batch, head)
   int n_items;
-  // kKeys: the first sink_tiles tiles are divided into sink_parts units each
-  // (0: none are), which write [B * Hkv][sink_tiles][sink_parts][dK, dV][128][D].
-  int sink_tiles, sink_parts;
-  float* sink_sums;
+  // kKeys: the first part_tiles tiles are divided into parts units each
+  // (0: none are), which write [B * Hkv][part_tiles][parts][dK, dV][128][D].
+  int part_tiles, parts;
+  float* part_sums;
   int window, sinks;
   float scale, scale_log2;
   // Coordinate factors of broadcast axes (own1, own2, str1, str2; batch, head).
@@ -103,33 +103,37 @@ enum : uint32_t {
 };
 
 // -lse and -delta of every query row, padded with zeros.  D/8 lanes to a row
-// (16 bytes each of dO and O), four rows of each in flight.
+// (16 bytes each of dO and O); a block's rows lie in one (batch, head).
+constexpr int kStatRows = 64;
+
 template <int D>
 __global__ void __launch_bounds__(256)
     stats_kernel(const View dout, const View o, const float* lse, float* stats, int64_t plane,
                  int sq_pad, int B, int Hq, int Sq) {
-  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = 4;
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes, kUnroll = kStatRows / kRows;
   pdl_launch_dependents();
   const int lane = static_cast<int>(threadIdx.x) % kLanes;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kUnroll) +
-                       static_cast<int>(threadIdx.x) / kLanes;
+  const int blocks_s = sq_pad / kStatRows;
+  const int bh = static_cast<int>(blockIdx.x) / blocks_s;
+  const int s0 = (static_cast<int>(blockIdx.x) - bh * blocks_s) * kStatRows +
+                 static_cast<int>(threadIdx.x) / kLanes;
+  const int b = bh / Hq, h = bh - b * Hq;
+  const uint16_t* x_row = dout.row(b, h, s0) + lane * 8;
+  const uint16_t* y_row = o.row(b, h, s0) + lane * 8;
   uint4 x[kUnroll], y[kUnroll];
   float l[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t row = row0 + u * kRows;
     x[u] = y[u] = make_uint4(0u, 0u, 0u, 0u);
     l[u] = 0.0f;
-    const int64_t bh = row / sq_pad, s = row - bh * sq_pad, b = bh / Hq, h = bh - b * Hq;
-    if (row < plane && s < Sq) {
-      x[u] = __ldg(reinterpret_cast<const uint4*>(dout.row(b, h, s)) + lane);
-      y[u] = __ldg(reinterpret_cast<const uint4*>(o.row(b, h, s)) + lane);
-      l[u] = __ldg(lse + bh * Sq + s);
+    if (s0 + u * kRows < Sq) {
+      x[u] = __ldg(reinterpret_cast<const uint4*>(x_row + u * kRows * dout.ss));
+      y[u] = __ldg(reinterpret_cast<const uint4*>(y_row + u * kRows * o.ss));
+      l[u] = __ldg(lse + static_cast<int64_t>(bh) * Sq + s0 + u * kRows);
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t row = row0 + u * kRows;
     const uint32_t a[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
     const uint32_t e[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
     float sum = 0.0f;
@@ -140,9 +144,10 @@ __global__ void __launch_bounds__(256)
     }
 #pragma unroll
     for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    if (lane == 0 && row < plane) {
-      stats[row] = l[u] == -INFINITY ? 0.0f : l[u] * -1.4426950408889634f;
-      stats[plane + row] = -sum;
+    if (lane == 0) {
+      float* dst = stats + static_cast<int64_t>(bh) * sq_pad + s0 + u * kRows;
+      dst[0] = l[u] == -INFINITY ? 0.0f : l[u] * -1.4426950408889634f;
+      dst[plane] = -sum;
     }
   }
 }
@@ -213,13 +218,13 @@ __device__ __forceinline__ TileItem<kKeys> tile_item(const TileParams& p, int k)
   // All (batch, head) of one tile index are adjacent: for keys the first tiles
   // (sinks, seen by most queries) start first, for queries the last ones.
   it.part = -1;
-  if (kKeys && p.sink_parts > 0) {
-    const int divided = p.B * heads * p.sink_tiles * p.sink_parts;
+  if (kKeys && p.parts > 0) {
+    const int divided = p.B * heads * p.part_tiles * p.parts;
     if (k < divided) {
-      it.part = k % p.sink_parts;
-      k /= p.sink_parts;
+      it.part = k % p.parts;
+      k /= p.parts;
     } else {
-      k -= divided - p.B * heads * p.sink_tiles;
+      k -= divided - p.B * heads * p.part_tiles;
     }
   }
   int tile = k / (p.B * heads);
@@ -242,8 +247,8 @@ __device__ __forceinline__ TileItem<kKeys> tile_item(const TileParams& p, int k)
     it.steps = it.per_head * p.group;
     if (it.part >= 0) {
       const int64_t all = it.steps;
-      it.first = static_cast<int>(all * it.part / p.sink_parts);
-      it.steps = static_cast<int>(all * (it.part + 1) / p.sink_parts) - it.first;
+      it.first = static_cast<int>(all * it.part / p.parts);
+      it.steps = static_cast<int>(all * (it.part + 1) / p.parts) - it.first;
     }
   } else {
     const int last = it.off + min(it.r0 + kOwn, p.Sq) - 1;
@@ -687,8 +692,8 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
       }
       float* sums = nullptr;  // a divided tile's row
       if (kKeys && part >= 0)
-        sums = p.sink_sums + ((((static_cast<int64_t>(b) * p.Hkv + h) * p.sink_tiles + r0 / kOwn) *
-                                   p.sink_parts + part) * 2 + second) * (kOwn * D) + row * D + c0;
+        sums = p.part_sums + ((((static_cast<int64_t>(b) * p.Hkv + h) * p.part_tiles + r0 / kOwn) *
+                                   p.parts + part) * 2 + second) * (kOwn * D) + row * D + c0;
       uint32_t w[C::kAccCols / 2];
 #pragma unroll
       for (int cc = 0; cc < C::kAccCols; cc += 16) {
@@ -751,7 +756,7 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
 // dK and dV of the divided tiles: the parts' sums, in part order.  Four columns
 // to a thread.
 template <int D>
-__global__ void __launch_bounds__(256) sink_sum_kernel(const __grid_constant__ TileParams p) {
+__global__ void __launch_bounds__(256) part_sum_kernel(const __grid_constant__ TileParams p) {
   int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int c = static_cast<int>(i % (D / 4)) * 4;
   i /= D / 4;
@@ -759,15 +764,15 @@ __global__ void __launch_bounds__(256) sink_sum_kernel(const __grid_constant__ T
   i /= kOwn;
   const int which = static_cast<int>(i % 2);
   i /= 2;
-  const int tile = static_cast<int>(i % p.sink_tiles);
-  const int64_t bh = i / p.sink_tiles;
+  const int tile = static_cast<int>(i % p.part_tiles);
+  const int64_t bh = i / p.part_tiles;
   const int key = tile * kOwn + row;
   if (bh >= static_cast<int64_t>(p.B) * p.Hkv || key >= p.Skv) return;
-  const float* src = p.sink_sums +
-                     (((bh * p.sink_tiles + tile) * p.sink_parts) * 2 + which) * (kOwn * D) +
+  const float* src = p.part_sums +
+                     (((bh * p.part_tiles + tile) * p.parts) * 2 + which) * (kOwn * D) +
                      row * D + c;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int part = 0; part < p.sink_parts; ++part) {
+  for (int part = 0; part < p.parts; ++part) {
     const float4 x = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(part) * 2 * kOwn * D);
     sum.x += x.x;
     sum.y += x.y;

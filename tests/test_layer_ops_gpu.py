@@ -192,6 +192,9 @@ WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks, lens
     # sinks that many queries see (backward divides their tiles)
     (1, 4, 2, 1500, 1500, 128, 64, 4, None),
     (3, 4, 1, 1000, 1300, 64, 32, 140, [1300, 1000, 30]),
+    # few key tiles (backward divides them all)
+    (2, 8, 1, 450, 900, 64, 1 << 40, 0, [900, 333]),
+    (1, 16, 2, 700, 700, 128, 300, 2, [650]),
 ]
 
 
