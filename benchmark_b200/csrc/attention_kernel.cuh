@@ -71,6 +71,8 @@
 //     no row of the item sees are zeroed in shared memory before the PV product
 //     reads them, since they may hold anything (0 * NaN is NaN); K's need not
 //     be: their scores are replaced.
+//   kWindowSplit: kWindow with an item's key tiles divided among p.nsplit units,
+//     which leave unnormalised O and (m, l) in a workspace.
 //   kPrefix: the queries of a whole batch against one shared K/V.  A tile's
 //     128 rows are a box of (batches, tokens, heads of one kv head) of Q; every
 //     unit takes a share of the keys and leaves unnormalised O and (m, l) in a
@@ -151,7 +153,9 @@ struct Params {
 };
 
 // Forms of the kernel.
-constexpr int kDense = 0, kWindow = 1, kPrefix = 2;
+constexpr int kDense = 0, kWindow = 1, kPrefix = 2, kWindowSplit = 3;
+template <int kForm>
+constexpr bool is_window = kForm == kWindow || kForm == kWindowSplit;
 
 // kWindow: the rows that sinks take in an item's first tile, and the maps of
 // its two parts, kFold and kBN - kFold rows.
@@ -161,7 +165,7 @@ struct FoldMaps {
 };
 struct NoFold {};  // the other forms'
 template <int kForm>
-using FoldOf = std::conditional_t<kForm == kWindow, FoldMaps, NoFold>;
+using FoldOf = std::conditional_t<is_window<kForm>, FoldMaps, NoFold>;
 
 // Clock-trace events (kTrace); names in benchmark_b200/trace.py.
 enum : uint32_t {
@@ -270,7 +274,7 @@ struct Item {
 // kWindow and kPrefix.
 struct FormItem : Item {
   int b, hq, hkv;
-  int split;       // kPrefix
+  int split;       // of the item's key tiles
   // kWindow: rows of the item see keys of [0, se) and [lo, hi) only.  Row r is
   // at position off + row0 + r / tile_heads; keys below top_lo (and past the
   // sinks) are hidden from the last row.  Tile j starts at key 128 j for the
@@ -280,7 +284,9 @@ struct FormItem : Item {
   bool fold;
 };
 
-__device__ __forceinline__ FormItem decode_window_item(const Params& p, int k) {
+template <bool kSplit>
+__device__ __forceinline__ FormItem decode_window_item(const Params& p, int unit) {
+  const int k = kSplit ? unit / p.nsplit : unit;
   const int planes_b = p.Hq / p.tile_heads;  // of a batch row
   const int planes = p.B * planes_b;
   const int per_group = p.cgroup * p.n_qtiles;
@@ -304,8 +310,10 @@ __device__ __forceinline__ FormItem decode_window_item(const Params& p, int k) {
   it.fold = it.se > 0 && it.se <= kFold;
   it.n_sink = it.fold ? 0 : (it.se + kBN - 1) / kBN;
   it.base = it.fold ? it.lo - kFold : it.lo;
-  it.n = it.n_sink + (it.hi - it.base + kBN - 1) / kBN;
-  it.j0 = 0;
+  const int n_all = it.n_sink + (it.hi - it.base + kBN - 1) / kBN;
+  it.split = kSplit ? unit - k * p.nsplit : 0;
+  it.j0 = kSplit ? n_all * it.split / p.nsplit : 0;
+  it.n = kSplit ? n_all * (it.split + 1) / p.nsplit - it.j0 : n_all;
   it.top_lo = last - p.window + 1;
   it.min_lim = min(it.kv_len, it.off + it.row0 + 1);
   return it;
@@ -507,8 +515,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int rounds = (p.n_items + units_per_round - 1) / units_per_round;
   auto item_at = [&](int r) { return kPair ? pair_item_index(r) : item_index(p, r); };
   auto decode_at = [&](int k) {
-    if constexpr (kForm == kWindow)
-      return decode_window_item(p, k);
+    if constexpr (is_window<kForm>)
+      return decode_window_item<kForm == kWindowSplit>(p, k);
     else if constexpr (kForm == kPrefix)
       return decode_prefix_item(p, k);
     else
@@ -516,10 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   // First key of an item's K/V tile j.
   auto kv_key = [](const auto& it, int j) {
-    if constexpr (kForm == kWindow)
+    j += it.j0;
+    if constexpr (is_window<kForm>)
       return j < it.n_sink ? j * kBN : it.base + (j - it.n_sink) * kBN;
     else
-      return (it.j0 + j) * kBN;
+      return j * kBN;
   };
   // kWindow: the two parts of a tile that holds sinks, box h.
   auto load_fold = [](uint8_t* dst, const CUtensorMap& sinks, const CUtensorMap& rest,
@@ -632,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int h = 0; h < C::kBoxes; ++h)
                 tma_load_3d_pair(q_buf + qb * C::kTileBytes + h * C::kBoxBytes, &q_map,
                                  lead_bar(&q_full[qb]), h * 64, it.row0, it.zq, pol_q);
-            } else if constexpr (kForm == kWindow) {
+            } else if constexpr (is_window<kForm>) {
               // A box of (64 columns, heads, tokens).
               mbar_arrive_expect_tx(&q_full[qb], static_cast<uint32_t>(C::kBoxes * 128 *
                                                                        p.tile_heads *
@@ -674,14 +683,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               } else if constexpr (kForm != kDense) {
                 mbar_arrive_expect_tx(&k_full[ks], C::kTileBytes);
                 bool folded = false;
-                if constexpr (kForm == kWindow) folded = it.fold && j == 0;
+                if constexpr (is_window<kForm>) folded = it.fold && it.j0 + j == 0;
                 for (int h = 0; h < C::kBoxes; ++h) {
                   uint8_t* dst = k_buf + ks * C::kTileBytes;
                   const int head = it.hkv * p.k_mh, b = it.b * p.k_mb;
                   if (!folded)
                     tma_load_4d(dst + h * C::kBoxBytes, &k_map, &k_full[ks], h * 64,
                                 kv_key(it, j), head, b, pol_kv);
-                  if constexpr (kForm == kWindow) {
+                  if constexpr (is_window<kForm>) {
                     if (folded)
                       load_fold(dst, fold.k_sinks, fold.k_rest, &k_full[ks], h, it.lo, head, b,
                                 pol_kv);
@@ -710,14 +719,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               } else if constexpr (kForm != kDense) {
                 mbar_arrive_expect_tx(&v_full[vs], C::kTileBytes);
                 bool folded = false;
-                if constexpr (kForm == kWindow) folded = it.fold && j == 0;
+                if constexpr (is_window<kForm>) folded = it.fold && it.j0 + j == 0;
                 for (int h = 0; h < C::kBoxes; ++h) {
                   uint8_t* dst = v_buf + vs * C::kTileBytes;
                   const int head = it.hkv * p.v_mh, b = it.b * p.v_mb;
                   if (!folded)
                     tma_load_4d(dst + h * C::kBoxBytes, &v_map, &v_full[vs], h * 64,
                                 kv_key(it, j), head, b, pol_kv);
-                  if constexpr (kForm == kWindow) {
+                  if constexpr (is_window<kForm>) {
                     if (folded)
                       load_fold(dst, fold.v_sinks, fold.v_rest, &v_full[vs], h, it.lo, head, b,
                                 pol_kv);
@@ -920,8 +929,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ra = rbase + static_cast<int>(lane >> 2);  // rows of this thread
     const int rb = ra + 8;
     // kWindow: their tokens.
-    const int token_a = kForm == kWindow ? ra / p.tile_heads : 0;
-    const int token_b = kForm == kWindow ? rb / p.tile_heads : 0;
+    const int token_a = is_window<kForm> ? ra / p.tile_heads : 0;
+    const int token_b = is_window<kForm> ? rb / p.tile_heads : 0;
     const uint32_t lane_addr = static_cast<uint32_t>(rbase) << 16;
     const float c = p.scale_log2;
     Tracer<kTrace> tr(p, 2 + static_cast<int>(warp >> 2), trace_cta && quad == 0 && lane == 0);
@@ -959,7 +968,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tO = tmem_base + lane_addr + C::kColO;
       int lim_a, lim_b;        // keys below these are visible to rows a and b,
       int low_a = 0, low_b = 0;  // kWindow: from these on (or before the sinks' end)
-      if constexpr (kForm == kWindow) {
+      if constexpr (is_window<kForm>) {
         lim_a = min(it.kv_len, it.off + it.row0 + token_a + 1);
         lim_b = min(it.kv_len, it.off + it.row0 + token_b + 1);
         low_a = it.off + it.row0 + token_a - p.window + 1;
@@ -993,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float* s = reinterpret_cast<float*>(sr);
         const int kbase = kv_key(it, j);
         bool masked = kbase + kBN > it.min_lim;  // uniform across the tile
-        if constexpr (kForm == kWindow)
+        if constexpr (is_window<kForm>)
           masked |= kbase < it.top_lo && kbase + kBN > p.sinks;
         float f_a = 1.0f, f_b = 1.0f;
         bool rescale = false;    // this thread's rows
@@ -1093,7 +1102,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           float mx_a, mx_b;
           if (masked) {
-            if constexpr (kForm == kWindow) {
+            if constexpr (is_window<kForm>) {
               // Hidden scores become -inf (scale_log2 is positive), by the one
               // bound that the tile needs where it is one: three comparisons for
               // each score doubled a masked tile's time.
@@ -1117,7 +1126,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int va = lim_a - at, vb = lim_b - at, wa = low_a - at, wb = low_b - at;
               // Sinks among the tile's keys: below sk (of a tile that holds them
               // in its first rows, by column).
-              const bool sinks_only = j < it.n_sink, folded = it.fold && j == 0;
+              const bool sinks_only = it.j0 + j < it.n_sink, folded = it.fold && it.j0 + j == 0;
               const int sk = p.sinks - (folded ? 2 * t0 : at);
               if (sinks_only || kbase >= it.top_lo) {
                 const int ua = sinks_only ? min(va, sk) : va, ub = sinks_only ? min(vb, sk) : vb;
@@ -1190,7 +1199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float nm_a = (m_a == -INFINITY) ? 0.0f : -m_a;
           const float nm_b = (m_b == -INFINITY) ? 0.0f : -m_b;
           // masked scores are pre-scaled (not kWindow's)
-          const float sc = masked && kForm != kWindow ? 1.0f : c;
+          const float sc = masked && !is_window<kForm> ? 1.0f : c;
           // P for keys 0-63 (repeats g = 0..7), then 64-127 (g = 8..15).
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -1205,11 +1214,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           ready_all = __all_sync(0xffffffffu, ready);
           if (rescale_w && j > 0) rescale_o();
         }
-        if constexpr (kForm == kWindow) {
+        if constexpr (is_window<kForm>) {
           // Zero the V rows of keys that no row of the item sees: eight warps,
           // two threads to a row, before this warp's P is published.
-          const bool folded = it.fold && j == 0;
-          const int end = j < it.n_sink ? it.se : it.hi;  // of the tile's live keys
+          const bool folded = it.fold && it.j0 + j == 0;
+          const int end = it.j0 + j < it.n_sink ? it.se : it.hi;  // of the tile's live keys
           if (ok && (kbase + kBN > end || (folded && it.se < kFold))) {
             const int vs = tt % C::kVStages;
             // With fewer V stages than S buffers the stage may still hold
@@ -1345,35 +1354,48 @@ __global__ void __launch_bounds__(kThreads, 1)
                      w[3]);
       };
       bool store = true;  // this unit stores the O tile
-      if constexpr (kForm == kWindow) {
+      // Unnormalised O and (m, l) go to the workspace.
+      constexpr bool partial = kForm == kPrefix || kForm == kWindowSplit;
+      int64_t part = 0;  // this row's place there
+      bool live = false;
+      if constexpr (is_window<kForm>) {
         const int token = row / p.tile_heads, head = it.hq + row - token * p.tile_heads;
-        if (p.lse && token < p.tile_tokens && it.row0 + token < p.Sq)
+        live = token < p.tile_tokens && it.row0 + token < p.Sq;
+        if constexpr (partial)  // [batch, kv head][split][token, head]
+          part = ((static_cast<int64_t>(it.b) * p.Hkv + it.hkv) * p.nsplit + it.split) * p.rows +
+                 (it.row0 + token) * p.group + head - it.hkv * p.group;
+        else if (p.lse && live)
           p.lse[(static_cast<int64_t>(it.b) * p.Hq + head) * p.Sq + it.row0 + token] =
               have_o && ml.y > 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : -INFINITY;
-      }
-      if constexpr (kForm == kPrefix) {
-        // This unit's unnormalised O rows and (m, l), [kv head][split][row].
+      } else if constexpr (kForm == kPrefix) {  // [kv head][split][row]
         const int r_all = it.row0 + row;
-        const bool live = got && row < p.tile_rows && r_all < p.rows;
-        const int64_t at =
-            (static_cast<int64_t>(it.hkv) * p.nsplit + it.split) * p.rows + r_all;
+        live = row < p.tile_rows && r_all < p.rows;
+        part = (static_cast<int64_t>(it.hkv) * p.nsplit + it.split) * p.rows + r_all;
+      }
+      if constexpr (partial) {
+        live = live && got;
 #pragma unroll 1
-        for (int c0 = 0; c0 < (got ? D : 0); c0 += 32) {
+        for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t o[32];
-          tmem_ld32(tO + c0, o);
-          tmem_wait_ld(o);
+          if (have_o) {
+            tmem_ld32(tO + c0, o);
+            tmem_wait_ld(o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
           if (live) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              reinterpret_cast<uint4*>(p.ws_o + at * D + c0)[e] =
+              reinterpret_cast<uint4*>(p.ws_o + part * D + c0)[e] =
                   make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
-        if (live) p.ws_ml[at] = ml;
+        if (live) p.ws_ml[part] = have_o ? ml : make_float2(-INFINITY, 0.0f);
         store = false;
         tc_fence_before();
         mbar_arrive(o_empty);
-      } else if (kPair || kForm == kWindow || p.nsplit == 1) {
+      } else if (kPair || is_window<kForm> || p.nsplit == 1) {
         const float inv = (have_o && ml.y > 0.0f) ? 1.0f / ml.y : 0.0f;
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
@@ -1512,7 +1534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // (A pair's second tile past the last Q row has nothing to store.)
         if (store && it.row0 < p.Sq) {
           for (int b = 0; b < C::kBoxes; ++b) {
-            if constexpr (kForm == kWindow)
+            if constexpr (is_window<kForm>)
               tma_store_4d_hint(&o_map, obuf + b * C::kBoxBytes, b * 64, it.hq, it.row0, it.b,
                                 pol_o);
             else

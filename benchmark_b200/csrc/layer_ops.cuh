@@ -245,6 +245,13 @@ struct WindowTile {
   int64_t key_tiles, items;  // tiles of 128 keys of an item, at most; items
 };
 
+// How a window call goes by 128-row tiles: splits of an item's keys, and the
+// time of its work in us.
+struct TilePlan {
+  int nsplit;
+  double us;
+};
+
 // Of the group's divisors the one with the least work: few tokens reach few keys
 // beyond the window, but heads x tokens may fall short of 128.  A map cannot
 // hold several heads of a broadcast axis (q null: it is none).
@@ -266,27 +273,41 @@ WindowTile window_tile(const WindowShape& s, const b200_tensor* q) {
   return best;
 }
 
+// A 128-row tile spends about 0.87 us on 128 keys, whatever its rows, and the
+// kernel starts 1.5 us after the 16-row one.  Where items leave SMs idle, their
+// keys are split, four tiles at least to a split; the splits' sums and the
+// kernel that merges them cost 4 us and their bytes.  Measured (us, whole /
+// split; B 1, heads 32/8 of 128): 32768 keys, Sq 64: 227 / 43; 8192 keys, Sq 16:
+// 61.0 / 16.2, 256: 62.8 / 43.9, 512: 64.9 / 65.5; window 2048, Sq 64: 22.4 / 16.7;
+// window 1024, Sq 128: 15.9 / 17.2.
+TilePlan tile_plan(const WindowShape& s) {
+  const WindowTile t = window_tile(s, nullptr);
+  const int64_t sms = sm_count();
+  const double rows = static_cast<double>(s.B) * s.Hq * s.Sq;
+  TilePlan best{1, 0.87 * static_cast<double>((t.items + sms - 1) / sms * t.key_tiles) + 1.5};
+  const int64_t ns = std::min<int64_t>({sms / t.items, t.key_tiles / 4, b200::split::kMaxSplits});
+  if (ns < 2) return best;
+  const double us = 0.87 * static_cast<double>((t.key_tiles + ns - 1) / ns) + 5.5 +
+                    8.0 * rows * static_cast<double>(ns) * s.D / 6.4e6;
+  return us < best.us ? TilePlan{static_cast<int>(ns), us} : best;
+}
+
 // Whether a window call goes by 128-row tiles: by the time of each kernel's
 // work, neither below its bytes'.  The 16-row kernel does 16,500 (D 64: 21,500)
 // keys x units a us with the GPU full; it splits the keys, so that few rows fill
-// the GPU.  A 128-row tile spends about 0.87 us on 128 keys, whatever its rows,
-// and starts 1.5 us later.  Measured (us, 16-row / 128-row; heads 32/8 of 128):
-// B 1, window 1024, Sq 32: 12.5 / 15.5, 64: 16.7 / 15.7, 128: 22.8 / 15.9; B 8,
-// 8192 keys, Sq 4: 46.3 / 62.4, 8: 70.5 / 62.7, 16: 128 / 62.7; B 1, 32768 keys,
-// Sq 32: 131 / 221, 64: 251 / 223; B 16, window 128, Sq 8: 8.4 / 10.5, 16: 14.9 /
-// 10.5; D 64, B 8, window 1024, Sq 8: 13.1 / 14.7, 16: 16.7 / 15.0; B 64, heads
-// 64/8, window 4096, Sq 2: 158 / 177, 4: 267 / 178.
-bool window_by_tiles(const WindowShape& s) {
+// the GPU.  Measured (us, 16-row / 128-row; heads 32/8 of 128): B 1, window 1024,
+// Sq 32: 12.5 / 15.5, 64: 16.7 / 15.7, 128: 22.8 / 15.9; B 8, 8192 keys, Sq 4:
+// 46.3 / 62.4, 8: 70.5 / 62.7, 16: 128 / 62.7; B 16, window 128, Sq 8: 8.4 / 10.5,
+// 16: 14.9 / 10.5; D 64, B 8, window 1024, Sq 8: 13.1 / 14.7, 16: 16.7 / 15.0;
+// B 64, heads 64/8, window 4096, Sq 2: 158 / 177, 4: 267 / 178.
+bool window_by_tiles(const WindowShape& s, const TilePlan& t) {
   const int64_t rows = static_cast<int64_t>(s.Hq / s.Hkv) * s.Sq;
   const double keys = static_cast<double>(
       std::min<int64_t>(s.Skv, static_cast<int64_t>(s.window) + s.sinks));
   const double heads = static_cast<double>(s.B) * s.Hkv;
   const double bytes_us = 4.0 * heads * keys * s.D / 6.4e6;
   const double split_us = heads * row_tiles_of(rows) * keys / (s.D == 128 ? 16500.0 : 21500.0);
-  const WindowTile t = window_tile(s, nullptr);
-  const int64_t sms = sm_count(), rounds = (t.items + sms - 1) / sms;
-  const double tiles_us = 0.87 * static_cast<double>(rounds * t.key_tiles) + 1.5;
-  return std::max(split_us, bytes_us) > std::max(tiles_us, bytes_us);
+  return std::max(split_us, bytes_us) > std::max(t.us, bytes_us);
 }
 
 size_t part_bytes(int64_t rows, int D) {
@@ -306,9 +327,12 @@ size_t split_bytes(int64_t rows, const SplitPlan& p, int D) {
 }
 
 WindowPlan window_plan(const WindowShape& s) {
-  if (window_by_tiles(s)) return WindowPlan{true, 1, 0, 0};
   const int64_t rows = static_cast<int64_t>(s.Hq / s.Hkv) * s.Sq;
   const int64_t heads = static_cast<int64_t>(s.B) * s.Hkv;
+  const TilePlan t = tile_plan(s);
+  if (window_by_tiles(s, t))
+    return WindowPlan{true, t.nsplit,
+                      t.nsplit > 1 ? part_bytes(heads * rows * t.nsplit, s.D) : 0, 0};
   const int64_t keys = std::min<int64_t>(s.Skv, static_cast<int64_t>(s.window) + s.sinks);
   const SplitPlan p = split_plan(heads * row_tiles_of(rows), keys, false);
   return WindowPlan{false, p.nsplit, split_bytes(heads * rows, p, s.D), p.units};
@@ -472,8 +496,13 @@ b200::attn::Params tile_params(const WindowShape& s) {
 template <int D>
 b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, const b200_tensor* k,
                                 const b200_tensor* v, const b200_tensor* o, float* lse,
-                                const int32_t* kv_len, cudaStream_t stream) {
+                                const int32_t* kv_len, int nsplit, float* part_o, float2* part_ml,
+                                cudaStream_t stream) {
   b200::attn::Params p = tile_params(s);
+  p.nsplit = nsplit;
+  p.rows = p.group * s.Sq;
+  p.ws_o = part_o;
+  p.ws_ml = part_ml;
   CUtensorMap qm, km, vm, om;
   int one;
   b200_status st;
@@ -514,8 +543,11 @@ b200_status launch_window_tiles(const WindowShape& s, const b200_tensor* q, cons
   const long long g =
       static_cast<long long>(64.0 * (1 << 20) / (4.0 * keys * D)) * (p.group / t.heads);
   p.cgroup = static_cast<int>(std::max<long long>(1, std::min<long long>(g, planes)));
-  return launch_tiles<D, b200::attn::kWindow>(qm, km, vm, om, p, planes * p.n_qtiles, sm_count(),
-                                              stream, fold);
+  const long long items = planes * p.n_qtiles * nsplit;
+  return nsplit > 1 ? launch_tiles<D, b200::attn::kWindowSplit>(qm, km, vm, om, p, items,
+                                                                sm_count(), stream, fold)
+                    : launch_tiles<D, b200::attn::kWindow>(qm, km, vm, om, p, items, sm_count(),
+                                                           stream, fold);
 }
 
 // ---- window attention's gradients ----
@@ -902,14 +934,18 @@ b200_status attention_window_fwd(const b200_tensor* q, const b200_tensor* k, con
   const WindowPlan plan = window_plan(s);
   if ((st = check_workspace(who, workspace, workspace_bytes, plan.bytes)) != B200_OK) return st;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  if (plan.tiles)
-    return D == 128 ? launch_window_tiles<128>(s, q, k, v, o, lse, kv_len, cs)
-                    : launch_window_tiles<64>(s, q, k, v, o, lse, kv_len, cs);
   b200::split::Params p = split_params(s, q, k, v, o, kv_len, plan.nsplit, plan.units);
   p.lse = lse;
   const int64_t rows = static_cast<int64_t>(B) * Hkv * plan.nsplit * p.rows;
   if (plan.bytes > 0) part_pointers(workspace, rows, D, &p.part_o, &p.part_ml);
-  if ((st = D == 128 ? launch_split<128>(p, cs) : launch_split<64>(p, cs)) != B200_OK) return st;
+  if (plan.tiles)
+    st = D == 128 ? launch_window_tiles<128>(s, q, k, v, o, lse, kv_len, plan.nsplit, p.part_o,
+                                             p.part_ml, cs)
+                  : launch_window_tiles<64>(s, q, k, v, o, lse, kv_len, plan.nsplit, p.part_o,
+                                            p.part_ml, cs);
+  else
+    st = D == 128 ? launch_split<128>(p, cs) : launch_split<64>(p, cs);
+  if (st != B200_OK) return st;
   if (plan.bytes == 0) return B200_OK;
   b200::split::CombineParams c{};
   c.o = p.o;

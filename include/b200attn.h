@@ -195,7 +195,7 @@ b200_status qk_norm_rope_bwd(const b200_tensor* dq_out, const b200_tensor* dk_ou
  *   lse: null, or [B, Hq, Sq] fp32 contiguous: the log of each row's sum of
  *   exponentials, -inf for a row that sees nothing (attention_window_bwd
  *   reads it)
- * Sq = 1 is a decoding step; short queries split the keys among CTAs and need
+ * Sq = 1 is a decoding step; few rows split the keys among CTAs and may need
  * a workspace, whose size attention_window_fwd_workspace gives for the
  * current device (0: none).  Calls that may overlap on the GPU need one each.
  */

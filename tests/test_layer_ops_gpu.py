@@ -185,6 +185,11 @@ WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks, lens
     (2, 48, 1, 130, 1500, 64, 300, 4, None),
     (2, 192, 1, 40, 700, 128, 100, 7, [700, 41]),
     (8, 8, 8, 300, 300, 128, 123, 4, [300, 299, 200, 128, 129, 1, 0, 250]),
+    # few tiles over many keys: their keys are split (the last: some splits see none)
+    (1, 8, 2, 200, 9000, 128, 1 << 40, 0, [8700]),
+    (1, 4, 1, 530, 6000, 64, 5000, 4, None),
+    (2, 4, 4, 600, 5000, 128, 4000, 140, [5000, 640]),
+    (2, 12, 4, 333, 7000, 64, 1 << 40, 0, [7000, 30]),
     # many short units: one to a warp
     (40, 32, 16, 3, 200, 64, 150, 4, [(37 * i) % 201 for i in range(40)]),
     (75, 16, 8, 1, 90, 128, 1 << 40, 0, [(17 * i) % 91 for i in range(75)]),
