@@ -268,7 +268,8 @@ WindowTile window_tile(const WindowShape& s, const b200_tensor* q) {
     t.key_tiles = (std::min<int64_t>(s.Skv, reach) + 127) / 128 +
                   (folded || reach >= s.Skv ? 0 : (s.sinks + 127) / 128);
     t.items = static_cast<int64_t>(s.B) * (s.Hq / heads) * ((s.Sq + t.tokens - 1) / t.tokens);
-    if (best.heads == 0 || t.key_tiles * t.items < best.key_tiles * best.items) best = t;
+    auto work = [](const WindowTile& x) { return static_cast<double>(x.key_tiles) * x.items; };
+    if (best.heads == 0 || work(t) < work(best)) best = t;
   }
   return best;
 }
@@ -284,7 +285,8 @@ TilePlan tile_plan(const WindowShape& s) {
   const WindowTile t = window_tile(s, nullptr);
   const int64_t sms = sm_count();
   const double rows = static_cast<double>(s.B) * s.Hq * s.Sq;
-  TilePlan best{1, 0.87 * static_cast<double>((t.items + sms - 1) / sms * t.key_tiles) + 1.5};
+  const double rounds = static_cast<double>((t.items + sms - 1) / sms);
+  TilePlan best{1, 0.87 * rounds * static_cast<double>(t.key_tiles) + 1.5};
   const int64_t ns = std::min<int64_t>({sms / t.items, t.key_tiles / 4, b200::split::kMaxSplits});
   if (ns < 2) return best;
   const double us = 0.87 * static_cast<double>((t.key_tiles + ns - 1) / ns) + 5.5 +
@@ -578,7 +580,9 @@ PartPlan part_plan(const WindowShape& s) {
   const int64_t most = group * ((s.Sq + 63) / 64);  // steps of a tile that all queries see
   const int64_t window = std::min(most, group * ((static_cast<int64_t>(s.window) + 127 + 63) / 64));
   const int64_t sms = sm_count();
-  const int64_t share = heads * (sinks * most + (all - sinks) * window) / sms;
+  const double steps = static_cast<double>(heads) * (static_cast<double>(sinks) * most +
+                                                     static_cast<double>(all - sinks) * window);
+  const int64_t share = static_cast<int64_t>(std::min(steps / sms, 1e15));
   auto cost = [&](int64_t tiles, int64_t parts) {
     const int64_t rest = tiles < all ? window : 0, longest = tiles > 0 && sinks > 0 ? most : window;
     const int64_t waves = tiles < all ? 1 : (heads * tiles * parts + sms - 1) / sms;

@@ -87,6 +87,19 @@ def test_window_bwd_workspace():
     assert L.attention_window_bwd_workspace(1, 8, 2, 1, 1, 128, 1, 0, None) == 1
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Skv", [
+    (1 << 10, 1 << 20, 1 << 20, 1 << 30, 1 << 30), (1, 1 << 10, 1, 1 << 20, 1 << 30),
+    (1 << 30, 1, 1, 1 << 30, 1 << 30), (1, 1, 1, 1, 1 << 30)])
+def test_workspaces_of_the_largest_shapes(B, Hq, Hkv, Sq, Skv):
+    """The plans of shapes that no memory holds are formed without overflow."""
+    L, n = _lib.lib(), ctypes.c_size_t()
+    for window in (1, 1 << 30):
+        args = (B, Hq, Hkv, Sq, Skv, 128, window, 4, ctypes.byref(n))
+        assert L.attention_window_fwd_workspace(*args) == 0 and n.value < 1 << 30
+        assert L.attention_window_bwd_workspace(*args) == 0
+        assert n.value >= 8 * B * Hq * Sq
+
+
 def rope(q=None, k=None, qo=None, ko=None, wq=256, wk=256, freq=256, R=128, pos=256, pos_sb=0,
          eps=1e-6, B=2, S=16, Hq=8, Hkv=2, D=128):
     t = [T() if x is None else x for x in (q, k, qo, ko)]
