@@ -625,3 +625,46 @@ def test_calls_read_the_small_inputs_that_were_written_before_them():
         got = step()
         assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2]))
     ops.check()
+
+
+def test_captured_behind_copies_and_on_forked_streams():
+    """A graph whose calls follow a copy, a fill and another stream's call, replayed with
+    new inputs."""
+    g = gen(33)
+    B, Hq, Hkv, S, D = 3, 8, 2, 700, 128
+    src = [[randn(g, B, h, S, D) for h in (Hq, Hkv, Hkv)] for _ in range(2)]
+    q, k, v = (torch.empty_like(t) for t in src[0])
+    stage = [torch.empty_like(t) for t in src[0]]
+    w, f = torch.ones(D, device="cuda"), torch.rand(64, device="cuda")
+    pos = torch.arange(S, device="cuda", dtype=torch.int32)
+
+    def step(side):
+        for t, x in zip((q, k, v), stage):
+            t.copy_(x)
+        qr, kr = ops.qk_norm_rope(q, k, w, w, f, pos)
+        lse = torch.zeros(B, Hq, S, device="cuda")
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            one = ops.attention_window_fwd(qr[:, :, -1:], kr, v, 300, 4)
+            pre = ops.attention_shared_prefix(qr[:, :, -1:], kr[0], v[0], kr, v)
+        o = ops.attention_window_fwd(qr, kr, v, 300, 4, lse=lse)
+        torch.cuda.current_stream().wait_stream(side)
+        return (one, pre, o, lse, *ops.attention_window_bwd(o, qr, kr, v, o, lse, 300, 4))
+
+    def load(x):
+        for t, y in zip(stage, x):
+            t.copy_(y)
+    side = torch.cuda.Stream()
+    want = []
+    for x in src:
+        load(x)
+        want.append([t.clone() for t in step(side)])
+        torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(side)
+    for i in (0, 1, 0, 1, 1):
+        load(src[i])
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+    ops.check()
