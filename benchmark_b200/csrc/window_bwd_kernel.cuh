@@ -63,8 +63,8 @@ struct TileCfg {
   static constexpr int kRing2Off = kRingOff + kStages1 * kStrBytes;
   static constexpr int kStatOff = kRing2Off + kStages2 * kStrBytes;
   static constexpr int kBarOff = kStatOff + kStages2 * kStatBytes;
-  // own_full own_empty p_free[3] sd_ready dp_free p_ready[2] acc_full acc_empty drain
-  static constexpr int kNumBars = 12 + 2 * (kStages1 + kStages2);
+  // own_full own_empty p_free[3] sd_ready dp_free p_ready[3] acc_full acc_empty drain
+  static constexpr int kNumBars = 13 + 2 * (kStages1 + kStages2);
   static constexpr int kSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kSlotOff + 16 + 1024;  // + alignment slack
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
@@ -327,8 +327,8 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   float* stat = reinterpret_cast<float*>(smem + C::kStatOff);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
   uint64_t *own_full = bars, *own_empty = bars + 1, *p_free = bars + 2, *sd_ready = bars + 5,
-           *dp_free = bars + 6, *p_ready = bars + 7, *acc_full = bars + 9,
-           *acc_empty = bars + 10, *drain = bars + 11, *full1 = bars + 12,
+           *dp_free = bars + 6, *p_ready = bars + 7, *acc_full = bars + 10,
+           *acc_empty = bars + 11, *drain = bars + 12, *full1 = bars + 13,
            *empty1 = full1 + C::kStages1, *full2 = empty1 + C::kStages1,
            *empty2 = full2 + C::kStages2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kSlotOff);
@@ -337,12 +337,15 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(own_full, 1);
     mbar_init(own_empty, 1);
-    for (int i = 0; i < 3; ++i) mbar_init(&p_free[i], 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&p_free[i], 1);
+      // One for each S buffer: the elementwise warps may be as many steps ahead of
+      // the accumulating one as there are buffers, but a buffer's next P waits for
+      // the products that this one's phase admits.
+      mbar_init(&p_ready[i], C::kWarps);
+    }
     mbar_init(sd_ready, 1);
     mbar_init(dp_free, C::kWarps);
-    // Two: a warp may be a step ahead of another, but not two (dP's buffer).
-    mbar_init(&p_ready[0], C::kWarps);
-    mbar_init(&p_ready[1], C::kWarps);
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, C::kWarps);
     mbar_init(drain, 2);
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
           mma_commit_warp(sd_ready);
           if (i + 1 == steps) mma_commit_warp(own_empty);
         } else {
-          ok = warp_wait(&p_ready[t & 1], static_cast<uint32_t>(t >> 1) & 1u, kSiteBwdP);
+          ok = warp_wait(&p_ready[sb], static_cast<uint32_t>(t / C::kSBufs) & 1u, kSiteBwdP);
           if (!ok) break;
           if constexpr (kKeys) {
 #pragma unroll
@@ -620,7 +623,8 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
         }
         tc_fence_after();
         uint32_t s[C::kCols], d[C::kCols];
-        const uint32_t t_s = tlane + static_cast<uint32_t>(sb * C::kN);
+        const int buf = sb;
+        const uint32_t t_s = tlane + static_cast<uint32_t>(buf * C::kN);
         if (++sb == C::kSBufs) sb = 0;
         ld_cols(t_s + col0, s);
         ld_cols(tlane + C::kColDp + col0, d);
@@ -668,7 +672,7 @@ __global__ void __launch_bounds__(TileCfg<D, kKeys>::kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_warp(&p_ready[t & 1]);
+        mbar_arrive_warp(&p_ready[buf]);
         if constexpr (kKeys) {
           str0 += 64;
           if (++head_i == it.per_head) {
