@@ -60,9 +60,9 @@ constexpr int kLOff = kVOff + kVStages * kTileBytes;  // (m, l) [pipe][128]
 constexpr int kFlagOff = kLOff + 2 * 128 * 8;          // abort flag (epilogue)
 constexpr int kBarOff = kFlagOff + 16;
 // q_full[2][2] q_empty[2][2] k_full[K] k_empty[K] v_full[V] v_empty[V]
-// s_ready[2][3] p_ready[3] p_free[3] o_full[2] o_empty[2] l_ready[2]
+// s_ready[2][3] p_ready[2][3] p_free[3] o_full[2] o_empty[2] l_ready[2]
 // drain done
-constexpr int kNumBars = 8 + 2 * kKStages + 2 * kVStages + 4 * kSBufs + 6 + 2;
+constexpr int kNumBars = 8 + 2 * kKStages + 2 * kVStages + 5 * kSBufs + 6 + 2;
 constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
 constexpr int kSmemBytes = kTmemSlotOff + 16 + 1024;  // + 1 KiB alignment slack
 static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
@@ -171,11 +171,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_full = k_empty + kKStages;
   uint64_t* v_empty = v_full + kVStages;
   uint64_t* s_ready = v_empty + kVStages;
-  // [pipe][its tile % kSBufs]: a pipe sees every phase of its own (the B pipe
-  // sits out a unit with one Q tile, and a barrier shared with the A pipe could
-  // be any number of phases behind or ahead when it comes back).
+  // Both [pipe][S buffer]: a pipe sees every phase of its own (the B pipe sits
+  // out a unit with one Q tile, and a barrier shared with the A pipe could be
+  // any number of phases behind or ahead when it comes back).  Who waits keeps
+  // the next phase's bit of each, and one address reaches both from a softmax
+  // warp, whose registers are full: with a count of the pipe's tiles instead
+  // the score loop spilled (48 bytes of loads), 181.4 us against 177.9 (B 8,
+  // 16 heads, 2048 tokens), 778 against 794 TFLOP/s (B 64).
   uint64_t* p_ready = s_ready + 2 * kSBufs;
-  uint64_t* p_free = p_ready + kSBufs;
+  uint64_t* p_free = p_ready + 2 * kSBufs;
   uint64_t* o_full = p_free + kSBufs;   // [pipe]
   uint64_t* o_empty = o_full + 2;       // [pipe]
   uint64_t* l_ready = o_empty + 2;      // [pipe]
@@ -206,6 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s_ready[i], 1);
       mbar_init(&s_ready[kSBufs + i], 1);
       mbar_init(&p_ready[i], 4);  // the pipe's four softmax warps
+      mbar_init(&p_ready[kSBufs + i], 4);
       mbar_init(&p_free[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -329,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       int u = 0, t = 0, lq[2] = {0, 0};
-      int ts_pipe[2] = {0, 0};  // S tiles issued for each pipe
+      uint32_t p_phase = 0;  // bit of each p_ready barrier's next phase
       bool ok = true;
       for (int r = 0; r < rounds && ok; ++r) {
         const int k = unit_index(r);
@@ -355,8 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int kk = 0; kk < D / 16; ++kk)
                 mma_ss_warp(ts, dq + kk * 2, dk + kk * 2, kIdescS, kk > 0 ? 1u : 0u);
-              mma_commit_warp(&s_ready[pp * kSBufs + ts_pipe[pp] % kSBufs]);
-              ++ts_pipe[pp];
+              mma_commit_warp(&s_ready[pp * kSBufs + sb]);
             }
             if (ok) mma_commit_warp(&k_empty[ks]);
           }
@@ -367,11 +371,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int sb = u % kSBufs;
               // V(j), P(u) and, for the unit's first tile, O of the pipe free
               // (the epilogue has read the pipe's previous unit).
+              const int pb = pp * kSBufs + sb;
               ok = wait3(bar(&v_full[vs]), static_cast<uint32_t>(t / kVStages) & 1u,
-                         bar(&p_ready[sb]), static_cast<uint32_t>(u / kSBufs) & 1u,
+                         bar(&p_ready[pb]), (p_phase >> pb) & 1u,
                          j == 0 ? bar(&o_empty[pp]) : dn_a,
                          j == 0 ? (static_cast<uint32_t>(lq[pp] & 1) ^ 1u) : dn_p, kSitePReady);
               if (!ok) break;
+              p_phase ^= 1u << pb;
               tr(kEvMmaPv, pp, u);
               const uint32_t to = tmem_base + kColO + static_cast<uint32_t>(pp * D);
               const uint32_t tp = tmem_base + static_cast<uint32_t>(sb * 128);
@@ -405,7 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tO = tmem_base + lane_addr + kColO + static_cast<uint32_t>(pp * D);
     const float c = p.scale_log2;
     Tracer<kTrace> tr(p, 2 + pp, trace_cta && quad == 0 && lane == 0);
-    int u = 0, tp = 0, lq = 0;  // S tiles of the CTA, tiles of this pipe, its units
+    int u = 0;  // S tiles of the CTA
+    // Phase bits of the next waits: s_ready's (bit of the S buffer), o_empty's.
+    constexpr uint32_t kUnitBit = 1u << kSBufs;
+    uint32_t phases = kUnitBit;
     bool ok = true;
 #pragma unroll 1
     for (int r = 0; r < rounds && ok; ++r) {
@@ -419,13 +428,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY;  // running max of this row (log2 units)
       float l = 0.0f;       // row sum in m
 #pragma unroll 1
-      for (int j = 0; j < n; ++j, ++tp) {
+      for (int j = 0; j < n; ++j) {
         const int uu = u + j * un.nq + pp;
         const int sb = uu % kSBufs;
         const uint32_t tS = tmem_base + lane_addr + static_cast<uint32_t>(sb * 128);
         tr(kEvSmWait, pp, uu);
-        ok = warp_wait(&s_ready[pp * kSBufs + tp % kSBufs], static_cast<uint32_t>(tp / kSBufs) & 1u,
-                       kSiteSReady);
+        ok = warp_wait(&s_ready[pp * kSBufs + sb], (phases >> sb) & 1u, kSiteSReady);
+        phases ^= 1u << sb;
         if (!ok) break;
         tc_fence_after();
         tr(kEvSmReady, pp, uu);
@@ -530,19 +539,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_warp(&p_ready[sb]);
+        mbar_arrive_warp(&p_ready[pp * kSBufs + sb]);
         tr(kEvSmPublished, pp, uu);
       }
       if (!ok) break;
       u += n * un.nq;
       // (m, l) of the unit's rows for the epilogue, once it has read the
       // pipe's previous unit.
-      ok = warp_wait(&o_empty[pp], (static_cast<uint32_t>(lq) & 1u) ^ 1u, kSiteOEmpty);
+      ok = warp_wait(&o_empty[pp], phases >> kSBufs, kSiteOEmpty);
       if (!ok) break;
       stat[pp * 128 + row] = make_float2(m, l);
       __syncwarp();
       mbar_arrive_warp(&l_ready[pp]);
-      ++lq;
+      phases ^= kUnitBit;
     }
   } else {
     setmaxnreg_dec<kEpiRegs>();

@@ -1,13 +1,12 @@
-"""CPU test of the barriers of window attention's gradient pipeline: every wait goes by one
-bit of a barrier's phase, so it is sound only if, while a warp stands at it, the phase before
-the awaited one has passed and the one after cannot.  The steps of one tile are written down
-as events with what must have happened before each; the ring depths, buffers and the indices
-of the p_ready barriers are read from the kernel's source."""
+"""CPU test of the barriers of window attention's gradient pipeline (pipeline_model): the
+steps of a tile, with the ring depths, buffers and the indices of the p_ready barriers read
+from the kernel's source."""
 import re
 from collections import defaultdict
 
 import pytest
 
+import pipeline_model
 from benchmark_b200 import build
 
 SOURCE = (build.CSRC / "window_bwd_kernel.cuh").read_text()
@@ -35,56 +34,19 @@ def p_ready_expressions():
 
 
 def faults(keys, D, index, phase):
-    """Waits that one phase bit does not decide, and arrivals that could meet a phase that
-    is not theirs."""
     n1, n2, bufs = (constant(c, keys, D) for c in ("kStages1", "kStages2", "kSBufs"))
-    names = {"kSBufs": bufs}
-    p_index = [eval(index.replace("C::", ""), dict(names, t=t)) for t in range(STEPS)]
-    p_bit = [eval(phase.replace("C::", "").replace("/", "//"), dict(names, t=t)) & 1
-             for t in range(STEPS)]
-    after = defaultdict(set)   # event -> events that must come before it
-    at, waits = [], []         # events; (at the wait, past it, barrier, phase)
-    arrivals = defaultdict(list)  # (barrier, arriver) -> its arrivals in order
-    bad = []                   # (barrier, phase, what)
-
-    def event(*before):
-        at.append(None)
-        e = len(at) - 1
-        after[e] |= set(b for b in before if b is not None)
-        return e
-
-    class Role:
-        def __init__(self):
-            self.last = None
-            self.done = None  # last completion of its asynchronous work
-
-        def wait(self, bar, m, bit=None):
-            if m >= 0 and bit is not None and bit != m & 1:
-                bad.append((bar, m, "bit"))
-            here = event(self.last)
-            self.last = event(here)
-            waits.append((here, self.last, bar, m))
-
-        def arrive(self, bar, who=0):
-            self.last = event(self.last)
-            arrivals[bar, who].append(self.last)
-
-        def commit(self, bar):  # arrives when the work issued so far is complete
-            self.last = event(self.last)
-            self.done = event(self.last, self.done)
-            arrivals[bar, 0].append(self.done)
-
-    tma, issue, acc = Role(), Role(), Role()
-    quads = [[Role() for _ in range(WARPS)] for _ in range(QUADS)]
+    index, phase = (x.replace("C::", "").replace("/", "//") for x in (index, phase))
+    model = pipeline_model.Pipeline()
+    tma, issue, acc = (model.role() for _ in range(3))
+    quads = [[model.role() for _ in range(WARPS)] for _ in range(QUADS)]
     phases = defaultdict(int)  # of each p_ready barrier so far
     for t in range(STEPS):
         s1, s2, sb = t % n1, t % n2, t % bufs
+        at, bit = (eval(x, {"kSBufs": bufs, "t": t}) for x in (index, phase))
         tma.wait(("empty1", s1), t // n1 - 1)
         tma.commit(("full1", s1))
-        tma.done = None  # copies complete in any order
         tma.wait(("empty2", s2), t // n2 - 1)
         tma.commit(("full2", s2))
-        tma.done = None
         issue.wait(("full1", s1), t // n1)
         issue.wait(("p_free", sb), t // bufs - 1)
         issue.wait(("full2", s2), t // n2)
@@ -97,59 +59,18 @@ def faults(keys, D, index, phase):
                 w.wait(("sd_ready",), t)
                 if keys:
                     w.wait(("full2", s2), t // n2)
-                w.arrive(("dp_free",), id(w))
-            meet = event(*(w.last for w in quad))  # the quadrant's named barrier
+                w.arrive(("dp_free",))
+            model.meet(*quad)
             for w in quad:
-                w.last = meet
                 w.wait(("full1", s1), t // n1)  # rows that nothing sees are zeroed
-                w.arrive(("p_ready", p_index[t]), id(w))
-        acc.wait(("p_ready", p_index[t]), phases[p_index[t]], p_bit[t])
-        phases[p_index[t]] += 1
+                w.arrive(("p_ready", at))
+        acc.wait(("p_ready", at), phases[at], bit & 1)
+        phases[at] += 1
         acc.commit(("empty1", s1))
         if keys:
             acc.commit(("empty2", s2))
         acc.commit(("p_free", sb))
-
-    # A phase is complete with all of its arrivals; a wait is passed after its phase.
-    by_bar = defaultdict(list)
-    for (bar, _), events in arrivals.items():
-        by_bar[bar].append(events)
-    complete = {(bar, m): events for bar, lists in by_bar.items()
-                for m, events in enumerate(zip(*lists))}
-    for here, passed, bar, m in waits:
-        if m >= 0:
-            after[passed] |= set(complete[bar, m])
-    # All that has happened before each event, as bits: earliest events first.
-    left = {e: len(after[e]) for e in range(len(at))}
-    then = defaultdict(list)
-    for e in range(len(at)):
-        for b in after[e]:
-            then[b].append(e)
-    past, ready = {}, [e for e, n in left.items() if n == 0]
-    while ready:
-        e = ready.pop()
-        past[e] = sum({1 << b for b in after[e]}, 0)
-        for b in after[e]:
-            past[e] |= past[b]
-        for x in then[e]:
-            left[x] -= 1
-            if left[x] == 0:
-                ready.append(x)
-    assert len(past) == len(at), "the steps wait for one another in a circle"
-
-    def before(events, e):
-        return all(past[e] >> x & 1 for x in events)
-    for here, passed, bar, m in waits:
-        if m >= 1 and not before(complete[bar, m - 1], here):
-            bad.append((bar, m, "the phase before may not have passed"))
-        after_it = complete.get((bar, m + 1))
-        if after_it and not any(before([passed], e) for e in after_it):
-            bad.append((bar, m, "the phase after may pass first"))
-    for (bar, _), events in arrivals.items():
-        for m, e in enumerate(events[1:]):
-            if not before(complete[bar, m], e):
-                bad.append((bar, m + 1, "an arrival may meet the phase before"))
-    return bad
+    return model.faults()
 
 
 @pytest.mark.parametrize("D", [64, 128])
