@@ -1366,7 +1366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                  (it.row0 + token) * p.group + head - it.hkv * p.group;
         else if (p.lse && live)
           p.lse[(static_cast<int64_t>(it.b) * p.Hq + head) * p.Sq + it.row0 + token] =
-              have_o && ml.y > 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : -INFINITY;
+              have_o && ml.y != 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : -INFINITY;
       } else if constexpr (kForm == kPrefix) {  // [kv head][split][row]
         const int r_all = it.row0 + row;
         live = row < p.tile_rows && r_all < p.rows;

@@ -1,0 +1,55 @@
+"""GPU tests of the attention layer's operators with NaN where queries look: each row that
+sees it is NaN, its log-sum-exp too (-inf is a row that sees nothing), and no other row."""
+import math
+
+import pytest
+import torch
+
+import layer_util as U
+from benchmark_b200 import ops
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+WINDOW = [  # B, Hq, Hkv, Sq, Skv, D, W, sinks
+    (2, 32, 8, 1, 5000, 128, 1024, 4),     # 16-row tiles, a cluster of splits
+    (1, 16, 8, 1, 8192, 64, 1 << 40, 0),   # many splits
+    (40, 32, 16, 3, 200, 64, 150, 4),      # a unit to a warp
+    (6, 8, 2, 300, 517, 128, 128, 4),      # 128-row tiles
+    (4, 16, 4, 260, 1000, 64, 1 << 40, 0),
+    (1, 32, 8, 600, 2000, 64, 700, 20),
+    (1, 8, 2, 200, 9000, 128, 1 << 40, 0),  # their keys split
+    (2, 12, 4, 333, 7000, 64, 1 << 40, 0),
+]
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda").to(BF16)
+
+
+def inputs(case, at):
+    """q, k, v with one NaN among each head's keys, and the rows [B, Hq, Sq] that see it."""
+    B, Hq, Hkv, Sq, Skv, D, W, sinks = case
+    g = torch.Generator(device="cuda").manual_seed(at)
+    q, k, v = randn(g, B, Hq, Sq, D), randn(g, B, Hkv, Skv, D), randn(g, B, Hkv, Skv, D)
+    first = max(0, Skv - Sq - min(W, Skv) + 1)  # the keys that some query may see
+    j = first + (torch.arange(B * Hkv, device="cuda").view(B, Hkv) * 37 + at) % (Skv - first)
+    clean = k.clone()
+    k.scatter_(2, j[:, :, None, None], math.nan)  # column 0 of key j
+    seen = U.visible(torch.full((B,), Skv, device="cuda"), Sq, Skv, W, sinks, "cuda")
+    heads = j.repeat_interleave(Hq // Hkv, dim=1)[:, :, None, None].expand(B, Hq, Sq, 1)
+    hit = seen.expand(B, Hq, Sq, Skv).gather(3, heads).squeeze(3)
+    return q, k, v, clean, hit
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=str)
+def test_lse_of_a_row_that_sees_nan(case):
+    B, Hq, _, Sq, _, _, W, sinks = case
+    for at in (0, 5, 40):
+        q, k, v, clean, hit = inputs(case, at)
+        lse, want = (torch.empty((B, Hq, Sq), device="cuda") for _ in range(2))
+        o = ops.attention_window_fwd(q, k, v, W, sinks, lse=lse)
+        ops.attention_window_fwd(q, clean, v, W, sinks, lse=want)
+        ops.check()
+        assert hit.any() and torch.isnan(lse[o.isnan().any(-1)]).all()
+        assert torch.equal(lse[~hit], want[~hit])
