@@ -435,7 +435,10 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
 // row a, pk[2g+1] row b (the 16x128b store order).  Accumulates fp32 row
 // sums in packed pairs.  kEmu of every 8 pairs use the FMA-pipe exp2
 // (exp2_fma_x2), the rest MUFU; masked blocks use MUFU only (exact zeros).
-template <int kEmu, bool kMasked>
+// kNan: as exp2_fma_x2's.  The forms have it, and are faster with it (d=64, 8192
+// tokens of 32/8 heads, window 1024: 152 -> 148 us); the dense kernels
+// lose 1 % by it (d=64, B 64, 16 heads, 2048 tokens: 1,376 -> 1,389 us).
+template <int kEmu, bool kMasked, bool kNan>
 __device__ __forceinline__ void p_rows(const float* s, float sc, float nm_a, float nm_b,
                                        uint64_t& rs_a, uint64_t& rs_b, uint32_t (&pk)[16]) {
   const uint64_t sc2 = f2_pack(sc, sc);
@@ -450,7 +453,7 @@ __device__ __forceinline__ void p_rows(const float* s, float sc, float nm_a, flo
       float x0, x1, p0, p1;
       f2_unpack(x2, x0, x1);
       if (!kMasked && ((2 * g + rr) & 7) < kEmu) {
-        exp2_fma_x2(x0, x1, p0, p1);
+        exp2_fma_x2<kNan>(x0, x1, p0, p1);
       } else {
         p0 = ex2_approx(x0);
         p1 = ex2_approx(x1);
@@ -1047,7 +1050,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint32_t pk[16];
-            p_rows<kEmu, false>(s + 32 * half, c, -m_a, -m_b, rs_a, rs_b, pk);
+            p_rows<kEmu, false, kForm != kDense>(s + 32 * half, c, -m_a, -m_b, rs_a, rs_b, pk);
             tmem_st_16x128b_x8(tS + 32 * half, pk);
           }
           ready = mbar_try_wait(smem_u32(&s_ready[nb]), static_cast<uint32_t>((tt + 1) / kSBufs) & 1u);
@@ -1093,7 +1096,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
                 uint32_t pk[16];
-                p_rows<kEmu, false>(s + 32 * half, c, -m_a, -m_b, rs_a, rs_b, pk);
+                p_rows<kEmu, false, kForm != kDense>(s + 32 * half, c, -m_a, -m_b, rs_a, rs_b, pk);
                 tmem_st_16x128b_x8(tS + 32 * half, pk);
               }
               rescale_o();
@@ -1205,9 +1208,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int half = 0; half < 2; ++half) {
             uint32_t pk[16];
             if (masked)
-              p_rows<kEmu, true>(s + 32 * half, sc, nm_a, nm_b, rs_a, rs_b, pk);
+              p_rows<kEmu, true, kForm != kDense>(s + 32 * half, sc, nm_a, nm_b, rs_a, rs_b, pk);
             else
-              p_rows<kEmu, false>(s + 32 * half, sc, nm_a, nm_b, rs_a, rs_b, pk);
+              p_rows<kEmu, false, kForm != kDense>(s + 32 * half, sc, nm_a, nm_b, rs_a, rs_b, pk);
             tmem_st_16x128b_x8(tS + 32 * half, pk);
           }
           ready = mbar_try_wait(smem_u32(&s_ready[nb]), static_cast<uint32_t>((tt + 1) / kSBufs) & 1u);

@@ -868,6 +868,18 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
+// max and min that return NaN where either value is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // exp2 of two values on the FMA pipe (inputs clamped to [-125, 126]):
 //   x = j + r with j = round(x) (adding 1.5 * 2^23 leaves round(x) in the low
 //   mantissa bits of t), r in [-0.5, 0.5];  2^r ~ c0 + r(c1 + r(c2 + r c3)),
@@ -877,11 +889,19 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // The clamp keeps the exponent field normal: with j >= -125 and p >= 2^-0.5
 // the sum never reaches the subnormal range (at j = -126 a p just below 1
 // would), and j <= 126 never overflows.  So x < -125 gives 2^-125 (MUFU's
-// ftz form gives 0 below 2^-126) and x > 126 gives 2^126.
+// ftz form gives 0 below 2^-126) and x > 126 gives 2^126.  kNan: NaN stays
+// NaN (else the clamp makes 2^-125 of it), by a clamp that keeps it and a
+// product with 2^j instead of the sum of bits (exact: the same values).
+template <bool kNan = false>
 __device__ __forceinline__ void exp2_fma_x2(float x0, float x1, float& y0, float& y1) {
   const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
-  const uint64_t x =
-      f2_pack(fminf(fmaxf(x0, -125.0f), 126.0f), fminf(fmaxf(x1, -125.0f), 126.0f));
+  auto clamp = [](float v) {
+    if constexpr (kNan)
+      return fmin_nan(fmax_nan(v, -125.0f), 126.0f);
+    else
+      return fminf(fmaxf(v, -125.0f), 126.0f);
+  };
+  const uint64_t x = f2_pack(clamp(x0), clamp(x1));
   const uint64_t t = f2_add(x, magic);
   const uint64_t r = f2_sub(x, f2_sub(t, magic));
   uint64_t p = f2_fma(f2_pack(0.0551716685295105f, 0.0551716685295105f), r,
@@ -889,8 +909,14 @@ __device__ __forceinline__ void exp2_fma_x2(float x0, float x1, float& y0, float
   p = f2_fma(p, r, f2_pack(0.6932609677314758f, 0.6932609677314758f));
   p = f2_fma(p, r, f2_pack(0.9999280571937561f, 0.9999280571937561f));
   float p0, p1, t0, t1;
-  f2_unpack(p, p0, p1);
   f2_unpack(t, t0, t1);
+  if constexpr (kNan) {
+    const float e0 = __uint_as_float(0x3f800000u + (__float_as_uint(t0) << 23));
+    const float e1 = __uint_as_float(0x3f800000u + (__float_as_uint(t1) << 23));
+    f2_unpack(f2_mul(p, f2_pack(e0, e1)), y0, y1);
+    return;
+  }
+  f2_unpack(p, p0, p1);
   y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
   y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }

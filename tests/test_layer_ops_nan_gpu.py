@@ -53,3 +53,31 @@ def test_lse_of_a_row_that_sees_nan(case):
         ops.check()
         assert hit.any() and torch.isnan(lse[o.isnan().any(-1)]).all()
         assert torch.equal(lse[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=str)
+def test_rows_that_see_nan(case):
+    """At head_dim 64 a part of the exponentials goes by a polynomial."""
+    W, sinks = case[6:]
+    for at in range(0, 64, 7):
+        q, k, v, clean, hit = inputs(case, at)
+        o = ops.attention_window_fwd(q, k, v, W, sinks)
+        want = ops.attention_window_fwd(q, clean, v, W, sinks)
+        ops.check()
+        assert o[hit].isnan().all() and torch.equal(o[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,P,S", [(40, 16, 16, 1, 5003, 20), (3, 16, 4, 1, 517, 128)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prefix_with_nan(B, Hq, Hkv, Sq, P, S, D):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, kp, vp = randn(g, B, Hq, Sq, D), randn(g, Hkv, P, D), randn(g, Hkv, P, D)
+    k, v = randn(g, B, Hkv, S, D), randn(g, B, Hkv, S, D)
+    want = ops.attention_shared_prefix(q, kp, vp, k, v)
+    for at in range(0, 64, 7):
+        x = kp.clone()
+        x[Hkv // 2, (at * 71) % P, 3] = math.nan
+        o = ops.attention_shared_prefix(q, x, vp, k, v)
+        ops.check()
+        hit = torch.arange(Hq, device="cuda") // (Hq // Hkv) == Hkv // 2
+        assert o[:, hit].isnan().all() and torch.equal(o[:, ~hit], want[:, ~hit])
