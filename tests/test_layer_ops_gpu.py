@@ -238,6 +238,27 @@ def test_window_fwd(case):
 
 
 @pytest.mark.parametrize("case", WINDOW, ids=str)
+def test_window_lse_row_by_row(case):
+    """Each row's log-sum-exp within the bound of its own scores."""
+    B, Hq, Hkv, Sq, Skv, D, W, sinks, lens = case
+    q, k, v, n, seen = window_inputs(*case, seed=3)
+    lse = torch.full((B, Hq, Sq), 5.0, device="cuda")
+    ops.attention_window_fwd(q, k, v, W, sinks, kv_len=n, lse=lse)
+    ops.check()
+    _, _, want, _ = U.attention(q, k, v, seen)
+    live = seen.any(-1).expand(B, Hq, Sq)
+    assert torch.isfinite(lse[live]).all() and (lse[~live] == -math.inf).all()
+    # Scores: fp32 sums of D products, off by D 2^-24 of the sum of their sizes; the weights by
+    # 2^-13 (exp2 on the FMA pipe at D = 64, 7.5e-5); the sum, its logarithm and the products
+    # with the maximum by 2^-20 of the value.
+    size = (q.double().abs() @ k.double().abs().repeat_interleave(Hq // Hkv, 1).transpose(2, 3))
+    size = size.masked_fill(~seen, 0.0).amax(-1) / math.sqrt(D)
+    bound = size * D * 2.0 ** -24 + 2.0 ** -13 + 2.0 ** -20 * want.abs()
+    off = ((lse.double() - want).abs() - bound)[live]
+    assert off.numel() == 0 or off.max().item() <= 0
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=str)
 def test_window_bwd(case):
     q, k, v, n, seen = window_inputs(*case, seed=1)
     B, Hq, Hkv, Sq, Skv, D, W, sinks, _ = case
