@@ -230,7 +230,8 @@ struct Cfg {
   static constexpr int kBarOff = kFlagOff + 16;
   // q_full[2] q_empty[2] k_full[K] k_empty[K] v_full[V] v_empty[V]
   // s_ready[3] p_ready[3] p_free[3] pv_done[2] o_full o_empty l_ready[2] drain done o_free
-  static constexpr int kNumBars = 4 + 2 * kKStages + 2 * kVStages + 3 * kSBufs + 2 + 4 + 3;
+  // q_seen[2]
+  static constexpr int kNumBars = 4 + 2 * kKStages + 2 * kVStages + 3 * kSBufs + 2 + 4 + 3 + 2;
   static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kSmemBytes = kTmemSlotOff + 16 + 1024;  // + 1 KiB alignment slack
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA may use");
@@ -505,6 +506,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // may overwrite it).  o_empty stays each CTA's own epilogue -> softmax
   // handshake.
   uint64_t* o_free = done + 1;
+  // The S issuer has seen Q of an item without K/V tiles, by its buffer.  (It has
+  // to see every phase of q_full: one that was skipped could not be told from
+  // the next by its bit.)
+  uint64_t* q_seen = o_free + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kTmemSlotOff);
 
   const uint32_t warp = warp_id();
@@ -554,6 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&l_ready[i], 8);
+      mbar_init(&q_seen[i], 1);
     }
     for (int i = 0; i < kSBufs; ++i) {
       mbar_init(&s_ready[i], 1);
@@ -838,7 +844,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int qb = li & 1;
             const uint32_t qpar = static_cast<uint32_t>(li >> 1) & 1u;
             ++li;
-            if (it.n == 0) continue;
+            if (it.n == 0) {
+              ok = wait3(bar(&q_full[qb]), qpar, dn_a, dn_p, dn_a, dn_p, kSiteQFull);
+              if (ok) mbar_arrive_warp(&q_seen[qb]);
+              continue;
+            }
             ok = wait3(bar(&q_full[qb]), qpar, dn_a, dn_p, dn_a, dn_p, kSiteQFull);
             const uint64_t dq = dq0 + qb * kTile16;
             for (int j = 0; j < it.n && ok; ++j, ++t) {
@@ -863,6 +873,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         } else {
+          uint32_t seen = 0;  // bit of each q_seen barrier's next phase
           for (int r = 0; r < rounds && ok; ++r) {
             const int k = item_at(r);
             if (k >= p.n_items) continue;
@@ -871,9 +882,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (it.n == 0) {
               // No K/V tiles: O stays unwritten (the epilogue stores zeros in Q's
               // buffer, so Q(li) must have landed first).
-              ok = wait3(bar(&q_full[li & 1]), static_cast<uint32_t>(li >> 1) & 1u, bar(o_rd),
-                         oe_par, dn_a, dn_p, kSiteQFull);
+              ok = wait3(bar(&q_seen[li & 1]), (seen >> (li & 1)) & 1u, bar(o_rd), oe_par, dn_a,
+                         dn_p, kSiteQFull);
               if (!ok) break;
+              seen ^= 1u << (li & 1);
               commit_both(o_full);
               ++li;
               continue;

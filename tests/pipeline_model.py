@@ -16,6 +16,7 @@ class Role:
     def __init__(self, pipeline):
         self.p = pipeline
         self.last = None
+        self.done = None  # its last commit's arrival
 
     def wait(self, bar, phase, bit=None):
         """Wait for `phase` of `bar` (-1: none, passed at once) by the bit `bit`."""
@@ -29,10 +30,13 @@ class Role:
         self.last = self.p.event(self.last)
         self.p.arrivals[bar, id(self)].append(self.last)
 
-    def commit(self, bar):
-        """An arrival at some time after this, which nothing else waits for."""
+    def commit(self, bar, in_order=False):
+        """An arrival at some time after this, which nothing else waits for.  in_order: not
+        before those of the role's earlier commits, which end with the same products."""
         self.last = self.p.event(self.last)
-        self.p.arrivals[bar, "async"].append(self.p.event(self.last))
+        done = self.p.event(self.last, self.done if in_order else None)
+        self.done = done
+        self.p.arrivals[bar, "async"].append(done)
 
 
 class Pipeline:
