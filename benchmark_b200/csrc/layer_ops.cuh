@@ -865,7 +865,11 @@ b200_status qk_norm_rope(const b200_tensor* q, const b200_tensor* k, const void*
 }
 
 b200_status qk_norm_rope_bwd_workspace(int B, int S, int D, size_t* bytes) {
-  if (!bytes || B < 1 || S < 1) return fail(B200_EINVAL, "qk_norm_rope_bwd_workspace: bad argument");
+  const char* who = "qk_norm_rope_bwd_workspace";
+  if (!bytes) return fail(B200_EINVAL, "%s: null result", who);
+  if (B < 1 || S < 1) return fail(B200_EINVAL, "%s: invalid shape B=%d S=%d", who, B, S);
+  if (D != 64 && D != 128)
+    return fail(B200_EUNSUPPORTED, "%s: head_dim must be 64 or 128; got D=%d", who, D);
   // The grid never exceeds its CTAs per SM, whatever the shape.
   *bytes = static_cast<size_t>(sm_count()) * b200::rope::kGradCtasPerSm * D * sizeof(float);
   return B200_OK;

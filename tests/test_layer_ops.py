@@ -136,6 +136,17 @@ def test_norm_rope_bwd_refuses():
     assert bwd(dq=T(ss=8)) == 1 and "dq" in _lib.last_error()
 
 
+@pytest.mark.parametrize("B,S,D,status,word", [
+    (2, 16, -1, 2, "head_dim"), (2, 16, 0, 2, "head_dim"), (2, 16, 96, 2, "head_dim"),
+    (2, 0, 128, 1, "shape"), (-1, 16, 128, 1, "shape"),
+])
+def test_norm_rope_bwd_workspace_refuses(B, S, D, status, word):
+    n = ctypes.c_size_t()
+    assert _lib.lib().qk_norm_rope_bwd_workspace(B, S, D, ctypes.byref(n)) == status
+    assert word in _lib.last_error()
+    assert _lib.lib().qk_norm_rope_bwd_workspace(2, 16, 128, None) == 1
+
+
 def prefix(P=4096, B=4, Hq=8, Hkv=2, Sq=1, S=64, D=128, kp=None, vp=None, k=None, o=None, ws=256,
            ws_bytes=1 << 40):
     t = T()
