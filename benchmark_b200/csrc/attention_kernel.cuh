@@ -549,7 +549,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- setup ----
   if constexpr (kForm != kDense) {
-    // Rows past a tile's box stay zero (their scores are computed, and dropped).
+    // Rows past a tile's box start as zeros; later they hold what an earlier item's O
+    // left in the buffer, which may be NaN.  Nothing may depend on them: their scores
+    // are computed, and dropped.
     for (int i = static_cast<int>(threadIdx.x); i < 2 * C::kTileBytes / 16; i += kThreads)
       reinterpret_cast<uint4*>(q_buf)[i] = make_uint4(0u, 0u, 0u, 0u);
     fence_proxy_async_smem();

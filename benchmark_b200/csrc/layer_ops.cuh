@@ -58,9 +58,14 @@ b200_status check_launch(const char* what) {
 }
 
 // Launch on `stream` a kernel that may start while its predecessor there still
-// runs: it waits (pdl_wait) before it touches memory that others use, so only
-// its launch overlaps.  Measured back to back: one token's attention over 1024
-// keys 10.3 -> 7.9 us a call, three requests behind 517 keys 8.2 -> 6.4.
+// runs.  It waits (pdl_wait) before it touches memory that others use, so only
+// its launch overlaps -- but for two kernels that run beside their predecessor
+// (the gradients' query tiles, split_attention_kernel with `overlaps`).  Those
+// read what the predecessor has waited for, and nothing that it writes: each
+// relies on the kernel directly before it calling pdl_wait before
+// pdl_launch_dependents.  Their last CTA ends after the predecessor has, so that
+// what follows them follows both.  Measured back to back: one token's attention
+// over 1024 keys 10.3 -> 7.9 us a call, three requests behind 517 keys 8.2 -> 6.4.
 template <typename... P, typename... A>
 b200_status launch_dependent(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem,
                              cudaStream_t stream, const char* what, A... args) {
@@ -275,9 +280,11 @@ WindowTile window_tile(const WindowShape& s, const b200_tensor* q) {
 }
 
 // A 128-row tile spends about 0.87 us on 128 keys, whatever its rows, and the
-// kernel starts 1.5 us after the 16-row one.  Where items leave SMs idle, their
-// keys are split, four tiles at least to a split; the splits' sums and the
-// kernel that merges them cost 4 us and their bytes.  Measured (us, whole /
+// kernel starts 1.5 us after the 16-row one.  (An item's start and end are not in
+// this: one round of nine tiles is 9.3 us by it and 15.9 measured, with masked
+// tiles, so that it ranks the kernels, and does not say their times.)  Where items
+// leave SMs idle, their keys are split, four tiles at least to a split; the splits'
+// sums and the kernel that merges them cost 4 us and their bytes.  Measured (us, whole /
 // split; B 1, heads 32/8 of 128): 32768 keys, Sq 64: 227 / 43; 8192 keys, Sq 16:
 // 61.0 / 16.2, 256: 62.8 / 43.9, 512: 64.9 / 65.5; window 2048, Sq 64: 22.4 / 16.7;
 // window 1024, Sq 128: 15.9 / 17.2.
@@ -685,6 +692,8 @@ b200_status window_bwd_tiles(const WindowShape& s, const WindowGrads& t, void* w
   p.s1_b = q_b, p.s1_h = q_h, p.s2_b = do_b, p.s2_h = do_h;
   if ((st = launch_bwd_tiles<D, true>({k, v, q[1], dout[1]}, p, s.Hkv, s.Skv, stream)) != B200_OK)
     return st;
+  // Beside the keys' kernel (see launch_dependent): nothing may stand between
+  // the two, and this one reads nothing that that one writes.
   p.out1 = p.out2 = view_of(t.dq);
   p.o1_b = q_b, p.o1_h = q_h, p.o2_b = do_b, p.o2_h = do_h;
   p.s1_b = k_b, p.s1_h = k_h, p.s2_b = v_b, p.s2_h = v_h;
@@ -768,7 +777,8 @@ struct PrefixPlan {
 // 26.0; P 2048, B 8: 16.2 / 14.3, B 16: 17.3 / 21.1; P 32768, B 2: 35.0 / 34.6,
 // B 4: 35.6 / 62.5; D 64, P 8192, B 4: 17.8 / 15.8, B 8: 18.0 / 24.8.  A tile
 // holds whole requests, and the queries' map cannot broadcast; q's strides
-// decide that (null: they do not).
+// decide that (null: they do not).  So requests of more than 128 rows (heads of a
+// kv head x tokens: prompts) go by 16-row tiles, however long the prefix.
 PrefixPlan prefix_plan(const WindowShape& own, int P, const b200_tensor* q) {
   const int64_t rows = static_cast<int64_t>(own.Hq / own.Hkv) * own.Sq;
   const int64_t heads = static_cast<int64_t>(own.B) * own.Hkv;
@@ -782,10 +792,11 @@ PrefixPlan prefix_plan(const WindowShape& own, int P, const b200_tensor* q) {
     const int64_t items = static_cast<int64_t>(own.Hkv) * prefix_tiles(own).count;
     const int64_t kv = (P + b200::attn::kBN - 1) / b200::attn::kBN;
     // Where the requests' own keys are long (4 us at the memory's rate), they
-    // stream through three tenths of the SMs beside the tiles.  Measured (us;
-    // 0 / 20 / 44 / 74 SMs left): 64 requests, heads 64/8, P 16384, up to 1024
-    // keys: 67.9 / 68.1 / 66.3 / 66.5; P 4096: 52.7 / 52.6 / 49.7 / 45.9; 32
-    // requests, P 16384, up to 512: 40.3 / 39.8 / 34.9 / 40.5.
+    // stream through three tenths of the SMs beside the tiles: one share for all,
+    // not the best of each.  Measured (us; 0 / 20 / 44 / 74 SMs left): 64 requests,
+    // heads 64/8, P 16384, up to 1024 keys: 67.9 / 68.1 / 66.3 / 66.5; P 4096:
+    // 52.7 / 52.6 / 49.7 / 45.9; 32 requests, P 16384, up to 512: 40.3 / 39.8 /
+    // 34.9 / 40.5.
     const double own_us = 4.0 * own.B * own.Hkv * static_cast<double>(own.Skv) * own.D / 6.4e6;
     int64_t sms = sm_count();
     if (own_us > 4.0) sms = std::max<int64_t>(1, sms * 7 / 10);
@@ -1062,6 +1073,8 @@ b200_status attention_shared_prefix(const b200_tensor* q, const b200_tensor* k_p
     c.part_b = part_o;
     c.ml_b = part_ml;
     c.nb = plan.prefix_splits;
+    // The requests' own keys run beside the tiles (see launch_dependent):
+    // nothing may be launched between the two.
     p.overlaps = 1;
   } else if (P > 0) {
     p.kp = view_of(k_prefix);

@@ -15,8 +15,9 @@
 // the rotation none.  A warp walks the heads of one token, so that its lanes
 // keep their angles and weights in registers; the next rows are on their way
 // through a ring in shared memory, of which each lane copies and reads its own
-// slots: nothing synchronises the warps.  16384 tokens of 32 + 8 heads of 128:
-// forward 54.6 us (6.1 TB/s), backward 88.4 us (5.7 TB/s).  (With the next rows
+// slots: nothing synchronises the warps.  16384 tokens of 32 + 8 heads of 128,
+// replayed in a graph at full clock: forward 54.3 us (6.2 TB/s), backward 88.3 us
+// (5.7 TB/s); called back to back 59 and 97 us.  (With the next rows
 // in registers instead, one row group ahead: 63.5 and 107 us.  With angles and
 // weights in shared memory for a block of tokens, their reads kept the
 // load/store unit 80 % busy: 77 us forward.)  With few heads a warp's lanes

@@ -20,8 +20,9 @@
 // product), longer than its products: with one buffer of S and dP the chain
 // took 2,050 cycles a step where the products need 1,280 (kKeys).  So S runs
 // steps ahead, and dP alone waits for its one buffer, which is free as soon as
-// it is in the registers.  kKeys steps are 64 queries wide: two accumulators
-// of D columns leave no room for 128.
+// it is in the registers.  kKeys steps are 64 queries wide: at D = 128 two
+// accumulators of D columns leave no room for 128 (at D = 64 they would; the
+// kernel is the same there).
 //
 // Roles: elementwise and epilogue warps (warp w: lanes 32 (w % 4), the w / 4th
 // share of the columns), then a TMA warp, one that issues S and dP and one that

@@ -8,6 +8,9 @@ The attention layer's operators (qk_norm_rope, attention_window_*,
 attention_shared_prefix) take [B, H, S, D] views of any strides with D
 contiguous, on any one device; they run on that device's current stream or on
 `stream`, where their outputs and workspaces are allocated too.
+
+No call records a gradient: outputs have no history, whatever their inputs require.
+The `_bwd` functions are for a torch.autograd.Function of the caller's.
 """
 from __future__ import annotations
 
@@ -198,6 +201,10 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 
     q [B,Hq,Sq,D]; k_prefix/v_prefix [Hkv,P,D]; k/v [B,Hkv,S,D]: each request's own keys
     (any strides, D contiguous) -> o [B,Hq,Sq,D].  Query i of request b sees the whole
-    prefix and its own keys j <= kv_len[b] - Sq + i (int32 [B]; default S)."""
+    prefix and its own keys j <= kv_len[b] - Sq + i (int32 [B]; default S).
+
+    Made for decoding: with Hq / Hkv * Sq above 128 (a prompt) a request reads the prefix
+    again for every 16 of these rows, and attention_window_fwd over caches that hold a copy
+    of the prefix is faster."""
     return _call("attention_shared_prefix", stream, q, k_prefix, v_prefix, k, v, kv_len, out,
                  softmax_scale)

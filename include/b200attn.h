@@ -132,6 +132,18 @@ b200_status attention_fwd_scalar(const void* q, const void* k, const void* v, vo
                                  float softmax_scale, b200_stream_t stream);
 
 /*
+ * The attention layer's operators.  Sums, softmax statistics and norms are held
+ * in fp32.  Rounded to bf16 inside: the weights P of attention before their
+ * product with V, and P and dS before the gradients' last products (what bf16
+ * tensor cores take: a relative 2^-8 of each at most).  At D = 64 a part of the
+ * 128-row tiles' exponentials goes by a polynomial (7.5e-5 relative).
+ * NaN in a key or query gives NaN in each row that meets it, in lse too.  What no
+ * query of the call sees may hold anything.  A row of V (for gradients: of any
+ * input) that some queries of the call see and others do not has to be finite:
+ * it may reach both (0 * NaN).
+ */
+
+/*
  * A [B, H, S, D] bf16 tensor by its strides in elements; D is contiguous.
  * The data is 16-byte aligned and the strides are multiples of 8, so a view
  * of a fused projection's [B, S, heads, D] output, or of a cache with room
@@ -226,8 +238,12 @@ b200_status attention_window_bwd(const b200_tensor* dout, const b200_tensor* q,
 /*
  * Attention of a batch whose requests share a prefix: query i of request b
  * sees all P prefix keys, and of its own keys those at j <= kv_len[b] - Sq + i
- * (kv_len as above, of at most S).  The prefix is read for the whole batch at
- * once, or, where that is little work, for each request through L2.
+ * (kv_len as above, of at most S).  Made for decoding: the prefix is read for the
+ * whole batch at once, or, where that is little work, for each request through
+ * L2.  That holds up to Hq / Hkv * Sq = 128.  With more rows (a prompt) a request
+ * reads the prefix again for every 16 of them: 8 requests of 512 tokens behind
+ * 4096 keys, heads 64/8 of 128, take 3,600 us, attention_window_fwd over caches
+ * that hold a copy of the prefix 520.
  *   q, o: [B, Hq, Sq, D]   k_prefix, v_prefix: [1, Hkv, P, D] (P = 0: ignored)
  *   k, v: [B, Hkv, S, D]   D in {64, 128}
  */
