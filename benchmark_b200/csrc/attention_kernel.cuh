@@ -847,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t qpar = static_cast<uint32_t>(li >> 1) & 1u;
             ++li;
             if (it.n == 0) {
-              ok = wait3(bar(&q_full[qb]), qpar, dn_a, dn_p, dn_a, dn_p, kSiteQFull);
+              ok = warp_wait(&q_full[qb], qpar, kSiteQFull);
               if (ok) mbar_arrive_warp(&q_seen[qb]);
               continue;
             }
@@ -884,8 +884,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (it.n == 0) {
               // No K/V tiles: O stays unwritten (the epilogue stores zeros in Q's
               // buffer, so Q(li) must have landed first).
-              ok = wait3(bar(&q_seen[li & 1]), (seen >> (li & 1)) & 1u, bar(o_rd), oe_par, dn_a,
-                         dn_p, kSiteQFull);
+              ok = warp_wait(&q_seen[li & 1], (seen >> (li & 1)) & 1u, kSiteQFull) &&
+                   warp_wait(o_rd, oe_par, kSiteOEmpty);
               if (!ok) break;
               seen ^= 1u << (li & 1);
               commit_both(o_full);

@@ -90,10 +90,11 @@ ITEMS = [[3] * 8, [1] * 10, [2, 1, 4, 1, 1], [0] * 6, [0, 0, 2, 0, 0, 3], [3, 0,
 def test_every_wait_is_decided_by_its_phase_bit(items, D):
     # What the model takes from the source: the S issuer waits for each item's Q first.
     flat = re.sub(r"\s+", " ", SOURCE)
-    wait = "ok = wait3(bar(&q_full[qb]), qpar, dn_a, dn_p, dn_a, dn_p, kSiteQFull);"
-    for text in ("++li; if (it.n == 0) { " + wait + " if (ok) mbar_arrive_warp(&q_seen[qb]); "
-                 "continue; } " + wait,
-                 "wait3(bar(&q_seen[li & 1]), (seen >> (li & 1)) & 1u, bar(o_rd), oe_par,",
+    for text in ("++li; if (it.n == 0) { ok = warp_wait(&q_full[qb], qpar, kSiteQFull); "
+                 "if (ok) mbar_arrive_warp(&q_seen[qb]); continue; } "
+                 "ok = wait3(bar(&q_full[qb]), qpar, dn_a, dn_p, dn_a, dn_p, kSiteQFull);",
+                 "ok = warp_wait(&q_seen[li & 1], (seen >> (li & 1)) & 1u, kSiteQFull) && "
+                 "warp_wait(o_rd, oe_par, kSiteOEmpty);",
                  "commit_both(&pv_done[t & 1]); commit_lead(&p_free[sb]);"):
         assert text in flat
     assert faults(items, D) == []
