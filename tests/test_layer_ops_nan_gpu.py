@@ -81,3 +81,19 @@ def test_prefix_with_nan(B, Hq, Hkv, Sq, P, S, D):
         ops.check()
         hit = torch.arange(Hq, device="cuda") // (Hq // Hkv) == Hkv // 2
         assert o[:, hit].isnan().all() and torch.equal(o[:, ~hit], want[:, ~hit])
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=str)
+def test_queries_that_hold_nan(case):
+    B, Hq, Hkv, Sq, Skv, D, W, sinks = case
+    q, k, v, clean, _ = inputs(case, 3)
+    hit = torch.rand((B, Hq, Sq), generator=torch.Generator(device="cuda").manual_seed(3),
+                     device="cuda") < 0.2
+    x = q.clone()
+    x[..., 5] = torch.where(hit, torch.tensor(math.nan, dtype=BF16, device="cuda"), x[..., 5])
+    lse, want_lse = (torch.empty((B, Hq, Sq), device="cuda") for _ in range(2))
+    o = ops.attention_window_fwd(x, clean, v, W, sinks, lse=lse)
+    want = ops.attention_window_fwd(q, clean, v, W, sinks, lse=want_lse)
+    ops.check()
+    assert o[hit].isnan().all() and lse[hit].isnan().all()
+    assert torch.equal(o[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
